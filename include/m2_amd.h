@@ -374,6 +374,37 @@ int m2_encoder_layers_taps_fwd(const m2_layer_params* layers, int nlayers, const
                                int filters_per_mixer, const void* h16, const float* h_channel_major, float* const* out_f32,
                                void* workspace, int B, int L, int d, int intermediate, int nblocks, float eps, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Products of few rows with weights in 4 bits (for the masked-LM head's two products, bert/src/bert_layers.py:862-877,1027-1052).
+ *   y (M, N) = act(x W^T + bias),  W[n, k] = (q - 8) * s,  q in 0 .. 15,  s bf16, one for each `group` (32, 64 or 128) values of a row
+ * `weight` (m2_int4_weight_bytes, 0: unsupported; 16-byte aligned) holds tiles of 16 rows by 128 columns, all tiles of 16 rows behind one another:
+ * 64 lanes times 16 bytes, lane 16 * (k / 8 % 4) + n % 16, with one 32-bit word for each of four steps of 32 columns, value j = k % 8 at bit
+ * 16 * (j % 2) + 4 * (j / 2); then 16 rows times 128 / group scales.  Rows and columns beyond N and K hold q = 8 and s = 0.
+ * x: M rows of K values, `x_row` values apart, fp32 or bf16; y of the same type, dense; bias (N) fp32 or NULL; gelu: 0 none, 1 erf-GELU. */
+size_t m2_int4_weight_bytes(int N, int K, int group);
+int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, int M, int N, int K, int group,
+                       int gelu, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Log probabilities of given tokens, entropies and the most likely alternatives from logits, and their gradient (the loss behind the
+ * masked-LM head, bert/src/bert_layers.py:1070-1318, is the mean of the first).
+ * logits: `rows` rows of V values, fp32 or bf16, row r at (r / inner) * outer_stride + (r % inner) * row_stride.  z = the logits where `allowed`
+ * (bytes, rows allowed_row apart, 0: one list of V for all rows; NULL: all) is not 0, -inf elsewhere.
+ *   logprobs[r]    z[token] - lse; 0 for ignore_index, NaN for other tokens outside 0 .. V - 1 (tokens NULL: not written)
+ *   entropy[r]     -sum p log p
+ *   top_*[r, k]    the top_k (0 .. 32, at most V) largest z - lse, equal ones by id; id -1 and -inf behind the last finite z
+ *   stats[r, 2]    for the gradient: max z, log sum exp(z - max z)
+ * A row of -inf: logprob -inf, entropy 0, gradient 0.  A NaN or +inf among a row's z: NaN throughout, ids -1.
+ * The gradient takes g_* fp32 (NULL: zero), g_logprobs and g_entropy with a stride (0: one value for all rows), g_top dense, and writes grad, of the
+ * logits' type, rows grad_row apart; positions with z = -inf get 0. */
+int m2_token_scores_fwd(const void* logits, int inner, long outer_stride, long row_stride, const long long* tokens, long long ignore_index,
+                        const unsigned char* allowed, long allowed_row, float* logprobs, float* entropy, float* stats, long long* top_ids,
+                        float* top_logprobs, long rows, int V, int top_k, int dtype, void* stream);
+int m2_token_scores_bwd(const void* logits, int inner, long outer_stride, long row_stride, const long long* tokens, long long ignore_index,
+                        const unsigned char* allowed, long allowed_row, const float* entropy, const float* stats, const long long* top_ids,
+                        const float* g_logprobs, long g_logprobs_stride, const float* g_entropy, long g_entropy_stride, const float* g_top,
+                        void* grad, long grad_row, long rows, int V, int top_k, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
