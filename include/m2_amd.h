@@ -394,12 +394,14 @@ int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const floa
  *   entropy[r]     -sum p log p
  *   top_*[r, k]    the top_k (0 .. 32, at most V) largest z - lse, equal ones by id; id -1 and -inf behind the last finite z
  *   stats[r, 2]    for the gradient: max z, log sum exp(z - max z)
+ * `workspace`: m2_token_scores_workspace_bytes (0: NULL does).
  * A row of -inf: logprob -inf, entropy 0, gradient 0.  A NaN or +inf among a row's z: NaN throughout, ids -1.
  * The gradient takes g_* fp32 (NULL: zero), g_logprobs and g_entropy with a stride (0: one value for all rows), g_top dense, and writes grad, of the
  * logits' type, rows grad_row apart; positions with z = -inf get 0. */
+size_t m2_token_scores_workspace_bytes(long rows, int V, int dtype);
 int m2_token_scores_fwd(const void* logits, int inner, long outer_stride, long row_stride, const long long* tokens, long long ignore_index,
                         const unsigned char* allowed, long allowed_row, float* logprobs, float* entropy, float* stats, long long* top_ids,
-                        float* top_logprobs, long rows, int V, int top_k, int dtype, void* stream);
+                        float* top_logprobs, void* workspace, long rows, int V, int top_k, int dtype, void* stream);
 int m2_token_scores_bwd(const void* logits, int inner, long outer_stride, long row_stride, const long long* tokens, long long ignore_index,
                         const unsigned char* allowed, long allowed_row, const float* entropy, const float* stats, const long long* top_ids,
                         const float* g_logprobs, long g_logprobs_stride, const float* g_entropy, long g_entropy_stride, const float* g_top,

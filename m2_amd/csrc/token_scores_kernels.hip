@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "m2_internal.h"
 
 namespace m2 {
@@ -105,6 +107,22 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return {m, a.s + b.s, a.t + b.t};
 }
 
+// The sums of LANES neighbours, in all of them.
+template <int LANES>
+__device__ __forceinline__ Sums join_lanes(Sums a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  rescale(a, m);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const float s = __shfl_xor(a.s, o), t = __shfl_xor(a.t, o);
+    a.s += s;
+    a.t += t;
+  }
+  return a;
+}
+
 template <int N>
 __device__ __forceinline__ void add_values(Sums& a, const float (&z)[N]) {
   float c = z[0];
@@ -123,85 +141,298 @@ __device__ __forceinline__ void add_values(Sums& a, const float (&z)[N]) {
 // (value, id) before (other, other_id): larger value first, then the lower id.
 __device__ __forceinline__ bool before(float v, int id, float w, int wid) { return v > w || (v == w && id < wid); }
 
-template <typename T, bool MASK>
-__global__ __launch_bounds__(256) void token_scores_kernel(LogitRows in, const long long* __restrict__ tokens, long long ignore_index,
-                                                           float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ stats,
-                                                           long long* __restrict__ top_ids, float* __restrict__ top_logprobs, long rows, int V, int top_k) {
-  constexpr int N = Row<T>::N;
-  __shared__ float part_m[4], part_s[4], part_t[4];
-  __shared__ float best_v[4];
-  __shared__ int best_i[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const char* x = row_of<T>(in, r);
-    const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
-    const int nvec = V / N;
-    Sums mine;
-    for (int i = tid; i < nvec; i += 256) {
-      float z[N];
-      Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
-      if (MASK) Row<T>::masks(a + (long)i * N, z);
-      add_values<N>(mine, z);
-    }
-    if (nvec * N + tid < V) {
-      const float z[1] = {value_at<T, MASK>(x, a, nvec * N + tid)};
-      add_values<1>(mine, z);
-    }
-    for (int o = 32; o > 0; o >>= 1) mine = join(mine, Sums{__shfl_xor(mine.m, o), __shfl_xor(mine.s, o), __shfl_xor(mine.t, o)});
-    if (lane == 0) part_m[wave] = mine.m, part_s[wave] = mine.s, part_t[wave] = mine.t;
-    __syncthreads();
-    const auto part = [&](int w) { return Sums{part_m[w], part_s[w], part_t[w]}; };
-    const Sums all = join(join(part(0), part(1)), join(part(2), part(3)));
-    const bool empty = all.s == 0.f;
-    const float logs = empty ? 0.f : logf(all.s);
-    const bool broken = all.s != all.s;          // a NaN or +inf among the values
-    if (tid == 0) {
-      if (tokens) {
-        const long long t = tokens[r];
-        float lp = 0.f;
-        if (t != ignore_index) {
-          if (t < 0 || t >= V) lp = __builtin_nanf("");
-          else {
-            const float z = value_at<T, MASK>(x, a, t);
-            lp = broken ? __builtin_nanf("") : z == kNegInf ? kNegInf : (z - all.m) - logs;
-          }
-        }
-        logprobs[r] = lp;
-      }
-      entropy[r] = empty ? 0.f : logs - all.t / all.s;
-      stats[2 * r] = broken ? __builtin_nanf("") : all.m;
-      stats[2 * r + 1] = logs;
-    }
-    // the alternatives one after the other: the first of those behind the last one
+// The vectors [first, end) of a row, and its last V % N values where this is the last part.
+struct Span {
+  int first, end, tail, V;      // tail: index of the first value behind the last vector
+};
+
+// Largest values of a part of a row, most likely first, in v and id (empty places: -inf, -1).  Called by the whole workgroup.
+//
+// The pass over the row leaves every thread with the largest value it has met.  Lane l of all waves is group l, of 64: the k-th largest of the groups' maxima is
+// a lower bound b of the k-th largest value, and values above b lie in the fewer than k groups whose maximum is larger, values equal to b in
+// those and the ones where it is equal.  Those groups are read again (out of the cache: about k / 64 of the part) and what reaches b is put in order by
+// counting.  Values equal to b may be any number (a row of one value): where they do not fit, they are taken from the front, reading in order.
+// Where the values above b do not fit (all large values of a row in one group), the alternatives are looked for one after the other.
+template <typename T, bool MASK, int THREADS>
+struct Top {
+  static constexpr int kRoom = 512, kWaves = THREADS / 64;
+  float v[kMaxTop];
+  int id[kMaxTop];
+  float most[kWaves][64];
+  float above_v[kRoom];
+  int above_i[kRoom], equal_i[kRoom];
+  int above, equal, count[kWaves], list[64];
+
+  __device__ void one_by_one(const char* x, const unsigned char* a, const Span& p, int k) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float last_v = __builtin_inff();
     int last_i = -1;
-    for (int k = 0; k < top_k; ++k) {
+    for (int n = 0; n < k; ++n) {
       float bv = kNegInf;
       int bi = 0x7fffffff;
-      if (!broken)
-        for (int j = tid; j < V; j += 256) {
-          const float v = value_at<T, MASK>(x, a, j);
-          if (before(last_v, last_i, v, j) && before(v, j, bv, bi)) bv = v, bi = j;
-        }
+      const auto see = [&](int j) {
+        const float z = value_at<T, MASK>(x, a, j);
+        if (before(last_v, last_i, z, j) && before(z, j, bv, bi)) bv = z, bi = j;
+      };
+      for (int j = p.first * Row<T>::N + tid; j < p.end * Row<T>::N; j += THREADS) see(j);
+      if (p.tail + tid < p.V) see(p.tail + tid);
       for (int o = 32; o > 0; o >>= 1) {
         const float ov = __shfl_xor(bv, o);
         const int oi = __shfl_xor(bi, o);
         if (before(ov, oi, bv, bi)) bv = ov, bi = oi;
       }
-      if (lane == 0) best_v[wave] = bv, best_i[wave] = bi;
+      if (lane == 0) most[0][wave] = bv, count[wave] = bi;
       __syncthreads();
-      for (int w = 0; w < 4; ++w)
-        if (before(best_v[w], best_i[w], bv, bi)) bv = best_v[w], bi = best_i[w];
+      for (int w = 0; w < kWaves; ++w)
+        if (before(most[0][w], count[w], bv, bi)) bv = most[0][w], bi = count[w];
       __syncthreads();
-      if (tid == 0) {
-        const bool none = broken || bv == kNegInf;
-        top_ids[r * top_k + k] = none ? -1 : bi;
-        top_logprobs[r * top_k + k] = broken ? __builtin_nanf("") : none ? kNegInf : (bv - all.m) - logs;
-      }
+      if (tid == 0) v[n] = bv, id[n] = bv == kNegInf ? -1 : bi;
       last_v = bv;
       last_i = bi;
     }
+    __syncthreads();
+  }
+
+  // The first `want` places that hold `b`, which there are.
+  __device__ void first_equal(const char* x, const unsigned char* a, const Span& p, float b, int want) {
+    constexpr int N = Row<T>::N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int found = 0;
+    const auto take = [&](const float* z, int n, int j) {      // n values from place j on; the threads' places ascend
+      int mine = 0;
+      for (int i = 0; i < n; ++i) mine += z[i] == b;
+      int upto = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(upto, o);
+        if (lane >= o) upto += u;
+      }
+      if (lane == 63) count[wave] = upto;
+      __syncthreads();
+      int at = found + upto - mine;
+      for (int w = 0; w < wave; ++w) at += count[w];
+      for (int i = 0; i < n; ++i)
+        if (z[i] == b) {
+          if (at < kRoom) equal_i[at] = j + i;
+          ++at;
+        }
+      for (int w = 0; w < kWaves; ++w) found += count[w];
+      __syncthreads();
+    };
+    for (int base = p.first; base < p.end && found < want; base += THREADS) {
+      float z[N] = {};
+      const int i = base + tid, n = i < p.end ? N : 0;
+      if (n) {
+        Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
+        if (MASK) Row<T>::masks(a + (long)i * N, z);
+      }
+      take(z, n, i * N);
+    }
+    if (found < want) {
+      const bool in = p.tail + tid < p.V;
+      const float z = in ? value_at<T, MASK>(x, a, p.tail + tid) : 0.f;
+      take(&z, in, p.tail + tid);
+    }
+  }
+
+  __device__ void find(const char* x, const unsigned char* a, const Span& p, float mine, int k) {
+    constexpr int N = Row<T>::N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    most[wave][lane] = mine;
+    if (tid == 0) above = equal = 0;
+    if (tid < k) v[tid] = kNegInf, id[tid] = -1;
+    __syncthreads();
+    float group = most[0][lane];
+    for (int w = 1; w < kWaves; ++w) group = fmaxf(group, most[w][lane]);
+    int larger = 0, same = 0;
+#pragma unroll 16
+    for (int l = 0; l < 64; ++l) {
+      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), l));
+      larger += o > group;
+      same += o == group;
+    }
+    const unsigned long long kth = __ballot(larger < k && larger + same >= k);      // never empty: k <= 64
+    const float b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), __builtin_ctzll(kth)));
+    const unsigned long long wanted = __ballot(group >= b && group > kNegInf);
+    const int groups = __builtin_popcountll(wanted);
+    if (groups == 0) return;      // nothing but -inf (all waves see the same groups)
+    const int nth = __builtin_popcountll(wanted & ((1ull << lane) - 1));
+    if (wave == 0 && (wanted >> lane & 1)) list[nth] = lane;
+    __syncthreads();
+    const auto see = [&](float z, int j) {
+      if (z > b) {
+        const int at = atomicAdd(&above, 1);
+        if (at < kRoom) above_v[at] = z, above_i[at] = j;
+      } else if (z == b && b > kNegInf) {
+        const int at = atomicAdd(&equal, 1);
+        if (at < kRoom) equal_i[at] = j;
+      }
+    };
+    const int each = (p.end - p.first + 63) / 64;      // vectors of a group
+    for (int u = tid; u < groups * each; u += THREADS) {
+      const int i = p.first + 64 * (u / groups) + list[u % groups];
+      if (i < p.end) {
+        float z[N];
+        Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
+        if (MASK) Row<T>::masks(a + (long)i * N, z);
+#pragma unroll
+        for (int n = 0; n < N; ++n) see(z[n], i * N + n);
+      }
+    }
+    if (p.tail + tid < p.V && (wanted >> lane & 1)) see(value_at<T, MASK>(x, a, p.tail + tid), p.tail + tid);
+    __syncthreads();
+    const int na = above;
+    int ne = equal;
+    __syncthreads();
+    if (na > kRoom) return one_by_one(x, a, p, k);
+    if (na < k && ne > kRoom) {
+      first_equal(x, a, p, b, k - na);
+      __syncthreads();
+      ne = k - na;
+    }
+    for (int i = tid; i < na; i += THREADS) {
+      int rank = 0;
+      for (int j = 0; j < na; ++j) rank += before(above_v[j], above_i[j], above_v[i], above_i[i]);
+      if (rank < k) v[rank] = above_v[i], id[rank] = above_i[i];
+    }
+    if (na < k)
+      for (int i = tid; i < ne; i += THREADS) {
+        int rank = na;
+        for (int j = 0; j < ne; ++j) rank += equal_i[j] < equal_i[i];
+        if (rank < k) v[rank] = b, id[rank] = equal_i[i];
+      }
+    __syncthreads();
+  }
+};
+
+// What is said of each row; see m2_amd.h.
+struct RowScores {
+  const long long* tokens;
+  long long ignore_index;
+  float *logprobs, *entropy, *stats;
+  long long* top_ids;
+  float* top_logprobs;
+};
+
+constexpr int kMaxParts = 32;
+
+struct PartScores {
+  Sums sums;
+  float v[kMaxTop];
+  int id[kMaxTop];
+};
+
+template <typename T, bool MASK>
+__device__ __forceinline__ void finish(const LogitRows& in, const RowScores& out, long r, int V, int top_k, const char* x, const unsigned char* a, const Sums& all,
+                                       const float* v, const int* id) {
+  const int tid = threadIdx.x;
+  const bool empty = all.s == 0.f, broken = all.s != all.s;      // broken: a NaN or +inf among the values
+  const float logs = empty ? 0.f : logf(all.s), nan = __builtin_nanf("");
+  if (tid == 0) {
+    if (out.tokens) {
+      const long long t = out.tokens[r];
+      float lp = 0.f;
+      if (t != out.ignore_index) {
+        if (t < 0 || t >= V) lp = nan;
+        else {
+          const float z = value_at<T, MASK>(x, a, t);
+          lp = broken ? nan : z == kNegInf ? kNegInf : (z - all.m) - logs;
+        }
+      }
+      out.logprobs[r] = lp;
+    }
+    out.entropy[r] = empty ? 0.f : logs - all.t / all.s;
+    out.stats[2 * r] = broken ? nan : all.m;
+    out.stats[2 * r + 1] = logs;
+  }
+  if (tid < top_k) {
+    const int at = broken ? -1 : id[tid];
+    out.top_ids[r * top_k + tid] = at;
+    out.top_logprobs[r * top_k + tid] = broken ? nan : at < 0 ? kNegInf : (v[tid] - all.m) - logs;
+  }
+}
+
+// One workgroup a row, or a part of one where `parts` > 1: then what it found goes to `work` and token_scores_join_kernel puts the parts together.
+template <typename T, bool MASK, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, RowScores out, long rows, int V, int top_k, int parts, PartScores* __restrict__ work) {
+  constexpr int N = Row<T>::N, kWaves = THREADS / 64, kAhead = 4;
+  __shared__ float part_m[kWaves], part_s[kWaves], part_t[kWaves];
+  __shared__ Top<T, MASK, THREADS> top;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int nvec = V / N, each = (nvec + parts - 1) / parts;
+  for (long b = blockIdx.x; b < rows * parts; b += gridDim.x) {
+    const long r = b / parts;
+    const int part = (int)(b % parts);
+    const char* x = row_of<T>(in, r);
+    const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
+    const Span p = {min(part * each, nvec), min((part + 1) * each, nvec), part == parts - 1 ? nvec * N : V, V};
+    Sums mine;
+    int i = p.first + tid;
+    for (; i + (kAhead - 1) * THREADS < p.end; i += kAhead * THREADS) {
+      u32x4_any q[kAhead];
+      float z[kAhead * N];
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) q[c] = *reinterpret_cast<const u32x4_any*>(x + (long)(i + c * THREADS) * 16);
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) {
+        float (&zc)[N] = *reinterpret_cast<float (*)[N]>(z + c * N);
+        Row<T>::unpack(q[c], zc);
+        if (MASK) Row<T>::masks(a + (long)(i + c * THREADS) * N, zc);
+      }
+      add_values<kAhead * N>(mine, z);
+    }
+    for (; i < p.end; i += THREADS) {
+      float z[N];
+      Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
+      if (MASK) Row<T>::masks(a + (long)i * N, z);
+      add_values<N>(mine, z);
+    }
+    if (p.tail + tid < V) {
+      const float z[1] = {value_at<T, MASK>(x, a, p.tail + tid)};
+      add_values<1>(mine, z);
+    }
+    const float most = mine.m;
+    mine = join_lanes<64>(mine);
+    if (lane == 0) part_m[wave] = mine.m, part_s[wave] = mine.s, part_t[wave] = mine.t;
+    __syncthreads();
+    const int w = lane % kWaves;
+    const Sums all = join_lanes<kWaves>(Sums{part_m[w], part_s[w], part_t[w]});
+    if (top_k && all.s == all.s) top.find(x, a, p, most, top_k);
+    if (parts > 1) {
+      PartScores& to = work[b];
+      if (tid == 0) to.sums = all;
+      if (tid < top_k) to.v[tid] = top.v[tid], to.id[tid] = top.id[tid];
+    } else {
+      finish<T, MASK>(in, out, r, V, top_k, x, a, all, top.v, top.id);
+    }
     __syncthreads();      // the row's shared values have been read
+  }
+}
+
+// The parts of a row, a workgroup each: the largest of all parts' largest, in order, by counting.
+template <typename T, bool MASK>
+__global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, RowScores out, long rows, int V, int top_k, int parts, const PartScores* __restrict__ work) {
+  __shared__ float v[kMaxParts * kMaxTop], best_v[kMaxTop];
+  __shared__ int id[kMaxParts * kMaxTop], best_i[kMaxTop];
+  const int tid = threadIdx.x;
+  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
+    const PartScores* from = work + r * parts;
+    Sums all = from[0].sums;
+    for (int p = 1; p < parts; ++p) all = join(all, from[p].sums);
+    if (top_k && all.s == all.s) {
+      const int n = parts * top_k;
+      for (int i = tid; i < n; i += 256) v[i] = from[i / top_k].v[i % top_k], id[i] = from[i / top_k].id[i % top_k];
+      if (tid < top_k) best_v[tid] = kNegInf, best_i[tid] = -1;
+      __syncthreads();
+      for (int i = tid; i < n; i += 256) {
+        if (id[i] < 0) continue;
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += id[j] >= 0 && before(v[j], id[j], v[i], id[i]);
+        if (rank < top_k) best_v[rank] = v[i], best_i[rank] = id[i];
+      }
+      __syncthreads();
+    }
+    finish<T, MASK>(in, out, r, V, top_k, row_of<T>(in, r), MASK ? in.allowed + r * in.allowed_row : nullptr, all, best_v, best_i);
+    __syncthreads();
   }
 }
 
@@ -298,20 +529,45 @@ static int check_rows(const char* who, const void* logits, int inner, long outer
 
 using namespace m2;
 
+// Workgroups a row: a part should keep a workgroup of 1024 threads busy for a few vectors each, and there is no use for more parts than fill the chip.
+static int parts_of(long rows, int V, int dtype) {
+  const long vectors = V / (dtype == M2_DTYPE_F32 ? 4 : 8);
+  long parts = vectors / 4096;
+  if (parts > 512 / rows) parts = 512 / rows;
+  return parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : (int)parts;
+}
+
+extern "C" size_t m2_token_scores_workspace_bytes(long rows, int V, int dtype) {
+  if (rows <= 0 || V <= 0) return 0;
+  const int parts = parts_of(rows, V, dtype);
+  return parts > 1 ? (size_t)rows * parts * sizeof(PartScores) : 0;
+}
+
 extern "C" int m2_token_scores_fwd(const void* logits, int inner, long outer_stride, long row_stride, const long long* tokens, long long ignore_index,
                                    const unsigned char* allowed, long allowed_row, float* logprobs, float* entropy, float* stats, long long* top_ids,
-                                   float* top_logprobs, long rows, int V, int top_k, int dtype, void* stream) {
+                                   float* top_logprobs, void* workspace, long rows, int V, int top_k, int dtype, void* stream) {
   const char* who = "m2_token_scores_fwd";
   if (int rc = check_rows(who, logits, inner, outer_stride, row_stride, allowed, allowed_row, rows, V, top_k, dtype)) return rc;
   if (!entropy || !stats || (tokens && !logprobs) || (top_k && (!top_ids || !top_logprobs))) return set_error(M2_ERR_ARG, "%s: null pointer", who);
+  const int parts = parts_of(rows, V, dtype);
+  if (parts > 1 && (!workspace || (uintptr_t)workspace % 4)) return set_error(M2_ERR_ARG, "%s: rows=%ld V=%d need a workspace, aligned to 4 bytes", who, rows, V);
   const LogitRows in = {logits, outer_stride, row_stride, inner, allowed, allowed_row};
+  const RowScores out = {tokens, ignore_index, logprobs, entropy, stats, top_ids, top_logprobs};
   hipStream_t st = (hipStream_t)stream;
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows < kMaxGrid ? rows : kMaxGrid)), dim3(256), 0, st, in, tokens, ignore_index, logprobs, entropy, stats, top_ids, top_logprobs,
-                       rows, V, top_k);
+  const long blocks = rows * parts < kMaxGrid ? rows * parts : kMaxGrid;
+  const auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, in, out, rows, V, top_k, parts, (PartScores*)workspace);
   };
-  if (dtype == M2_DTYPE_F32) allowed ? go(token_scores_kernel<float, true>) : go(token_scores_kernel<float, false>);
-  else allowed ? go(token_scores_kernel<uint16_t, true>) : go(token_scores_kernel<uint16_t, false>);
+  const auto pick = [&](auto* t, auto masked) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    constexpr bool M = decltype(masked)::value;
+    if (blocks <= 512) go(token_scores_kernel<T, M, 1024>, 1024);
+    else go(token_scores_kernel<T, M, 256>, 256);
+    if (parts > 1)
+      hipLaunchKernelGGL((token_scores_join_kernel<T, M>), dim3((unsigned)rows), dim3(256), 0, st, in, out, rows, V, top_k, parts, (const PartScores*)workspace);
+  };
+  const auto type = [&](auto* t) { allowed ? pick(t, std::true_type{}) : pick(t, std::false_type{}); };
+  dtype == M2_DTYPE_F32 ? type((float*)nullptr) : type((uint16_t*)nullptr);
   return check_launch("token_scores");
 }
 

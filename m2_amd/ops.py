@@ -870,9 +870,11 @@ def token_scores(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: 
         top = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
     if rows:
         x, inner, outer, row = _rows_apart(logits)
+        nbytes = lib.m2_token_scores_workspace_bytes(rows, V, code)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _on_device(x):
             check(lib.m2_token_scores_fwd(x.data_ptr(), inner, outer, row, _ptr(tokens), ignore_index, _ptr(allowed), allowed_row, _ptr(lp), h.data_ptr(),
-                                          stats.data_ptr(), _ptr(ids), _ptr(top), rows, V, top_k, code, _stream()))
+                                          stats.data_ptr(), _ptr(ids), _ptr(top), _ptr(workspace), rows, V, top_k, code, _stream()))
     return lp, h, stats, ids, top
 
 

@@ -220,6 +220,13 @@ def test_the_largest_in_few_places(gpu, dtype, V):
         x[0, at] += 20
         x[1, at] = 30 + (at.float() * 37 % 11).to(gpu)
         compare(x.to(dtype), None, 32)
+    each = torch.arange(V, device=gpu)
+    for group in (each // 8 % 64 == 3, each // 4 % 64 == 60, each // 8 % 256 == 255, each % 512 < 30):      # hundreds in one of the places that share a maximum
+        x = torch.randn(2, V, generator=torch.Generator().manual_seed(9)).to(gpu)
+        x[0, group] += 20
+        x[1, group] = 30 + (each[group].float() * 37 % 11)
+        compare(x.to(dtype), None, 32)
+        compare(x.to(dtype), None, 3)
 
 
 def test_tokens_that_are_none(gpu):
@@ -279,7 +286,7 @@ def test_many_rows_and_nothing_behind_them(gpu):
     t = _tokens(gpu, (rows,), V)
     room = [torch.full((rows + 2,), 7.0, device=gpu), torch.full((rows + 2,), 7.0, device=gpu), torch.full((2 * rows + 2,), 7.0, device=gpu),
             torch.full((rows * k + 2,), 7, dtype=torch.int64, device=gpu), torch.full((rows * k + 2,), 7.0, device=gpu)]
-    check(lib.m2_token_scores_fwd(x.data_ptr(), rows, 0, V, t.data_ptr(), -100, None, 0, *[r.data_ptr() + r.element_size() for r in room], rows, V, k, 1, ops._stream()))
+    check(lib.m2_token_scores_fwd(x.data_ptr(), rows, 0, V, t.data_ptr(), -100, None, 0, *[r.data_ptr() + r.element_size() for r in room], None, rows, V, k, 1, ops._stream()))
     grad = torch.full((rows * (V + 4) + 8,), 7.0, dtype=torch.bfloat16, device=gpu)
     g = [v.contiguous() for v in _grads(gpu, (rows,), k)]
     check(lib.m2_token_scores_bwd(x.data_ptr(), rows, 0, V, t.data_ptr(), -100, None, 0, room[1].data_ptr() + 4, room[2].data_ptr() + 4, room[3].data_ptr() + 8,

@@ -89,7 +89,7 @@ def test_entry_points_refuse_before_a_launch():
     assert linear(bias=ctypes.c_void_p(4098)) == -2
 
     def fwd(x=p, inner=1, outer=0, row=0, tokens=None, allowed=None, a_row=0, lp=None, h=p, stats=p, ids=None, top=None, rows=1, V=8, k=0, dtype=1):
-        return lib.m2_token_scores_fwd(x, inner, outer, row, tokens, -100, allowed, a_row, lp, h, stats, ids, top, rows, V, k, dtype, None)
+        return lib.m2_token_scores_fwd(x, inner, outer, row, tokens, -100, allowed, a_row, lp, h, stats, ids, top, None, rows, V, k, dtype, None)
 
     assert fwd(x=None) == fwd(h=None) == fwd(stats=None) == fwd(tokens=p) == fwd(k=1) == fwd(k=1, ids=p) == -1
     assert fwd(rows=0) == fwd(V=0) == fwd(inner=0) == fwd(outer=-1) == fwd(row=-1) == fwd(dtype=2) == fwd(allowed=p, a_row=7) == -1
