@@ -17,14 +17,14 @@ namespace m2 {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxTop = 32;
-constexpr long kMaxGrid = 1 << 20;      // workgroups of a launch; what is left of the rows they take in turn
+constexpr long kMaxGrid = 1 << 21;      // workgroups of a launch (a grid holds below 2^32 threads)
 constexpr float kNegInf = -__builtin_inff();
 
-// The rows of logits: row r starts (r / inner) * outer + (r % inner) * row values behind the first.
+// The rows of logits: row r starts (r / inner) * outer + (r % inner) * row values behind the first (inner 0: all rows are one group).
 struct LogitRows {
   const void* x;
   long outer, row;
-  int inner;
+  uint32_t inner;
   const unsigned char* allowed;      // or null: all
   long allowed_row;                  // 0: one list for all rows
 };
@@ -45,11 +45,6 @@ template <> struct Row<float> {
     return u32x4_any{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
   }
   static __device__ __forceinline__ void put(void* p, long i, float f) { reinterpret_cast<float*>(p)[i] = f; }
-  static __device__ __forceinline__ void masks(const unsigned char* a, float (&f)[4]) {
-    const uint32_t b = *reinterpret_cast<const u32_any*>(a);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = (b >> (8 * i)) & 0xff ? f[i] : kNegInf;
-  }
 };
 template <> struct Row<uint16_t> {
   static constexpr int N = 8;
@@ -65,17 +60,34 @@ template <> struct Row<uint16_t> {
     return u32x4_any{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
   }
   static __device__ __forceinline__ void put(void* p, long i, float f) { reinterpret_cast<uint16_t*>(p)[i] = f32_to_bf16(f); }
-  static __device__ __forceinline__ void masks(const unsigned char* a, float (&f)[8]) {
-    const u32x2_any b = *reinterpret_cast<const u32x2_any*>(a);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (b[i / 4] >> (8 * (i % 4))) & 0xff ? f[i] : kNegInf;
-  }
 };
 
 template <typename T>
-__device__ __forceinline__ const char* row_of(const LogitRows& in, long r) {
-  return reinterpret_cast<const char*>(in.x) + ((r / in.inner) * in.outer + (r % in.inner) * in.row) * (long)sizeof(T);
+__device__ __forceinline__ const char* row_of(const LogitRows& in, uint32_t r) {
+  const uint32_t group = in.inner ? r / in.inner : 0, at = in.inner ? r % in.inner : r;
+  return reinterpret_cast<const char*>(in.x) + (group * in.outer + at * in.row) * (long)sizeof(T);
 }
+
+// Vector i of a row and what is allowed of it.  Its offset is below 2^32 (V <= 2^30), which lets the row's address stay in scalar registers.
+template <typename T, bool MASK>
+struct Vector {
+  u32x4_any x;
+  u32x2_any a;
+  __device__ __forceinline__ void load(const char* row, const unsigned char* allowed, int i) {
+    x = *reinterpret_cast<const u32x4_any*>(row + (uint32_t)i * 16u);
+    if (MASK) {
+      const unsigned char* p = allowed + (uint32_t)i * (uint32_t)Row<T>::N;
+      if (Row<T>::N == 8) a = *reinterpret_cast<const u32x2_any*>(p); else a.x = *reinterpret_cast<const u32_any*>(p);
+    }
+  }
+  __device__ __forceinline__ void values(float (&z)[Row<T>::N]) const {
+    Row<T>::unpack(x, z);
+    if (MASK) {
+#pragma unroll
+      for (int n = 0; n < Row<T>::N; ++n) z[n] = (a[n / 4] >> (8 * (n % 4))) & 0xff ? z[n] : kNegInf;
+    }
+  }
+};
 
 template <typename T, bool MASK>
 __device__ __forceinline__ float value_at(const char* x, const unsigned char* a, long j) {
@@ -123,8 +135,9 @@ __device__ __forceinline__ Sums join_lanes(Sums a) {
   return a;
 }
 
+// Returns the largest of the values.
 template <int N>
-__device__ __forceinline__ void add_values(Sums& a, const float (&z)[N]) {
+__device__ __forceinline__ float add_values(Sums& a, const float (&z)[N]) {
   float c = z[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) c = fmaxf(c, z[i]);
@@ -136,6 +149,7 @@ __device__ __forceinline__ void add_values(Sums& a, const float (&z)[N]) {
     a.s += e;
     a.t = fmaf(e, fmaxf(d, -1e4f), a.t);
   }
+  return c;
 }
 
 // (value, id) before (other, other_id): larger value first, then the lower id.
@@ -146,12 +160,43 @@ struct Span {
   int first, end, tail, V;      // tail: index of the first value behind the last vector
 };
 
+// What a thread remembers of the vectors it has met: the largest value and where it was, and the largest of the other vectors.
+constexpr int kTail = -1;      // in place of a vector: the value behind them
+struct Met {
+  float most = kNegInf, next = kNegInf;
+  int at = kTail;
+  __device__ __forceinline__ void see(float c, int i) {
+    next = fmaxf(next, fminf(most, c));
+    at = c > most ? i : at;
+    most = fmaxf(most, c);
+  }
+};
+
+// A number that orders as the value does (0 behind all of them, NaN apart).
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);      // -0 as 0
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The k-th largest of a wave's 64 values, which have `BITS` leading bits: bit by bit, the largest number that k of them reach.
+template <int BITS>
+__device__ __forceinline__ float kth_largest(float v, int k) {
+  const uint32_t mine = ordered(v) >> (32 - BITS);
+  uint32_t at = 0;
+#pragma unroll
+  for (int i = BITS - 1; i >= 0; --i) {
+    const uint32_t next = at | 1u << i;
+    if (__builtin_popcountll(__ballot(mine >= next)) >= k) at = next;
+  }
+  const uint32_t u = at >> (BITS - 1) ? at ^ (1u << (BITS - 1)) : ~at;
+  return __uint_as_float(u << (32 - BITS));
+}
+
 // Largest values of a part of a row, most likely first, in v and id (empty places: -inf, -1).  Called by the whole workgroup.
 //
 // The pass over the row leaves every thread with the largest value it has met.  Lane l of all waves is group l, of 64: the k-th largest of the groups' maxima is
-// a lower bound b of the k-th largest value, and values above b lie in the fewer than k groups whose maximum is larger, values equal to b in
-// those and the ones where it is equal.  Those groups are read again (out of the cache: about k / 64 of the part) and what reaches b is put in order by
-// counting.  Values equal to b may be any number (a row of one value): where they do not fit, they are taken from the front, reading in order.
+// a lower bound b of the k-th largest value.  Threads that met one of at least b, k and a few in general, read its vector again, or all their vectors where the
+// largest value of the others reaches b too, and what reaches b is put in order by counting.  Values equal to b may be any number (a row of one value): where they do not fit, they are taken from the front, reading in order.
 // Where the values above b do not fit (all large values of a row in one group), the alternatives are looked for one after the other.
 template <typename T, bool MASK, int THREADS>
 struct Top {
@@ -161,7 +206,8 @@ struct Top {
   float most[kWaves][64];
   float above_v[kRoom];
   int above_i[kRoom], equal_i[kRoom];
-  int above, equal, count[kWaves], list[64];
+  int above, equal, chosen, count[kWaves], list[THREADS];
+  float bound;
 
   __device__ void one_by_one(const char* x, const unsigned char* a, const Span& p, int k) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -222,8 +268,9 @@ struct Top {
       float z[N] = {};
       const int i = base + tid, n = i < p.end ? N : 0;
       if (n) {
-        Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
-        if (MASK) Row<T>::masks(a + (long)i * N, z);
+        Vector<T, MASK> q;
+        q.load(x, a, i);
+        q.values(z);
       }
       take(z, n, i * N);
     }
@@ -234,30 +281,21 @@ struct Top {
     }
   }
 
-  __device__ void find(const char* x, const unsigned char* a, const Span& p, float mine, int k) {
+  __device__ void find(const char* x, const unsigned char* a, const Span& p, const Met& met, int k) {
     constexpr int N = Row<T>::N;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    most[wave][lane] = mine;
-    if (tid == 0) above = equal = 0;
+    most[wave][lane] = met.most;
     if (tid < k) v[tid] = kNegInf, id[tid] = -1;
     __syncthreads();
-    float group = most[0][lane];
-    for (int w = 1; w < kWaves; ++w) group = fmaxf(group, most[w][lane]);
-    int larger = 0, same = 0;
-#pragma unroll 16
-    for (int l = 0; l < 64; ++l) {
-      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), l));
-      larger += o > group;
-      same += o == group;
+    if (wave == 0) {
+      float group = met.most;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) group = fmaxf(group, most[w][lane]);
+      const float b = kth_largest<8 * (int)sizeof(T)>(group, k);
+      if (lane == 0) bound = b, above = equal = chosen = 0;
     }
-    const unsigned long long kth = __ballot(larger < k && larger + same >= k);      // never empty: k <= 64
-    const float b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(group), __builtin_ctzll(kth)));
-    const unsigned long long wanted = __ballot(group >= b && group > kNegInf);
-    const int groups = __builtin_popcountll(wanted);
-    if (groups == 0) return;      // nothing but -inf (all waves see the same groups)
-    const int nth = __builtin_popcountll(wanted & ((1ull << lane) - 1));
-    if (wave == 0 && (wanted >> lane & 1)) list[nth] = lane;
     __syncthreads();
+    const float b = bound;
     const auto see = [&](float z, int j) {
       if (z > b) {
         const int at = atomicAdd(&above, 1);
@@ -267,18 +305,35 @@ struct Top {
         if (at < kRoom) equal_i[at] = j;
       }
     };
-    const int each = (p.end - p.first + 63) / 64;      // vectors of a group
-    for (int u = tid; u < groups * each; u += THREADS) {
-      const int i = p.first + 64 * (u / groups) + list[u % groups];
-      if (i < p.end) {
-        float z[N];
-        Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
-        if (MASK) Row<T>::masks(a + (long)i * N, z);
+    const auto see_vector = [&](int i) {
+      Vector<T, MASK> q;
+      q.load(x, a, i);
+      float z[N];
+      q.values(z);
+      float c = z[0];
 #pragma unroll
+      for (int n = 1; n < N; ++n) c = fmaxf(c, z[n]);
+      if (c >= b)
         for (int n = 0; n < N; ++n) see(z[n], i * N + n);
+    };
+    if (met.most >= b && met.most > kNegInf) {
+      if (met.next >= b && met.next > kNegInf) {
+        list[atomicAdd(&chosen, 1)] = tid;
+        if (p.tail + tid < p.V) see(value_at<T, MASK>(x, a, p.tail + tid), p.tail + tid);
+      } else if (met.at == kTail) {
+        see(met.most, p.tail + tid);
+      } else {
+        see_vector(met.at);
       }
     }
-    if (p.tail + tid < p.V && (wanted >> lane & 1)) see(value_at<T, MASK>(x, a, p.tail + tid), p.tail + tid);
+    __syncthreads();
+    // all vectors of the threads that met such values in more than one: as many threads to each as there are
+    const int n = chosen;
+    if (n > 0) {
+      const int each = THREADS / n, sub = tid / n;
+      if (sub < each)
+        for (int i = p.first + list[tid - sub * n] + THREADS * sub; i < p.end; i += THREADS * each) see_vector(i);
+    }
     __syncthreads();
     const int na = above;
     int ne = equal;
@@ -321,24 +376,21 @@ struct PartScores {
   int id[kMaxTop];
 };
 
+// The value at a row's token, for the first thread; NaN where there is none.  The token is asked for before the row is read, its value behind it.
 template <typename T, bool MASK>
-__device__ __forceinline__ void finish(const LogitRows& in, const RowScores& out, long r, int V, int top_k, const char* x, const unsigned char* a, const Sums& all,
-                                       const float* v, const int* id) {
+__device__ __forceinline__ float token_value(long long t, int V, const char* x, const unsigned char* a) {
+  if (threadIdx.x != 0) return 0.f;
+  return t < 0 || t >= V ? __builtin_nanf("") : value_at<T, MASK>(x, a, t);
+}
+
+__device__ __forceinline__ void finish(const RowScores& out, long r, int top_k, long long id_given, float token, const Sums& all, const float* v, const int* id) {
   const int tid = threadIdx.x;
   const bool empty = all.s == 0.f, broken = all.s != all.s;      // broken: a NaN or +inf among the values
   const float logs = empty ? 0.f : logf(all.s), nan = __builtin_nanf("");
   if (tid == 0) {
     if (out.tokens) {
-      const long long t = out.tokens[r];
-      float lp = 0.f;
-      if (t != out.ignore_index) {
-        if (t < 0 || t >= V) lp = nan;
-        else {
-          const float z = value_at<T, MASK>(x, a, t);
-          lp = broken ? nan : z == kNegInf ? kNegInf : (z - all.m) - logs;
-        }
-      }
-      out.logprobs[r] = lp;
+      const float lp = broken ? nan : token == kNegInf ? kNegInf : (token - all.m) - logs;
+      out.logprobs[r] = id_given == out.ignore_index ? 0.f : lp;
     }
     out.entropy[r] = empty ? 0.f : logs - all.t / all.s;
     out.stats[2 * r] = broken ? nan : all.m;
@@ -352,88 +404,106 @@ __device__ __forceinline__ void finish(const LogitRows& in, const RowScores& out
 }
 
 // One workgroup a row, or a part of one where `parts` > 1: then what it found goes to `work` and token_scores_join_kernel puts the parts together.
-template <typename T, bool MASK, int THREADS>
-__global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, RowScores out, long rows, int V, int top_k, int parts, PartScores* __restrict__ work) {
+template <typename T, bool MASK, bool TOP, int THREADS>
+__global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, RowScores out, uint32_t first, int V, int top_k, int parts, PartScores* __restrict__ work) {
   constexpr int N = Row<T>::N, kWaves = THREADS / 64, kAhead = 4;
   __shared__ float part_m[kWaves], part_s[kWaves], part_t[kWaves];
   __shared__ Top<T, MASK, THREADS> top;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nvec = V / N, each = (nvec + parts - 1) / parts;
-  for (long b = blockIdx.x; b < rows * parts; b += gridDim.x) {
-    const long r = b / parts;
-    const int part = (int)(b % parts);
-    const char* x = row_of<T>(in, r);
-    const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
-    const Span p = {min(part * each, nvec), min((part + 1) * each, nvec), part == parts - 1 ? nvec * N : V, V};
-    Sums mine;
-    int i = p.first + tid;
-    for (; i + (kAhead - 1) * THREADS < p.end; i += kAhead * THREADS) {
-      u32x4_any q[kAhead];
-      float z[kAhead * N];
+  const uint32_t b = first + blockIdx.x;
+  const uint32_t r = parts > 1 ? b / parts : b;
+  const int part = parts > 1 ? b % parts : 0;
+  const long long token = out.tokens && tid == 0 ? out.tokens[r] : 0;
+  const char* x = row_of<T>(in, r);
+  const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
+  const Span p = {min(part * each, nvec), min((part + 1) * each, nvec), part == parts - 1 ? nvec * N : V, V};
+  Sums mine;
+  int i = p.first + tid;
+  Met met;
+  const auto add = [&](const Vector<T, MASK>& q, int at) {
+    float z[N];
+    q.values(z);
+    const float c = add_values<N>(mine, z);
+    if (TOP) met.see(c, at);
+  };
+  for (; i + (kAhead - 1) * THREADS < p.end; i += kAhead * THREADS) {
+    Vector<T, MASK> q[kAhead];
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) q[c] = *reinterpret_cast<const u32x4_any*>(x + (long)(i + c * THREADS) * 16);
+    for (int c = 0; c < kAhead; ++c) q[c].load(x, a, i + c * THREADS);
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) {
-        float (&zc)[N] = *reinterpret_cast<float (*)[N]>(z + c * N);
-        Row<T>::unpack(q[c], zc);
-        if (MASK) Row<T>::masks(a + (long)(i + c * THREADS) * N, zc);
-      }
-      add_values<kAhead * N>(mine, z);
-    }
-    for (; i < p.end; i += THREADS) {
-      float z[N];
-      Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
-      if (MASK) Row<T>::masks(a + (long)i * N, z);
-      add_values<N>(mine, z);
-    }
-    if (p.tail + tid < V) {
-      const float z[1] = {value_at<T, MASK>(x, a, p.tail + tid)};
-      add_values<1>(mine, z);
-    }
-    const float most = mine.m;
-    mine = join_lanes<64>(mine);
-    if (lane == 0) part_m[wave] = mine.m, part_s[wave] = mine.s, part_t[wave] = mine.t;
-    __syncthreads();
-    const int w = lane % kWaves;
-    const Sums all = join_lanes<kWaves>(Sums{part_m[w], part_s[w], part_t[w]});
-    if (top_k && all.s == all.s) top.find(x, a, p, most, top_k);
-    if (parts > 1) {
-      PartScores& to = work[b];
-      if (tid == 0) to.sums = all;
-      if (tid < top_k) to.v[tid] = top.v[tid], to.id[tid] = top.id[tid];
-    } else {
-      finish<T, MASK>(in, out, r, V, top_k, x, a, all, top.v, top.id);
-    }
-    __syncthreads();      // the row's shared values have been read
+    for (int c = 0; c < kAhead; ++c) add(q[c], i + c * THREADS);
+  }
+  // the last vectors: as many loads at a time
+  Vector<T, MASK> q[kAhead - 1];
+#pragma unroll
+  for (int c = 0; c < kAhead - 1; ++c)
+    if (i + c * THREADS < p.end) q[c].load(x, a, i + c * THREADS);
+#pragma unroll
+  for (int c = 0; c < kAhead - 1; ++c)
+    if (i + c * THREADS < p.end) add(q[c], i + c * THREADS);
+  if (p.tail + tid < V) {
+    const float z[1] = {value_at<T, MASK>(x, a, p.tail + tid)};
+    const float c = add_values<1>(mine, z);
+    if (TOP) met.see(c, kTail);
+  }
+  const float at_token = parts > 1 ? 0.f : token_value<T, MASK>(token, V, x, a);
+  mine = join_lanes<64>(mine);
+  if (lane == 0) part_m[wave] = mine.m, part_s[wave] = mine.s, part_t[wave] = mine.t;
+  __syncthreads();
+  const int w = lane % kWaves;
+  const Sums all = join_lanes<kWaves>(Sums{part_m[w], part_s[w], part_t[w]});
+  if (TOP)
+    if (all.s == all.s) top.find(x, a, p, met, top_k);
+  if (parts > 1) {
+    PartScores& to = work[b];
+    if (tid == 0) to.sums = all;
+    if (TOP && tid < top_k) to.v[tid] = top.v[tid], to.id[tid] = top.id[tid];
+  } else {
+    finish(out, r, top_k, token, at_token, all, top.v, top.id);
   }
 }
 
 // The parts of a row, a workgroup each: the largest of all parts' largest, in order, by counting.
 template <typename T, bool MASK>
-__global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, RowScores out, long rows, int V, int top_k, int parts, const PartScores* __restrict__ work) {
-  __shared__ float v[kMaxParts * kMaxTop], best_v[kMaxTop];
-  __shared__ int id[kMaxParts * kMaxTop], best_i[kMaxTop];
+__global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, RowScores out, int V, int top_k, int parts, const PartScores* __restrict__ work) {
+  constexpr int kTogether = 8;      // parts that are searched at the same time
+  __shared__ unsigned long long key[kMaxParts * kMaxTop];
+  __shared__ float best_v[kMaxTop];
+  __shared__ int best_i[kMaxTop];
   const int tid = threadIdx.x;
-  for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const PartScores* from = work + r * parts;
-    Sums all = from[0].sums;
-    for (int p = 1; p < parts; ++p) all = join(all, from[p].sums);
-    if (top_k && all.s == all.s) {
-      const int n = parts * top_k;
-      for (int i = tid; i < n; i += 256) v[i] = from[i / top_k].v[i % top_k], id[i] = from[i / top_k].id[i % top_k];
-      if (tid < top_k) best_v[tid] = kNegInf, best_i[tid] = -1;
-      __syncthreads();
-      for (int i = tid; i < n; i += 256) {
-        if (id[i] < 0) continue;
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += id[j] >= 0 && before(v[j], id[j], v[i], id[i]);
-        if (rank < top_k) best_v[rank] = v[i], best_i[rank] = id[i];
-      }
-      __syncthreads();
+  const uint32_t r = blockIdx.x;
+  const PartScores* from = work + r * parts;
+  const long long token = out.tokens && tid == 0 ? out.tokens[r] : 0;
+  const Sums all = join_lanes<kMaxParts>(tid % kMaxParts < parts ? from[tid % kMaxParts].sums : Sums{});
+  if (top_k && all.s == all.s) {
+    // larger values first, then lower ids: all keys are different, empty places are 0
+    for (int i = tid; i < (parts + kTogether - 1) / kTogether * kTogether * kMaxTop; i += 256) {
+      const int p = i / kMaxTop, n = i % kMaxTop;
+      const bool is = p < parts && n < top_k && from[p].id[n] >= 0;
+      key[i] = is ? (unsigned long long)ordered(from[p].v[n]) << 32 | (uint32_t)~from[p].id[n] : 0;
     }
-    finish<T, MASK>(in, out, r, V, top_k, row_of<T>(in, r), MASK ? in.allowed + r * in.allowed_row : nullptr, all, best_v, best_i);
+    if (tid < top_k) best_v[tid] = kNegInf, best_i[tid] = -1;
     __syncthreads();
+    for (int i = tid; i < parts * kMaxTop; i += 256) {
+      const unsigned long long mine = key[i];
+      int rank = 0;
+      // how many come before in each part, which is sorted
+      for (int p = 0; p < parts; p += kTogether) {
+        int at[kTogether] = {};
+#pragma unroll
+        for (int step = kMaxTop / 2; step > 0; step /= 2)
+#pragma unroll
+          for (int q = 0; q < kTogether; ++q) at[q] += key[(p + q) * kMaxTop + at[q] + step - 1] > mine ? step : 0;
+#pragma unroll
+        for (int q = 0; q < kTogether; ++q) rank += at[q] + (key[(p + q) * kMaxTop + at[q]] > mine ? 1 : 0);
+      }
+      if (mine && rank < top_k) best_v[rank] = from[i / kMaxTop].v[i % kMaxTop], best_i[rank] = (int)~(uint32_t)mine;
+    }
   }
+  const float at_token = token_value<T, MASK>(token, V, row_of<T>(in, r), MASK ? in.allowed + r * in.allowed_row : nullptr);
+  __syncthreads();
+  finish(out, r, top_k, token, at_token, all, best_v, best_i);
 }
 
 struct ScoreGrads {
@@ -447,69 +517,71 @@ template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void token_scores_grad_kernel(LogitRows in, const long long* __restrict__ tokens, long long ignore_index,
                                                                 const float* __restrict__ entropy, const float* __restrict__ stats,
                                                                 const long long* __restrict__ top_ids, ScoreGrads g, char* __restrict__ grad,
-                                                                long grad_row, long rows, int V, int top_k) {
+                                                                long grad_row, uint32_t first_row, uint32_t chunks, int V, int top_k) {
   constexpr int N = Row<T>::N;
   __shared__ int ids[kMaxTop + 1];
   __shared__ float gs[kMaxTop + 1];
   const int tid = threadIdx.x;
-  for (long r = blockIdx.y; r < rows; r += gridDim.y) {
-    const char* x = row_of<T>(in, r);
-    const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
-    char* out = grad + r * grad_row * (long)sizeof(T);
-    const float m = stats[2 * r], logs = stats[2 * r + 1];
-    const bool empty = m == kNegInf;
-    // the outputs' tokens and gradients
-    if (tid <= top_k) {
-      int id = -1;
-      float v = 0.f;
-      if (tid < top_k) {
-        if (g.top) id = (int)top_ids[r * top_k + tid], v = id < 0 ? 0.f : g.top[r * top_k + tid];
-      } else if (tokens && g.logprobs) {
-        const long long t = tokens[r];
-        if (t != ignore_index) {
-          const bool bad = t < 0 || t >= V;
-          id = bad ? -1 : (int)t;
-          v = bad ? __builtin_nanf("") : g.logprobs[r * g.logprobs_stride];
-        }
-      }
-      ids[tid] = id;
-      gs[tid] = v;
-    }
-    __syncthreads();
-    float total = 0.f;
-    for (int e = 0; e <= top_k; ++e) total += gs[e];
-    const float gh = g.entropy ? g.entropy[r * g.entropy_stride] : 0.f, h = entropy[r];
-    const auto slope = [&](float z) {
-      if (z == kNegInf || empty) return 0.f;
-      const float lp = (z - m) - logs;
-      return -exp2_(lp * kLog2e) * fmaf(gh, fmaxf(lp, -1e4f) + h, total);
-    };
-    const int nvec = V / N, first = (int)blockIdx.x * 256 * kBwdChunk, lo = first * N;
-  #pragma unroll
-    for (int c = 0; c < kBwdChunk; ++c) {
-      const int i = first + c * 256 + tid;
-      if (i < nvec) {
-        float z[N];
-        Row<T>::unpack(*reinterpret_cast<const u32x4_any*>(x + (long)i * 16), z);
-        if (MASK) Row<T>::masks(a + (long)i * N, z);
-  #pragma unroll
-        for (int n = 0; n < N; ++n) z[n] = slope(z[n]);
-        *reinterpret_cast<u32x4_any*>(out + (long)i * 16) = Row<T>::pack(z);
+  const uint32_t chunk = blockIdx.x % chunks;
+  const long r = first_row + blockIdx.x / chunks;
+  const char* x = row_of<T>(in, (uint32_t)r);
+  const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
+  char* out = grad + r * grad_row * (long)sizeof(T);
+  const int nvec = V / N, first = (int)chunk * 256 * kBwdChunk, lo = first * N;
+  Vector<T, MASK> q[kBwdChunk];      // asked for before all else
+#pragma unroll
+  for (int c = 0; c < kBwdChunk; ++c)
+    if (first + c * 256 + tid < nvec) q[c].load(x, a, first + c * 256 + tid);
+  const float m = stats[2 * r], logs = stats[2 * r + 1];
+  const bool empty = m == kNegInf;
+  // the outputs' tokens and gradients
+  if (tid <= top_k) {
+    int id = -1;
+    float v = 0.f;
+    if (tid < top_k) {
+      if (g.top) id = (int)top_ids[r * top_k + tid], v = id < 0 ? 0.f : g.top[r * top_k + tid];
+    } else if (tokens && g.logprobs) {
+      const long long t = tokens[r];
+      if (t != ignore_index) {
+        const bool bad = t < 0 || t >= V;
+        id = bad ? -1 : (int)t;
+        v = bad ? __builtin_nanf("") : g.logprobs[r * g.logprobs_stride];
       }
     }
-    const bool last = blockIdx.x == gridDim.x - 1;
-    if (last && nvec * N + tid < V) Row<T>::put(out, nvec * N + tid, slope(value_at<T, MASK>(x, a, nvec * N + tid)));
-    __syncthreads();
-    // the tokens themselves: what the whole row's pass wrote there lacks the outputs' own gradients
-    const int hi = last ? V : lo + 256 * kBwdChunk * N;
-    if (tid <= top_k && ids[tid] >= lo && ids[tid] < hi) {
-      const int id = ids[tid];
-      float own = 0.f;
-      for (int e = 0; e <= top_k; ++e) own += ids[e] == id ? gs[e] : 0.f;
-      const float z = value_at<T, MASK>(x, a, id);
-      Row<T>::put(out, id, z == kNegInf || empty ? 0.f : slope(z) + own);
+    ids[tid] = id;
+    gs[tid] = v;
+  }
+  __syncthreads();
+  float total = 0.f;
+  for (int e = 0; e <= top_k; ++e) total += gs[e];
+  const float gh = g.entropy ? g.entropy[r * g.entropy_stride] : 0.f, h = entropy[r];
+  const auto slope = [&](float z) {
+    if (z == kNegInf || empty) return 0.f;
+    const float lp = (z - m) - logs;
+    return -exp2_(lp * kLog2e) * fmaf(gh, fmaxf(lp, -1e4f) + h, total);
+  };
+#pragma unroll
+  for (int c = 0; c < kBwdChunk; ++c) {
+    const int i = first + c * 256 + tid;
+    if (i < nvec) {
+      float z[N];
+      q[c].values(z);
+#pragma unroll
+      for (int n = 0; n < N; ++n) z[n] = slope(z[n]);
+      *reinterpret_cast<u32x4_any*>(out + (long)i * 16) = Row<T>::pack(z);
     }
-    __syncthreads();      // ids and gs have been read
+  }
+  const bool last = chunk == chunks - 1;
+  if (last && nvec * N + tid < V) Row<T>::put(out, nvec * N + tid, slope(value_at<T, MASK>(x, a, nvec * N + tid)));
+  __syncthreads();
+  // the tokens themselves: what the whole row's pass wrote there lacks the outputs' own gradients
+  const int hi = last ? V : lo + 256 * kBwdChunk * N;
+  if (tid <= top_k && ids[tid] >= lo && ids[tid] < hi) {
+    const int id = ids[tid];
+    float own = 0.f;
+    for (int e = 0; e <= top_k; ++e) own += ids[e] == id ? gs[e] : 0.f;
+    const float z = value_at<T, MASK>(x, a, id);
+    Row<T>::put(out, id, z == kNegInf || empty ? 0.f : slope(z) + own);
   }
 }
 
@@ -518,6 +590,7 @@ static int check_rows(const char* who, const void* logits, int inner, long outer
   if (!logits) return set_error(M2_ERR_ARG, "%s: null pointer", who);
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype must be M2_DTYPE_F32 or M2_DTYPE_BF16 (got %d)", who, dtype);
   if (rows <= 0 || V <= 0 || inner <= 0 || outer < 0 || row < 0) return set_error(M2_ERR_ARG, "%s: rows=%ld V=%d inner=%d outer=%ld row=%ld", who, rows, V, inner, outer, row);
+  if (rows > 0x7fffffffL) return set_error(M2_ERR_UNSUPPORTED, "%s: at most 2^31 - 1 rows (rows=%ld)", who, rows);
   if (V > (1 << 30)) return set_error(M2_ERR_UNSUPPORTED, "%s: at most 2^30 values in a row (V=%d)", who, V);
   if (top_k < 0 || top_k > kMaxTop || top_k > V) return set_error(M2_ERR_UNSUPPORTED, "%s: 0 to %d alternatives, at most V (top_k=%d V=%d)", who, kMaxTop, top_k, V);
   if (allowed && allowed_row != 0 && allowed_row < V) return set_error(M2_ERR_ARG, "%s: allowed_row=%ld is less than V=%d", who, allowed_row, V);
@@ -551,20 +624,22 @@ extern "C" int m2_token_scores_fwd(const void* logits, int inner, long outer_str
   if (!entropy || !stats || (tokens && !logprobs) || (top_k && (!top_ids || !top_logprobs))) return set_error(M2_ERR_ARG, "%s: null pointer", who);
   const int parts = parts_of(rows, V, dtype);
   if (parts > 1 && (!workspace || (uintptr_t)workspace % 4)) return set_error(M2_ERR_ARG, "%s: rows=%ld V=%d need a workspace, aligned to 4 bytes", who, rows, V);
-  const LogitRows in = {logits, outer_stride, row_stride, inner, allowed, allowed_row};
+  const LogitRows in = {logits, outer_stride, row_stride, inner < rows ? (uint32_t)inner : 0, allowed, allowed_row};
   const RowScores out = {tokens, ignore_index, logprobs, entropy, stats, top_ids, top_logprobs};
   hipStream_t st = (hipStream_t)stream;
-  const long blocks = rows * parts < kMaxGrid ? rows * parts : kMaxGrid;
+  const long blocks = rows * parts;
   const auto go = [&](auto kernel, int threads) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, in, out, rows, V, top_k, parts, (PartScores*)workspace);
+    for (long first = 0; first < blocks; first += kMaxGrid)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks - first < kMaxGrid ? blocks - first : kMaxGrid)), dim3(threads), 0, st, in, out, (uint32_t)first, V, top_k, parts,
+                         (PartScores*)workspace);
   };
   const auto pick = [&](auto* t, auto masked) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr bool M = decltype(masked)::value;
-    if (blocks <= 512) go(token_scores_kernel<T, M, 1024>, 1024);
-    else go(token_scores_kernel<T, M, 256>, 256);
+    if (blocks <= 512) top_k ? go(token_scores_kernel<T, M, true, 1024>, 1024) : go(token_scores_kernel<T, M, false, 1024>, 1024);
+    else top_k ? go(token_scores_kernel<T, M, true, 256>, 256) : go(token_scores_kernel<T, M, false, 256>, 256);
     if (parts > 1)
-      hipLaunchKernelGGL((token_scores_join_kernel<T, M>), dim3((unsigned)rows), dim3(256), 0, st, in, out, rows, V, top_k, parts, (const PartScores*)workspace);
+      hipLaunchKernelGGL((token_scores_join_kernel<T, M>), dim3((unsigned)rows), dim3(256), 0, st, in, out, V, top_k, parts, (const PartScores*)workspace);
   };
   const auto type = [&](auto* t) { allowed ? pick(t, std::true_type{}) : pick(t, std::false_type{}); };
   dtype == M2_DTYPE_F32 ? type((float*)nullptr) : type((uint16_t*)nullptr);
@@ -581,13 +656,16 @@ extern "C" int m2_token_scores_bwd(const void* logits, int inner, long outer_str
   if (g_logprobs_stride < 0 || g_entropy_stride < 0) return set_error(M2_ERR_ARG, "%s: strides %ld and %ld", who, g_logprobs_stride, g_entropy_stride);
   if (grad_row < V) return set_error(M2_ERR_ARG, "%s: grad_row=%ld is less than V=%d", who, grad_row, V);
   if ((uintptr_t)grad % (dtype == M2_DTYPE_F32 ? 4 : 2)) return set_error(M2_ERR_UNSUPPORTED, "%s: grad must be aligned to its type", who);
-  const LogitRows in = {logits, outer_stride, row_stride, inner, allowed, allowed_row};
+  const LogitRows in = {logits, outer_stride, row_stride, inner < rows ? (uint32_t)inner : 0, allowed, allowed_row};
   const ScoreGrads g = {g_logprobs, g_entropy, g_top, g_logprobs_stride, g_entropy_stride};
   hipStream_t st = (hipStream_t)stream;
-  const int each = dtype == M2_DTYPE_F32 ? 4 : 8, span = 256 * kBwdChunk * each;
+  const int span = 256 * kBwdChunk * (dtype == M2_DTYPE_F32 ? 4 : 8);
+  const uint32_t chunks = (uint32_t)((V + (long)span - 1) / span);
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((V + span - 1) / span), (unsigned)(rows < 65535 ? rows : 65535)), dim3(256), 0, st, in, tokens, ignore_index, entropy, stats, top_ids, g,
-                       (char*)grad, grad_row, rows, V, top_k);
+    const long most = kMaxGrid / chunks;
+    for (long first = 0; first < rows; first += most)
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows - first < most ? rows - first : most) * chunks), dim3(256), 0, st, in, tokens, ignore_index, entropy, stats, top_ids, g,
+                         (char*)grad, grad_row, (uint32_t)first, chunks, V, top_k);
   };
   if (dtype == M2_DTYPE_F32) allowed ? go(token_scores_grad_kernel<float, true>) : go(token_scores_grad_kernel<float, false>);
   else allowed ? go(token_scores_grad_kernel<uint16_t, true>) : go(token_scores_grad_kernel<uint16_t, false>);

@@ -821,7 +821,7 @@ def int4_linear(x: Tensor, weight: Tensor, N: int, group: int, bias: Optional[Te
     if M == 0:
         return out
     x, inner, outer, row = _rows_apart(x)
-    if outer:
+    if inner < M:                                 # rows at two distances
         x, row = x.reshape(M, K), K
     with _on_device(x):
         check(lib.m2_int4_linear_fwd(x.data_ptr(), row, weight.data_ptr(), _ptr(bias), out.data_ptr(), M, N, K, group, activation is not None, code, _stream()))

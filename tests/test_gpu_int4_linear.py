@@ -74,6 +74,8 @@ def test_rows_any_distance_apart(gpu, dtype, M):
         assert torch.equal(lin(x), lin(x.contiguous().clone()))
     both = rows(gpu, 3, M, 2 * K, dtype=dtype)[:, : max(1, M - 1), K // 2:K // 2 + K]      # rows at two distances
     check(lin(both), both, w, scales, group)
+    again = room[:M, :K].expand(3, M, K)          # the same rows three times over
+    check(lin(again), again, w, scales, group)
     v = rows(gpu, K, dtype=dtype)
     check(lin(v), v, w, scales, group)
     assert lin(room[:0, :K]).shape == (0, N)
