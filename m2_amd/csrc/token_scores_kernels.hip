@@ -178,6 +178,11 @@ __device__ __forceinline__ uint32_t ordered(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+
+// Larger for what comes first: larger values, of equal ones the lower id.
+__device__ __forceinline__ unsigned long long key_of(float v, int id) { return (unsigned long long)ordered(v) << 32 | (uint32_t)~id; }
+
 // The k-th largest of a wave's 64 values, which have `BITS` leading bits: bit by bit, the largest number that k of them reach.
 template <int BITS>
 __device__ __forceinline__ float kth_largest(float v, int k) {
@@ -204,8 +209,8 @@ struct Top {
   float v[kMaxTop];
   int id[kMaxTop];
   float most[kWaves][64];
-  float above_v[kRoom];
-  int above_i[kRoom], equal_i[kRoom];
+  unsigned long long above_key[kRoom];
+  int equal_i[kRoom];
   int above, equal, chosen, count[kWaves], list[THREADS];
   float bound;
 
@@ -299,7 +304,7 @@ struct Top {
     const auto see = [&](float z, int j) {
       if (z > b) {
         const int at = atomicAdd(&above, 1);
-        if (at < kRoom) above_v[at] = z, above_i[at] = j;
+        if (at < kRoom) above_key[at] = key_of(z, j);
       } else if (z == b && b > kNegInf) {
         const int at = atomicAdd(&equal, 1);
         if (at < kRoom) equal_i[at] = j;
@@ -345,13 +350,16 @@ struct Top {
       ne = k - na;
     }
     for (int i = tid; i < na; i += THREADS) {
+      const unsigned long long mine = above_key[i];
       int rank = 0;
-      for (int j = 0; j < na; ++j) rank += before(above_v[j], above_i[j], above_v[i], above_i[i]);
-      if (rank < k) v[rank] = above_v[i], id[rank] = above_i[i];
+#pragma unroll 8
+      for (int j = 0; j < na; ++j) rank += above_key[j] > mine;
+      if (rank < k) v[rank] = unordered(mine >> 32), id[rank] = (int)~(uint32_t)mine;
     }
     if (na < k)
       for (int i = tid; i < ne; i += THREADS) {
         int rank = na;
+#pragma unroll 8
         for (int j = 0; j < ne; ++j) rank += equal_i[j] < equal_i[i];
         if (rank < k) v[rank] = b, id[rank] = equal_i[i];
       }
@@ -481,7 +489,7 @@ __global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, Ro
     for (int i = tid; i < (parts + kTogether - 1) / kTogether * kTogether * kMaxTop; i += 256) {
       const int p = i / kMaxTop, n = i % kMaxTop;
       const bool is = p < parts && n < top_k && from[p].id[n] >= 0;
-      key[i] = is ? (unsigned long long)ordered(from[p].v[n]) << 32 | (uint32_t)~from[p].id[n] : 0;
+      key[i] = is ? key_of(from[p].v[n], from[p].id[n]) : 0;
     }
     if (tid < top_k) best_v[tid] = kNegInf, best_i[tid] = -1;
     __syncthreads();
@@ -498,7 +506,7 @@ __global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, Ro
 #pragma unroll
         for (int q = 0; q < kTogether; ++q) rank += at[q] + (key[(p + q) * kMaxTop + at[q]] > mine ? 1 : 0);
       }
-      if (mine && rank < top_k) best_v[rank] = from[i / kMaxTop].v[i % kMaxTop], best_i[rank] = (int)~(uint32_t)mine;
+      if (mine && rank < top_k) best_v[rank] = unordered(mine >> 32), best_i[rank] = (int)~(uint32_t)mine;
     }
   }
   const float at_token = token_value<T, MASK>(token, V, row_of<T>(in, r), MASK ? in.allowed + r * in.allowed_row : nullptr);
