@@ -20,48 +20,167 @@ constexpr int tile_bytes(int group) { return 64 * 16 + kTileN * (kTileK / group)
 
 __device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f)); }
 
-constexpr int kRows = 4;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) u32x4_any;      // at any address of x's type
 
-// A wave has a tile's 16 rows of W and up to four of x; its lanes share K.
-template <typename T, int GROUP>
-__global__ __launch_bounds__(256) void int4_linear_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w,
-                                                          const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = (int)blockIdx.x * 4 + wave, m0 = (int)blockIdx.y * kRows, kt = (K + kTileK - 1) / kTileK;
-  if (tile * kTileN >= N) return;
-  float acc[kRows] = {};
-  for (int b = 0; b < kt; ++b) {
-    const unsigned char* p = w + ((long)tile * kt + b) * tile_bytes(GROUP);
-    const uint4 q4 = *reinterpret_cast<const uint4*>(p + lane * 16);
-    const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+// Eight codes as bf16 16 + q, exactly: 0x4180 is 16, and its last bits but three are worth 1 each.  What a row of x sums to, times 24, is taken off again.
+__device__ __forceinline__ bf16x8 codes(uint32_t q) {
+  const u32x4 v = {((q << 3) & 0x00780078u) | 0x41804180u, ((q >> 1) & 0x00780078u) | 0x41804180u, ((q >> 5) & 0x00780078u) | 0x41804180u,
+                   ((q >> 9) & 0x00780078u) | 0x41804180u};
+  return __builtin_bit_cast(bf16x8, v);
+}
+__device__ __forceinline__ bf16x8 minus24() {
+  const u32x4 v = {0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};
+  return __builtin_bit_cast(bf16x8, v);
+}
+__device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// Rows of x as the operand of 16 rows by 32 columns: lane l has row l % 16, columns 8 (l / 16) .. + 7.
+// bf16: 16 rows.  fp32: 4 rows in 4 places each, the first three of them the row's three bf16 parts, x = part + part + part with the low bits
+// cut off in turn (no rounding, so none overflows); what the fourth holds is not looked at.
+template <typename T> struct Operand;
+template <> struct Operand<uint16_t> {
+  static constexpr int kRows = 16;
+  static __device__ __forceinline__ int row(int lane) { return lane & 15; }
+  u32x4 v;
+  __device__ __forceinline__ void load(const uint16_t* p) { v = *reinterpret_cast<const u32x4_any*>(p); }
+  __device__ __forceinline__ void load(const uint16_t* p, int n) {      // the first n of eight
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      const float s = bf16_to_f32(*reinterpret_cast<const uint16_t*>(p + 1024 + ((lane & 15) * (kTileK / GROUP) + step * 32 / GROUP) * 2));
+    for (int i = 0; i < 4; ++i) v[i] = (2 * i < n ? p[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+  }
+  __device__ __forceinline__ bf16x8 get(int) const { return __builtin_bit_cast(bf16x8, v); }
+};
+template <> struct Operand<float> {
+  static constexpr int kRows = 4;
+  static __device__ __forceinline__ int row(int lane) { return (lane & 15) >> 2; }
+  u32x4 v[2];
+  __device__ __forceinline__ void load(const float* p) {
+    v[0] = *reinterpret_cast<const u32x4_any*>(p);
+    v[1] = *reinterpret_cast<const u32x4_any*>(p + 4);
+  }
+  __device__ __forceinline__ void load(const float* p, int n) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = b * kTileK + step * 32 + (lane >> 4) * 8 + j;
-        const float v = (float)((int)((q[step] >> (16 * (j % 2) + 4 * (j / 2))) & 15) - 8) * s;
-        if (k < K)
+    for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = i < n ? __float_as_uint(p[i]) : 0u;
+  }
+  __device__ __forceinline__ bf16x8 get(int lane) const {
+    const uint32_t second = (lane & 3) > 0 ? 0xffff0000u : 0u, third = (lane & 3) > 1 ? 0xffff0000u : 0u;
+    uint32_t f[8];
 #pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            const T* row = x + (long)min(m0 + r, M - 1) * x_row;
-            float xv;
-            if constexpr (sizeof(T) == 4) xv = row[k]; else xv = bf16_to_f32(row[k]);
-            acc[r] = fmaf(xv, v, acc[r]);
-          }
-      }
+    for (int i = 0; i < 8; ++i) {
+      float x = __uint_as_float(v[i / 4][i % 4]);
+      x -= __uint_as_float(__float_as_uint(x) & second);
+      x -= __uint_as_float(__float_as_uint(x) & third);
+      f[i] = __float_as_uint(x);
+    }
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_amdgcn_perm(f[2 * i + 1], f[2 * i], 0x07060302u);      // the upper halves
+    return __builtin_bit_cast(bf16x8, o);
+  }
+};
+
+// The scales of a lane's row in a tile.
+template <int GROUP>
+struct Scales {
+  uint32_t v[GROUP == 32 ? 2 : 1];
+  __device__ __forceinline__ void load(const unsigned char* tile, int lane) {
+    const unsigned char* p = tile + 1024 + (lane & 15) * (kTileK / GROUP) * 2;
+    if (GROUP == 32) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      v[0] = u.x;
+      v[GROUP == 32 ? 1 : 0] = u.y;
+    } else {
+      v[0] = GROUP == 64 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
     }
   }
-  const int n = tile * kTileN + (lane & 15);
+  __device__ __forceinline__ float get(int g) const { return __uint_as_float(g % 2 ? v[g / 2] & 0xffff0000u : v[g / 2] << 16); }
+};
+
+// One tile of 128 columns for all: what a wave has asked for, and what it makes of it.
+template <typename T, int GROUP>
+struct Step {
+  u32x4 q;
+  Scales<GROUP> s;
+  Operand<T> x[4];
+  __device__ __forceinline__ void load(const unsigned char* w, const T* row, int b, int K, int lane) {
+    const unsigned char* p = w + (long)b * tile_bytes(GROUP);
+    q = *reinterpret_cast<const u32x4*>(p + lane * 16);
+    s.load(p, lane);
+    const int k = b * kTileK + (lane >> 4) * 8;
+    if ((b + 1) * kTileK <= K) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    float y = acc[r];
-    y += __shfl_xor(y, 16);
-    y += __shfl_xor(y, 32);
-    if (lane < 16 && n < N && m0 + r < M) {
-      y += bias ? bias[n] : 0.f;
-      if (gelu) y = gelu_erf(y);
-      if constexpr (sizeof(T) == 4) out[(long)(m0 + r) * N + n] = y; else out[(long)(m0 + r) * N + n] = f32_to_bf16(y);
+      for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32, K - k - i * 32);
+    }
+  }
+  __device__ __forceinline__ void add(floatx4& sum, int lane) const {
+#pragma unroll
+    for (int g = 0; g < kTileK / GROUP; ++g) {
+      constexpr int kSteps = GROUP / 32;
+      bf16x8 a[kSteps];
+      floatx4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        a[i] = x[g * kSteps + i].get(lane);
+        c = mfma(a[i], minus24(), c);
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes(q[g * kSteps + i]), c);
+      const float scale = s.get(g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(scale, c[i], sum[i]);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void put(T* out, long at, float y, int gelu) {
+  if (gelu) y = gelu_erf(y);
+  if constexpr (sizeof(T) == 4) out[at] = y; else out[at] = f32_to_bf16(y);
+}
+
+// Up to 16 rows of bf16 or 4 of fp32.  SPLIT waves share the columns of a tile of 16 rows of W, each every SPLIT-th tile of 128; their sums meet in shared memory.
+template <typename T, int GROUP, int SPLIT>
+__global__ __launch_bounds__(256) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
+                                                            T* __restrict__ out, int M, int N, int K, int gelu) {
+  __shared__ floatx4 sums[SPLIT > 1 ? 4 : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
+  const int tile = (int)blockIdx.x * (4 / SPLIT) + wave / SPLIT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (tile < tiles) {
+    const unsigned char* mine = w + (long)tile * kt * tile_bytes(GROUP);
+    const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
+    Step<T, GROUP> now, next;
+    if (part < kt) now.load(mine, row, part, K, lane);
+    for (int b = part; b < kt; b += SPLIT) {
+      if (b + SPLIT < kt) next.load(mine, row, b + SPLIT, K, lane);
+      now.add(sum, lane);
+      now = next;
+    }
+  }
+  if (SPLIT > 1) {
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 1; i < SPLIT; ++i) sum += sums[wave + (SPLIT > 1 ? i : 0)][lane];
+  }
+  const int n = tile * kTileN + (lane & 15);
+  if (n >= N) return;
+  const float b = bias ? bias[n] : 0.f;
+  if constexpr (sizeof(T) == 4) {
+    const int m = m0 + (lane >> 4);
+    if (m < M) put(out, (long)m * N + n, (sum[2] + sum[1]) + sum[0] + b, gelu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = m0 + (lane >> 4) * 4 + i;
+      if (m < M) put(out, (long)m * N + n, sum[i] + b, gelu);
     }
   }
 }
@@ -86,16 +205,25 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   const uintptr_t size = dtype == M2_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)x % size || (uintptr_t)out % size || (uintptr_t)bias % 4) return set_error(M2_ERR_UNSUPPORTED, "%s: x, out and bias must be aligned to their type", who);
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + kRows - 1) / kRows));
+  const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
+  // eight waves a compute unit, where there are as many
+  const int split = tiles >= 2048 || kt < 2 ? 1 : tiles >= 1024 || kt < 4 ? 2 : 4;
   const auto go = [&](auto kernel, auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
+    const dim3 grid((unsigned)((tiles * (long)split + 3) / 4), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows));
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
   };
-  const auto pick = [&](auto* t) {
+  const auto parts = [&](auto* t, auto g) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (group == 32) go(int4_linear_kernel<T, 32>, t);
-    else if (group == 64) go(int4_linear_kernel<T, 64>, t);
-    else go(int4_linear_kernel<T, 128>, t);
+    constexpr int G = decltype(g)::value;
+    if (split == 1) go(int4_few_rows_kernel<T, G, 1>, t);
+    else if (split == 2) go(int4_few_rows_kernel<T, G, 2>, t);
+    else go(int4_few_rows_kernel<T, G, 4>, t);
+  };
+  const auto pick = [&](auto* t) {
+    if (group == 32) parts(t, std::integral_constant<int, 32>{});
+    else if (group == 64) parts(t, std::integral_constant<int, 64>{});
+    else parts(t, std::integral_constant<int, 128>{});
   };
   dtype == M2_DTYPE_F32 ? pick((float*)nullptr) : pick((uint16_t*)nullptr);
   return check_launch("int4_linear");
