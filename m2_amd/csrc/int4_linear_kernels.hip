@@ -46,10 +46,11 @@ template <> struct Operand<uint16_t> {
   static __device__ __forceinline__ int row(int lane) { return lane & 15; }
   u32x4 v;
   __device__ __forceinline__ void load(const uint16_t* p) { v = *reinterpret_cast<const u32x4_any*>(p); }
-  __device__ __forceinline__ void load(const uint16_t* p, int n) {      // the first n of eight
+  __device__ __forceinline__ void one(const uint16_t* p, int n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (2 * i < n ? p[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] << 16 : 0u);
   }
+  __device__ __forceinline__ void keep(bool is) { v = is ? v : u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ bf16x8 get(int) const { return __builtin_bit_cast(bf16x8, v); }
 };
 template <> struct Operand<float> {
@@ -60,10 +61,11 @@ template <> struct Operand<float> {
     v[0] = *reinterpret_cast<const u32x4_any*>(p);
     v[1] = *reinterpret_cast<const u32x4_any*>(p + 4);
   }
-  __device__ __forceinline__ void load(const float* p, int n) {
+  __device__ __forceinline__ void one(const float* p, int n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = i < n ? __float_as_uint(p[i]) : 0u;
   }
+  __device__ __forceinline__ void keep(bool is) { v[0] = is ? v[0] : u32x4{0, 0, 0, 0}, v[1] = is ? v[1] : u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ bf16x8 get(int lane) const {
     const uint32_t second = (lane & 3) > 0 ? 0xffff0000u : 0u, third = (lane & 3) > 1 ? 0xffff0000u : 0u;
     uint32_t f[8];
@@ -80,6 +82,17 @@ template <> struct Operand<float> {
     return __builtin_bit_cast(bf16x8, o);
   }
 };
+
+// The eight values of a row from column k on, 0 behind the last: where K is a multiple of eight (EVEN), all of them or none; else one by one.
+template <typename T, bool EVEN>
+__device__ __forceinline__ void load_edge(Operand<T>& to, const T* row, int k, int K) {
+  if (EVEN) {
+    to.load(row + (k < K ? k : 0));
+    to.keep(k < K);
+  } else {
+    to.one(row + k, K - k);
+  }
+}
 
 // The scales of a lane's row in a tile.
 template <int GROUP>
@@ -99,7 +112,7 @@ struct Scales {
 };
 
 // One tile of 128 columns for all: what a wave has asked for, and what it makes of it.
-template <typename T, int GROUP>
+template <typename T, int GROUP, bool EVEN>
 struct Step {
   u32x4 q;
   Scales<GROUP> s;
@@ -114,7 +127,7 @@ struct Step {
       for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32, K - k - i * 32);
+      for (int i = 0; i < 4; ++i) load_edge<T, EVEN>(x[i], row, k + i * 32, K);
     }
   }
   __device__ __forceinline__ void add(floatx4& sum, int lane) const {
@@ -144,7 +157,7 @@ __device__ __forceinline__ void put(T* out, long at, float y, int gelu) {
 }
 
 // Up to 16 rows of bf16 or 4 of fp32.  SPLIT waves share the columns of a tile of 16 rows of W, each every SPLIT-th tile of 128; their sums meet in shared memory.
-template <typename T, int GROUP, int SPLIT>
+template <typename T, int GROUP, bool EVEN, int SPLIT>
 __global__ __launch_bounds__(256) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
                                                             T* __restrict__ out, int M, int N, int K, int gelu) {
   __shared__ floatx4 sums[SPLIT > 1 ? 4 : 1][64];
@@ -155,7 +168,7 @@ __global__ __launch_bounds__(256) void int4_few_rows_kernel(const T* __restrict_
   if (tile < tiles) {
     const unsigned char* mine = w + (long)tile * kt * tile_bytes(GROUP);
     const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
-    Step<T, GROUP> now, next;
+    Step<T, GROUP, EVEN> now, next;
     if (part < kt) now.load(mine, row, part, K, lane);
     for (int b = part; b < kt; b += SPLIT) {
       if (b + SPLIT < kt) next.load(mine, row, b + SPLIT, K, lane);
@@ -185,6 +198,127 @@ __global__ __launch_bounds__(256) void int4_few_rows_kernel(const T* __restrict_
   }
 }
 
+// More rows: a workgroup has MT times 16 places of rows (as Operand) and 4 NT tiles of W's rows, NT a wave.  x goes through shared memory, one tile of 128
+// columns after the other in two buffers, in the operand's order: 64 lanes times 16 bytes for each 16 places and 32 columns.  A lane's place among
+// the 16 of its eighth is turned by the number of the eighth, so that the threads that write a row's sixteen eighths meet in no bank; readers are permuted
+// among themselves.
+template <typename T, bool EVEN, int MT>
+struct Staged {
+  static constexpr int kRows = MT * Operand<T>::kRows, kBytes = MT * 4 * 1024, kEach = kRows / 16;      // kEach: eighths of a thread
+  static_assert(kRows % 16 == 0, "a row for every 16 threads");
+  Operand<T> v[kEach];
+  __device__ __forceinline__ void load(const T* x, long x_row, int m0, int M, int b, int K) {
+    const int k = b * kTileK + (threadIdx.x & 15) * 8;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const T* row = x + (long)min(m0 + (int)(threadIdx.x >> 4) + 16 * i, M - 1) * x_row;
+      if ((b + 1) * kTileK <= K) v[i].load(row + k); else load_edge<T, EVEN>(v[i], row, k, K);
+    }
+  }
+  __device__ __forceinline__ void store(unsigned char* to) const {
+    const int c = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int row = (int)(threadIdx.x >> 4) + 16 * i;
+      constexpr int kPlaces = sizeof(T) == 4 ? 3 : 1, kSpread = sizeof(T) == 4 ? 4 : 1;
+#pragma unroll
+      for (int part = 0; part < kPlaces; ++part) {
+        const int place = row * kSpread + part;
+        *reinterpret_cast<bf16x8*>(to + (place / 16 * 4 + c / 4) * 1024 + (c % 4 * 16 + ((place & 15) ^ c)) * 16) = v[i].get(part);
+      }
+    }
+  }
+  static __device__ __forceinline__ bf16x8 read(const unsigned char* from, int mt, int step, int lane) {
+    const int c = step * 4 + (lane >> 4);
+    return *reinterpret_cast<const bf16x8*>(from + (mt * 4 + step) * 1024 + ((lane & 48) + ((lane & 15) ^ c)) * 16);
+  }
+};
+
+template <typename T, int GROUP, bool EVEN, int MT, int NT>
+__global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
+                                                        T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks) {
+  constexpr int kSteps = GROUP / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char staged[2][Staged<T, EVEN, MT>::kBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
+  const int m0 = (int)(blockIdx.x % row_blocks) * Staged<T, EVEN, MT>::kRows, t0 = ((int)(blockIdx.x / row_blocks) * 4 + wave) * NT;
+  const unsigned char* mine[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) mine[t] = w + (long)min(t0 + t, tiles - 1) * kt * tile_bytes(GROUP);
+  floatx4 sum[MT][NT] = {};
+  Staged<T, EVEN, MT> x_now;
+  u32x4 q[NT], q_next[NT];
+  Scales<GROUP> s[NT], s_next[NT];
+  const auto ask = [&](int b) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const unsigned char* p = mine[t] + (long)b * tile_bytes(GROUP);
+      q_next[t] = *reinterpret_cast<const u32x4*>(p + lane * 16);
+      s_next[t].load(p, lane);
+    }
+    x_now.load(x, x_row, m0, M, b, K);
+  };
+  ask(0);
+  x_now.store(staged[0]);
+  __syncthreads();
+  for (int b = 0; b < kt; ++b) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) q[t] = q_next[t], s[t] = s_next[t];
+    if (b + 1 < kt) ask(b + 1);
+    const unsigned char* from = staged[b & 1];
+#pragma unroll
+    for (int g = 0; g < kTileK / GROUP; ++g) {
+      bf16x8 a[MT][kSteps];
+      floatx4 c0[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        c0[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          a[m][i] = Staged<T, EVEN, MT>::read(from, m, g * kSteps + i, lane);
+          c0[m] = mfma(a[m][i], minus24(), c0[m]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        bf16x8 v[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) v[i] = codes(q[t][g * kSteps + i]);
+        const float scale = s[t].get(g);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          floatx4 c = c0[m];
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) c = mfma(a[m][i], v[i], c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[m][t][i] = fmaf(scale, c[i], sum[m][t][i]);
+        }
+      }
+    }
+    if (b + 1 < kt) x_now.store(staged[(b + 1) & 1]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int n = (t0 + t) * kTileN + (lane & 15);
+    if (n >= N) continue;
+    const float bn = bias ? bias[n] : 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if constexpr (sizeof(T) == 4) {
+        const int row = m0 + m * 4 + (lane >> 4);
+        if (row < M) put(out, (long)row * N + n, (sum[m][t][2] + sum[m][t][1]) + sum[m][t][0] + bn, gelu);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = m0 + m * 16 + (lane >> 4) * 4 + i;
+          if (row < M) put(out, (long)row * N + n, sum[m][t][i] + bn, gelu);
+        }
+      }
+    }
+  }
+}
+
 }  // namespace m2
 
 using namespace m2;
@@ -207,18 +341,33 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   hipStream_t st = (hipStream_t)stream;
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
   // eight waves a compute unit, where there are as many
-  const int split = tiles >= 2048 || kt < 2 ? 1 : tiles >= 1024 || kt < 4 ? 2 : 4;
+  const int split = K % 8 ? 4 : tiles >= 2048 || kt < 2 ? 1 : tiles >= 1024 || kt < 4 ? 2 : 4;
   const auto go = [&](auto kernel, auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const dim3 grid((unsigned)((tiles * (long)split + 3) / 4), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows));
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
   };
+  const auto rows = [&](auto kernel, auto* t, int mt, int nt) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const int each = mt * Operand<T>::kRows, row_blocks = (M + each - 1) / each;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 4L * nt - 1) / (4 * nt) * row_blocks)), dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias,
+                       (T*)out, M, N, K, gelu, row_blocks);
+  };
   const auto parts = [&](auto* t, auto g) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int G = decltype(g)::value;
-    if (split == 1) go(int4_few_rows_kernel<T, G, 1>, t);
-    else if (split == 2) go(int4_few_rows_kernel<T, G, 2>, t);
-    else go(int4_few_rows_kernel<T, G, 4>, t);
+    const int places = (M + Operand<T>::kRows - 1) / Operand<T>::kRows;      // times 16
+    if (places > 1) {
+      constexpr int kMt = sizeof(T) == 4 ? 4 : 2;      // 32 rows of bf16, 16 of fp32
+      const long blocks = (places + kMt - 1L) / kMt * ((tiles + 7) / 8);
+      if (K % 8) return rows(int4_rows_kernel<T, G, false, kMt, 1>, t, kMt, 1);
+      if (blocks < 512) return rows(int4_rows_kernel<T, G, true, kMt, 1>, t, kMt, 1);
+      return rows(int4_rows_kernel<T, G, true, kMt, 2>, t, kMt, 2);
+    }
+    if (K % 8) return go(int4_few_rows_kernel<T, G, false, 4>, t);
+    if (split == 1) go(int4_few_rows_kernel<T, G, true, 1>, t);
+    else if (split == 2) go(int4_few_rows_kernel<T, G, true, 2>, t);
+    else go(int4_few_rows_kernel<T, G, true, 4>, t);
   };
   const auto pick = [&](auto* t) {
     if (group == 32) parts(t, std::integral_constant<int, 32>{});
