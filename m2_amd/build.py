@@ -46,30 +46,32 @@ def _compile(src: str, incremental: bool = False) -> str:
     return obj
 
 
-def _build_param_check(incremental: bool = False) -> str:
-    """m2_amd/_param_check.so, a host-only CPython extension against torch's headers."""
+def _build_extension(name: str, incremental: bool = False) -> str:
+    """m2_amd/_NAME.so from csrc/NAME.cpp, a host-only CPython extension against torch's headers."""
     import sysconfig
 
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    src, out = os.path.join(CSRC, "param_check.cpp"), os.path.join(HERE, "_param_check.so")
-    if incremental and os.path.exists(out) and os.path.getmtime(src) < os.path.getmtime(out):
+    src, out = os.path.join(CSRC, name + ".cpp"), os.path.join(HERE, f"_{name}.so")
+    header = os.path.join(HERE, "..", "include", "m2_amd.h")
+    if incremental and os.path.exists(out) and max(os.path.getmtime(src), os.path.getmtime(header)) < os.path.getmtime(out):
         return out
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f"-I{p}" for p in include_paths()], f"-I{sysconfig.get_paths()['include']}", src, "-o", out,
-           *[f"-L{p}" for p in library_paths()], "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           *[f"-I{p}" for p in include_paths()], "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}", src, "-o", out,
+           *[f"-L{p}" for p in library_paths()], "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for param_check.cpp:\n{r.stderr}")
+        raise RuntimeError(f"g++ failed for {name}.cpp:\n{r.stderr}")
     return out
 
 
 def build(verbose: bool = True, incremental: bool = False) -> str:
     """Compiles every source (or, with incremental=True, only those older than their .hip / headers) and links."""
     with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        check = ex.submit(_build_param_check, incremental)
+        checks = [ex.submit(_build_extension, name, incremental) for name in ("answer_calls", "param_check")]
         objs = list(ex.map(lambda src: _compile(src, incremental), SOURCES))
-        check.result()
+        for check in checks:
+            check.result()
     cmd = [HIPCC, "-shared", "-fPIC", "--offload-arch=gfx950", "-o", LIB, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -1,0 +1,243 @@
+// CPython extension m2_amd._answer_calls: the host side of Int4Linear and token_logprobs (m2_amd/int4.py, m2_amd/scores.py).
+//
+// Their calls are a few microseconds of GPU time for a row or a handful of them, and checks, output tensors and the call through ctypes took
+// 10 to 17 us in Python (torch's own linear: 19), a gradient 100: here the same checks raise the same errors.  us a call, one stream, back to back, Python / here:
+// Int4Linear 768 x 768 11.8 / 7.5; token_logprobs 1 x 30522 17.0 / 8.7, 1 x 30522 fp32 with its gradient 118 / 66 (most of it torch's own backward pass).
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <ATen/ATen.h>
+
+#include "../../include/m2_amd.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+
+// The entry points of libm2_amd.so, which m2_amd/_lib.py has loaded.
+decltype(&m2_last_error) last_error;
+decltype(&m2_int4_weight_bytes) int4_weight_bytes;
+decltype(&m2_int4_linear_fwd) int4_linear_fwd;
+decltype(&m2_token_scores_workspace_bytes) token_scores_workspace_bytes;
+decltype(&m2_token_scores_fwd) token_scores_fwd;
+decltype(&m2_token_scores_bwd) token_scores_bwd;
+
+template <typename F>
+void set(F& f, uintptr_t address) { f = reinterpret_cast<F>(address); }
+
+void bind(std::vector<uintptr_t> a) {
+  TORCH_CHECK(a.size() == 6, "six addresses");
+  set(last_error, a[0]);
+  set(int4_weight_bytes, a[1]);
+  set(int4_linear_fwd, a[2]);
+  set(token_scores_workspace_bytes, a[3]);
+  set(token_scores_fwd, a[4]);
+  set(token_scores_bwd, a[5]);
+}
+
+void check(int rc) { TORCH_CHECK(rc == M2_OK, "libm2_amd error ", rc, ": ", last_error()); }
+
+void* current_stream() { return c10::hip::getCurrentHIPStream().stream(); }
+
+void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+int type_of(const char* name, const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), name, ": must live on the GPU (m2_amd has no CPU path); got device ", t.device());
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, ": must be float32 or bfloat16, got ", t.scalar_type());
+  return t.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16;
+}
+
+// t (..., n): row r of its leading dimensions lies (r / inner) * outer + (r % inner) * row values behind the first, in t or a copy of it: one is made where
+// a row's values lie apart, or the rows at more than `distances` (1 or 2) distances.
+struct Rows {
+  Tensor t;
+  int64_t inner = 1, outer = 0, row = 0;
+};
+Rows rows_of(Tensor t, int distances) {
+  const int64_t d = t.dim() - 1;
+  if (t.size(d) > 1 && t.stride(d) != 1) t = t.contiguous();
+  int64_t size[2] = {1, 1}, stride[2] = {0, 0};      // the innermost first
+  int n = 0;
+  for (int64_t i = d - 1; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (n > 0 && t.stride(i) == size[n - 1] * stride[n - 1]) {
+      size[n - 1] *= t.size(i);
+    } else {
+      if (n == distances) return rows_of(t.contiguous(), distances);
+      size[n] = t.size(i), stride[n] = t.stride(i);
+      ++n;
+    }
+  }
+  return {std::move(t), size[0], n > 1 ? stride[1] : 0, stride[0]};
+}
+
+Tensor int4_linear(const Tensor& x, const Tensor& weight, int64_t N, int64_t group, const optional<Tensor>& bias, bool gelu) {
+  const int type = type_of("x", x);
+  TORCH_CHECK_VALUE(x.dim() > 0, "x: expected (..., K), got a single value");
+  const int64_t K = x.size(-1);
+  TORCH_CHECK_VALUE(N > 0 && N < INT_MAX && K > 0 && K < INT_MAX, "x ", x.sizes(), " and N = ", N, ": sizes must be positive and below 2^31");
+  const auto bytes = static_cast<int64_t>(int4_weight_bytes(static_cast<int>(N), static_cast<int>(K), static_cast<int>(group)));
+  TORCH_CHECK(weight.device() == x.device() && (!bias || bias->device() == x.device()), "weight and bias must live on x's device, ", x.device());
+  TORCH_CHECK_VALUE(bytes > 0 && weight.scalar_type() == at::kByte && weight.is_contiguous() && weight.numel() == bytes, "weight: expected ", bytes, " bytes for (", N, ", ", K,
+                    ") in groups of ", group, ", got ", weight.scalar_type(), " ", weight.sizes());
+  TORCH_CHECK_VALUE(!bias || (bias->scalar_type() == at::kFloat && bias->is_contiguous() && bias->dim() == 1 && bias->numel() == N), "bias: expected float32 (", N, ")");
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  const c10::DeviceGuard guard(x.device());
+  Tensor out = at::empty(shape, x.options().requires_grad(false));
+  const int64_t M = x.numel() / K;
+  if (M == 0) return out;
+  TORCH_CHECK_VALUE(M < INT_MAX, "x: below 2^31 rows, got ", M);
+  const Rows r = rows_of(x, 1);
+  check(int4_linear_fwd(r.t.data_ptr(), r.row, weight.data_ptr(), bias ? bias->data_ptr<float>() : nullptr, out.data_ptr(), static_cast<int>(M), static_cast<int>(N),
+                        static_cast<int>(K), static_cast<int>(group), gelu, type, current_stream()));
+  return out;
+}
+
+// What both directions take of the arguments.
+struct Scores {
+  int type;
+  int64_t V, rows, top_k, ignore_index, allowed_row = 0;
+  Tensor tokens, allowed;
+};
+Scores arguments(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
+  Scores s;
+  s.type = type_of("logits", logits);
+  TORCH_CHECK_VALUE(logits.dim() > 0 && logits.size(-1) > 0, "logits: expected (..., V), got ", logits.sizes());
+  s.V = logits.size(-1);
+  s.rows = logits.numel() / s.V;
+  s.top_k = top_k;
+  s.ignore_index = ignore_index;
+  TORCH_CHECK_VALUE(s.V <= 1 << 30 && s.rows < INT_MAX, "logits: at most 2^30 values in a row and below 2^31 rows, got ", logits.sizes());
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= std::min<int64_t>(32, s.V), "top_k must lie in 0 .. ", std::min<int64_t>(32, s.V), ", got ", top_k);
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  if (tokens) {
+    TORCH_CHECK_VALUE(tokens->scalar_type() == at::kLong && tokens->sizes() == lead && tokens->device() == logits.device(), "tokens: expected int64 ", lead, " on ",
+                      logits.device(), ", got ", tokens->scalar_type(), " ", tokens->sizes(), " on ", tokens->device());
+    s.tokens = tokens->contiguous();
+  }
+  if (allowed) {
+    const bool one = allowed->dim() == 1 && allowed->size(0) == s.V;
+    TORCH_CHECK_VALUE(allowed->scalar_type() == at::kBool && (one || allowed->sizes() == logits.sizes()) && allowed->device() == logits.device(), "allowed: expected bool (",
+                      s.V, ") or ", logits.sizes(), " on ", logits.device(), ", got ", allowed->scalar_type(), " ", allowed->sizes(), " on ", allowed->device());
+    if (one) {
+      s.allowed = allowed->contiguous();
+    } else {
+      const Rows r = rows_of(*allowed, 1);
+      // rows that overlap (one list expanded to all) are one list where there is nothing else
+      const bool shared = r.row == 0 && r.inner > 1;
+      s.allowed = shared || r.row >= s.V || r.inner == 1 ? r.t : allowed->contiguous();
+      s.allowed_row = shared ? 0 : std::max(s.V, s.allowed.is_same(r.t) ? r.row : s.V);
+    }
+  }
+  return s;
+}
+
+struct Found {
+  Tensor logprobs, entropy, stats, ids, top;
+};
+Found scores(const Tensor& logits, const Scores& s) {
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
+  const c10::DeviceGuard guard(logits.device());
+  Found f;
+  if (s.tokens.defined()) f.logprobs = at::empty(lead, f32);
+  f.entropy = at::empty(lead, f32);
+  f.stats = at::empty({s.rows, 2}, f32);
+  if (s.top_k) {
+    c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
+    shape.push_back(s.top_k);
+    f.ids = at::empty(shape, f32.dtype(at::kLong));
+    f.top = at::empty(shape, f32);
+  }
+  if (s.rows == 0) return f;
+  const Rows r = rows_of(logits, 2);
+  const auto bytes = static_cast<int64_t>(token_scores_workspace_bytes(s.rows, static_cast<int>(s.V), s.type));
+  const Tensor workspace = bytes ? at::empty({bytes}, f32.dtype(at::kByte)) : Tensor();
+  check(token_scores_fwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(s.tokens)), s.ignore_index,
+                         static_cast<const unsigned char*>(pointer(s.allowed)), s.allowed_row, static_cast<float*>(pointer(f.logprobs)), f.entropy.data_ptr<float>(),
+                         f.stats.data_ptr<float>(), static_cast<long long*>(pointer(f.ids)), static_cast<float*>(pointer(f.top)), pointer(workspace), s.rows,
+                         static_cast<int>(s.V), static_cast<int>(s.top_k), s.type, current_stream()));
+  return f;
+}
+
+// A gradient of one value a row: it may be one value for all of them.
+Tensor per_row(const Tensor& g) { return g.defined() ? g.reshape({-1}) : g; }
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed,
+                               int64_t ignore_index) {
+    const Scores s = arguments(logits, tokens, top_k, allowed, ignore_index);
+    const Found f = scores(logits, s);
+    ctx->save_for_backward({logits, s.tokens, s.allowed, f.entropy, f.stats, f.ids});
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["allowed_row"] = s.allowed_row;
+    ctx->set_materialize_grads(false);
+    if (f.ids.defined()) ctx->mark_non_differentiable({f.ids});
+    variable_list out = {f.entropy};      // all outputs are defined: the entropy, the log probabilities where there are tokens, alternatives' ids and log probabilities
+    if (s.tokens.defined()) out.push_back(f.logprobs);
+    if (top_k) out.push_back(f.ids), out.push_back(f.top);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &tokens = saved[1], &allowed = saved[2], &entropy = saved[3], &stats = saved[4], &ids = saved[5];
+    const int64_t top_k = ctx->saved_data["top_k"].toInt();
+    const Tensor g_entropy = g[0], g_logprobs = tokens.defined() ? g[1] : Tensor(), g_alternatives = top_k ? g.back() : Tensor();
+    if (!g_entropy.defined() && !g_logprobs.defined() && !g_alternatives.defined()) return variable_list(5);
+    Tensor grad;
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const c10::DeviceGuard guard(logits.device());
+      const int64_t V = logits.size(-1), rows = logits.numel() / V;
+      grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      if (rows) {
+        const Tensor g_lp = per_row(g_logprobs), g_h = per_row(g_entropy),
+                     g_top = g_alternatives.defined() ? g_alternatives.contiguous() : g_alternatives;
+        const Rows r = rows_of(logits.detach(), 2);
+        check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(tokens)), ctx->saved_data["ignore_index"].toInt(),
+                               static_cast<const unsigned char*>(pointer(allowed)), ctx->saved_data["allowed_row"].toInt(), entropy.data_ptr<float>(), stats.data_ptr<float>(),
+                               static_cast<const long long*>(pointer(ids)), static_cast<const float*>(pointer(g_lp)), g_lp.defined() ? g_lp.stride(0) : 0,
+                               static_cast<const float*>(pointer(g_h)), g_h.defined() ? g_h.stride(0) : 0, static_cast<const float*>(pointer(g_top)), grad.data_ptr(), V, rows,
+                               static_cast<int>(V), static_cast<int>(top_k), logits.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16, current_stream()));
+      }
+    }
+    if (at::GradMode::is_enabled()) {      // a graph of the backward pass is made: what is asked of it later has to fail
+      auto node = std::make_shared<torch::autograd::DelayedError>("token_logprobs has no second derivative", 1);
+      grad.set_requires_grad(true);
+      grad = (*node)({grad})[0];
+    }
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+using Results = std::tuple<optional<Tensor>, Tensor, optional<Tensor>, optional<Tensor>>;      // logprobs, entropy, ids, log probabilities of the alternatives
+
+optional<Tensor> given(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
+
+Results token_logprobs(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
+  if (logits.requires_grad() && at::GradMode::is_enabled()) {
+    const variable_list v = TokenLogprobs::apply(logits, tokens, top_k, allowed, ignore_index);
+    const bool has = tokens.has_value();
+    return {has ? given(v[1]) : std::nullopt, v[0], top_k ? given(v[1 + has]) : std::nullopt, top_k ? given(v[2 + has]) : std::nullopt};
+  }
+  const Found f = scores(logits, arguments(logits, tokens, top_k, allowed, ignore_index));
+  return {given(f.logprobs), f.entropy, given(f.ids), given(f.top)};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_answer_calls, m) {
+  m.def("bind", torch::wrap_pybind_function(bind));
+  m.def("int4_linear", torch::wrap_pybind_function_no_gil(int4_linear));
+  m.def("token_logprobs", torch::wrap_pybind_function_no_gil(token_logprobs));
+}

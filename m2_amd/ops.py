@@ -13,10 +13,14 @@ from typing import Optional, Sequence
 import torch
 from torch.autograd.forward_ad import unpack_dual as _unpack_dual
 
-from . import _lib
+from . import _answer_calls, _lib
 from ._lib import HyenaFilterParams, SplitJob, M2_DTYPE_BF16, M2_DTYPE_F32, check, lib
 
 Tensor = torch.Tensor
+
+# what the calls of Int4Linear and token_logprobs need of the library that _lib has loaded
+_answer_calls.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+    "m2_last_error", "m2_int4_weight_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd")])
 
 
 # handle of the current stream of a device: 0.3 us, where torch.cuda.current_stream() makes an object in 3 us
@@ -752,145 +756,20 @@ def require_values(t: Tensor, name: str, grad_ok: bool = False) -> None:
         raise RuntimeError(f"{name}: this operator has no gradient; call it under torch.no_grad() or on a detached tensor")
 
 
-class _on_device:
-    """The device of a tensor as the current one, for the launches inside."""
-
-    def __init__(self, t: Tensor):
-        self.index, self.before = t.device.index, -1
-
-    def __enter__(self):
-        at = torch._C._cuda_getDevice()
-        if at != self.index:
-            torch.cuda.set_device(self.index)
-            self.before = at
-
-    def __exit__(self, *_):
-        if self.before >= 0:
-            torch.cuda.set_device(self.before)
-
-
 def int4_weight_bytes(N: int, K: int, group: int) -> int:
     return lib.m2_int4_weight_bytes(N, K, group)
-
-
-def _rows_apart(t: Tensor):
-    """t (..., n) -> (t or a copy of it, inner, outer, row): row r of its leading dimensions lies (r // inner) * outer + (r % inner) * row values behind
-    the first; a copy where its values lie apart, or its rows at more than two distances."""
-    if t.dim() == 2 and t.stride(1) == 1:
-        return t, max(t.shape[0], 1), 0, t.stride(0)
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        t = t.contiguous()
-    dims = []
-    for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
-        if size == 1:
-            continue
-        if dims and dims[-1][1] == size * stride:
-            dims[-1] = (dims[-1][0] * size, stride)
-        else:
-            dims.append((size, stride))
-    if len(dims) > 2:
-        return _rows_apart(t.contiguous())
-    if not dims:
-        return t, 1, 0, 0
-    if len(dims) == 1:
-        return t, max(dims[0][0], 1), 0, dims[0][1]
-    return t, max(dims[1][0], 1), dims[0][1], dims[1][1]
 
 
 def int4_linear(x: Tensor, weight: Tensor, N: int, group: int, bias: Optional[Tensor] = None, activation: Optional[str] = None) -> Tensor:
     """act(x W^T + bias): x (..., K) fp32 or bf16, weight uint8 in the order of m2_int4_linear_fwd, bias (N) fp32 -> (..., N) of x's type."""
     require_values(x, "x")
-    if not x.is_cuda:
-        raise RuntimeError(f"x: must live on the GPU (m2_amd has no CPU path); got device {x.device}")
-    code = _act_code(x.dtype)
-    if x.dim() == 0:
-        raise ValueError("x: expected (..., K), got a single value")
-    K = x.shape[-1]
-    if activation not in (None, "gelu"):
+    if activation is not None and activation != "gelu":
         raise ValueError(f'activation must be None or "gelu", got {activation!r}')
-    nbytes = lib.m2_int4_weight_bytes(N, K, group) if K else 0
-    if nbytes == 0 or weight.numel() != nbytes:
-        raise ValueError(f"weight holds {weight.numel()} bytes, ({N}, {K}) in groups of {group} takes {nbytes}")
-    _require(weight, "weight", torch.uint8)
-    if weight.device != x.device or (bias is not None and bias.device != x.device):
-        raise RuntimeError(f"weight and bias must live on x's device, {x.device}")
-    if bias is not None:
-        _require(bias, "bias", torch.float32, (N,))
-    M = x.numel() // K
-    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    if M == 0:
-        return out
-    x, inner, outer, row = _rows_apart(x)
-    if inner < M:                                 # rows at two distances
-        x, row = x.reshape(M, K), K
-    with _on_device(x):
-        check(lib.m2_int4_linear_fwd(x.data_ptr(), row, weight.data_ptr(), _ptr(bias), out.data_ptr(), M, N, K, group, activation is not None, code, _stream()))
-    return out
+    return _answer_calls.int4_linear(x, weight, N, group, bias, activation is not None)
 
 
-def _scores_arguments(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: Optional[Tensor]):
-    if not logits.is_cuda:
-        raise RuntimeError(f"logits: must live on the GPU (m2_amd has no CPU path); got device {logits.device}")
-    code = _act_code(logits.dtype)
-    if logits.dim() == 0 or logits.shape[-1] == 0:
-        raise ValueError(f"logits: expected (..., V), got {tuple(logits.shape)}")
-    lead, V = logits.shape[:-1], logits.shape[-1]
-    if not 0 <= top_k <= min(32, V):
-        raise ValueError(f"top_k must lie in 0 .. {min(32, V)}, got {top_k}")
-    if tokens is not None:
-        if tokens.dtype != torch.int64 or tokens.shape != lead or tokens.device != logits.device:
-            raise ValueError(f"tokens: expected int64 {tuple(lead)} on {logits.device}, got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
-        tokens = tokens.contiguous()
-    allowed_row = 0
-    if allowed is not None:
-        if allowed.dtype != torch.bool or allowed.device != logits.device or (allowed.shape != logits.shape and allowed.shape != (V,)):
-            raise ValueError(f"allowed: expected bool ({V},) or {tuple(logits.shape)} on {logits.device}, got {allowed.dtype} {tuple(allowed.shape)} on {allowed.device}")
-        if allowed.dim() > 1:
-            allowed = allowed.reshape(-1, V)
-            if allowed.stride(1) != 1 or allowed.stride(0) < V:
-                allowed = allowed.contiguous()
-            allowed_row = allowed.stride(0)
-        else:
-            allowed = allowed.contiguous()
-    return code, lead, V, tokens, allowed, allowed_row
-
-
-def token_scores(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: Optional[Tensor], ignore_index: int):
-    """-> (log probabilities of `tokens` | None, entropies, what the gradient needs of the rows, alternatives' ids | None, their log probabilities | None); see
-    scores.token_logprobs."""
-    code, lead, V, tokens, allowed, allowed_row = _scores_arguments(logits, tokens, top_k, allowed)
-    rows = logits.numel() // V
-    dev = logits.device
-    lp = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
-    h = torch.empty(lead, dtype=torch.float32, device=dev)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
-    ids = top = None
-    if top_k:
-        ids = torch.empty(*lead, top_k, dtype=torch.int64, device=dev)
-        top = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
-    if rows:
-        x, inner, outer, row = _rows_apart(logits)
-        nbytes = lib.m2_token_scores_workspace_bytes(rows, V, code)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with _on_device(x):
-            check(lib.m2_token_scores_fwd(x.data_ptr(), inner, outer, row, _ptr(tokens), ignore_index, _ptr(allowed), allowed_row, _ptr(lp), h.data_ptr(),
-                                          stats.data_ptr(), _ptr(ids), _ptr(top), _ptr(workspace), rows, V, top_k, code, _stream()))
-    return lp, h, stats, ids, top
-
-
-def token_scores_grad(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: Optional[Tensor], ignore_index: int, entropy: Tensor, stats: Tensor,
-                      top_ids: Optional[Tensor], g_logprobs: Optional[Tensor], g_entropy: Optional[Tensor], g_top: Optional[Tensor]) -> Tensor:
-    """Gradient of the logits for gradients of the three outputs (None: not asked for)."""
-    code, lead, V, tokens, allowed, allowed_row = _scores_arguments(logits, tokens, top_k, allowed)
-    rows = logits.numel() // V
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if rows:
-        g_lp = None if g_logprobs is None else g_logprobs.reshape(-1)
-        g_h = None if g_entropy is None else g_entropy.reshape(-1)
-        g_top = None if g_top is None else g_top.contiguous()
-        x, inner, outer, row = _rows_apart(logits)
-        with _on_device(x):
-            check(lib.m2_token_scores_bwd(x.data_ptr(), inner, outer, row, _ptr(tokens), ignore_index, _ptr(allowed), allowed_row, entropy.data_ptr(),
-                                          stats.data_ptr(), _ptr(top_ids), _ptr(g_lp), 0 if g_lp is None else g_lp.stride(0), _ptr(g_h),
-                                          0 if g_h is None else g_h.stride(0), _ptr(g_top), grad.data_ptr(), V, rows, V, top_k, code, _stream()))
-    return grad
+def token_logprobs(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: Optional[Tensor], ignore_index: int):
+    """-> (log probabilities of `tokens` | None, entropies, alternatives' ids | None, their log probabilities | None), with a gradient where the logits ask for one;
+    see scores.token_logprobs."""
+    require_values(logits, "logits", grad_ok=True)
+    return _answer_calls.token_logprobs(logits, tokens, top_k, allowed, ignore_index)

@@ -9,7 +9,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -20,27 +19,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor                     # of the row's distribution, in nats
     top_ids: Optional[torch.Tensor]           # the most likely tokens, most likely first, equal ones by id; None for top_k = 0
     top_logprobs: Optional[torch.Tensor]
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top_k, allowed, ignore_index):
-        lp, h, stats, ids, top = ops.token_scores(logits, tokens, top_k, allowed, ignore_index)
-        ctx.save_for_backward(logits, tokens, allowed, h, stats, ids)
-        ctx.top_k, ctx.ignore_index = top_k, ignore_index
-        ctx.set_materialize_grads(False)
-        if ids is not None:
-            ctx.mark_non_differentiable(ids)
-        return lp, h, ids, top
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_h, _, g_top):
-        if g_lp is None and g_h is None and g_top is None:
-            return (None,) * 5
-        logits, tokens, allowed, h, stats, ids = ctx.saved_tensors
-        grad = ops.token_scores_grad(logits, tokens, ctx.top_k, allowed, ctx.ignore_index, h, stats, ids, g_lp, g_h, g_top)
-        return grad, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0, allowed: Optional[torch.Tensor] = None,
@@ -55,8 +33,4 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 
     Differentiable once with respect to `logits`: log probabilities, entropy and the alternatives' log probabilities (their ids are taken
     as given).  Arithmetic is fp32; rows may lie any distance apart."""
-    ops.require_values(logits, "logits", grad_ok=True)
-    if logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, allowed, ignore_index))
-    lp, h, _, ids, top = ops.token_scores(logits, tokens, top_k, allowed, ignore_index)
-    return TokenLogprobs(lp, h, ids, top)
+    return TokenLogprobs(*ops.token_logprobs(logits, tokens, top_k, allowed, ignore_index))
