@@ -111,16 +111,20 @@ struct Scales {
   __device__ __forceinline__ float get(int g) const { return __uint_as_float(g % 2 ? v[g / 2] & 0xffff0000u : v[g / 2] << 16); }
 };
 
-// One tile of 128 columns for all: what a wave has asked for, and what it makes of it.
-template <typename T, int GROUP, bool EVEN>
+// 128 columns of x's rows and of NT tiles of W: what a wave has asked for, and what it makes of it.
+template <typename T, int GROUP, bool EVEN, int NT>
 struct Step {
-  u32x4 q;
-  Scales<GROUP> s;
+  u32x4 q[NT];
+  Scales<GROUP> s[NT];
   Operand<T> x[4];
-  __device__ __forceinline__ void load(const unsigned char* w, const T* row, int b, int K, int lane) {
-    const unsigned char* p = w + (long)b * tile_bytes(GROUP);
-    q = *reinterpret_cast<const u32x4*>(p + lane * 16);
-    s.load(p, lane);
+  // `w`: the first tile's part, the others' `apart` bytes behind one another; those from `tiles` on are the last one again
+  __device__ __forceinline__ void load(const unsigned char* w, long apart, int tiles, const T* row, int b, int K, int lane) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const unsigned char* p = w + min(t, tiles - 1) * apart + (long)b * tile_bytes(GROUP);
+      q[t] = *reinterpret_cast<const u32x4*>(p + lane * 16);
+      s[t].load(p, lane);
+    }
     const int k = b * kTileK + (lane >> 4) * 8;
     if ((b + 1) * kTileK <= K) {
 #pragma unroll
@@ -130,22 +134,26 @@ struct Step {
       for (int i = 0; i < 4; ++i) load_edge<T, EVEN>(x[i], row, k + i * 32, K);
     }
   }
-  __device__ __forceinline__ void add(floatx4& sum, int lane) const {
+  __device__ __forceinline__ void add(floatx4 (&sum)[NT], int lane) const {
+    constexpr int kSteps = GROUP / 32;
 #pragma unroll
     for (int g = 0; g < kTileK / GROUP; ++g) {
-      constexpr int kSteps = GROUP / 32;
       bf16x8 a[kSteps];
-      floatx4 c = {0.f, 0.f, 0.f, 0.f};
+      floatx4 c0 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         a[i] = x[g * kSteps + i].get(lane);
-        c = mfma(a[i], minus24(), c);
+        c0 = mfma(a[i], minus24(), c0);
       }
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes(q[g * kSteps + i]), c);
-      const float scale = s.get(g);
+      for (int t = 0; t < NT; ++t) {
+        floatx4 c = c0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = fmaf(scale, c[i], sum[i]);
+        for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes(q[t][g * kSteps + i]), c);
+        const float scale = s[t].get(g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(scale, c[i], sum[t][i]);
+      }
     }
   }
 };
@@ -156,44 +164,57 @@ __device__ __forceinline__ void put(T* out, long at, float y, int gelu) {
   if constexpr (sizeof(T) == 4) out[at] = y; else out[at] = f32_to_bf16(y);
 }
 
-// Up to 16 rows of bf16 or 4 of fp32.  SPLIT waves share the columns of a tile of 16 rows of W, each every SPLIT-th tile of 128; their sums meet in shared memory.
-template <typename T, int GROUP, bool EVEN, int SPLIT>
-__global__ __launch_bounds__(256) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
+constexpr int waves_of(int split) { return split > 4 ? split : 4; }
+
+// Up to 16 rows of bf16 or 4 of fp32.  A wave has NT tiles of 16 rows of W, and of their tiles of 128 columns every SPLIT-th; the SPLIT waves' sums meet in shared
+// memory.
+template <typename T, int GROUP, bool EVEN, int NT, int SPLIT>
+__global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
                                                             T* __restrict__ out, int M, int N, int K, int gelu) {
-  __shared__ floatx4 sums[SPLIT > 1 ? 4 : 1][64];
+  __shared__ floatx4 sums[SPLIT > 1 ? waves_of(SPLIT) : 1][SPLIT > 1 ? NT : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
-  const int tile = (int)blockIdx.x * (4 / SPLIT) + wave / SPLIT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
-  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-  if (tile < tiles) {
-    const unsigned char* mine = w + (long)tile * kt * tile_bytes(GROUP);
+  const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
+  floatx4 sum[NT] = {};
+  if (t0 < tiles) {
+    const long apart = (long)kt * tile_bytes(GROUP);
+    const unsigned char* mine = w + t0 * apart;
     const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
-    Step<T, GROUP, EVEN> now, next;
-    if (part < kt) now.load(mine, row, part, K, lane);
+    Step<T, GROUP, EVEN, NT> now, next;
+    if (part < kt) now.load(mine, apart, tiles - t0, row, part, K, lane);
     for (int b = part; b < kt; b += SPLIT) {
-      if (b + SPLIT < kt) next.load(mine, row, b + SPLIT, K, lane);
+      if (b + SPLIT < kt) next.load(mine, apart, tiles - t0, row, b + SPLIT, K, lane);
       now.add(sum, lane);
       now = next;
     }
   }
   if (SPLIT > 1) {
-    sums[wave][lane] = sum;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sums[wave][t][lane] = sum[t];
     __syncthreads();
-    if (part) return;
-#pragma unroll
-    for (int i = 1; i < SPLIT; ++i) sum += sums[wave + (SPLIT > 1 ? i : 0)][lane];
+    if (NT == 1 && part) return;
   }
-  const int n = tile * kTileN + (lane & 15);
-  if (n >= N) return;
-  const float b = bias ? bias[n] : 0.f;
-  if constexpr (sizeof(T) == 4) {
-    const int m = m0 + (lane >> 4);
-    if (m < M) put(out, (long)m * N + n, (sum[2] + sum[1]) + sum[0] + b, gelu);
-  } else {
+  // with more than one tile the waves share them out
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = m0 + (lane >> 4) * 4 + i;
-      if (m < M) put(out, (long)m * N + n, sum[i] + b, gelu);
+  for (int t = 0; t < NT; ++t) {
+    if (SPLIT > 1) {
+      if (NT > 1 && t % SPLIT != part) continue;
+      sum[t] = sums[wave - part][t][lane];
+#pragma unroll
+      for (int i = 1; i < SPLIT; ++i) sum[t] += sums[wave - part + i][t][lane];
+    }
+    const int n = (t0 + t) * kTileN + (lane & 15);
+    if (n >= N) continue;
+    const float b = bias ? bias[n] : 0.f;
+    if constexpr (sizeof(T) == 4) {
+      const int m = m0 + (lane >> 4);
+      if (m < M) put(out, (long)m * N + n, (sum[t][2] + sum[t][1]) + sum[t][0] + b, gelu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = m0 + (lane >> 4) * 4 + i;
+        if (m < M) put(out, (long)m * N + n, sum[t][i] + b, gelu);
+      }
     }
   }
 }
@@ -340,12 +361,11 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   if ((uintptr_t)x % size || (uintptr_t)out % size || (uintptr_t)bias % 4) return set_error(M2_ERR_UNSUPPORTED, "%s: x, out and bias must be aligned to their type", who);
   hipStream_t st = (hipStream_t)stream;
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
-  // eight waves a compute unit, where there are as many
-  const int split = K % 8 ? 4 : tiles >= 2048 || kt < 2 ? 1 : tiles >= 1024 || kt < 4 ? 2 : 4;
-  const auto go = [&](auto kernel, auto* t) {
+  const auto go = [&](auto kernel, auto* t, int nt, int split) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const dim3 grid((unsigned)((tiles * (long)split + 3) / 4), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows));
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
+    const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((waves + each - 1) / each), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows)), dim3(64 * each), 0, st, (const T*)x, x_row,
+                       (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
   };
   const auto rows = [&](auto kernel, auto* t, int mt, int nt) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -364,10 +384,15 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
       if (blocks < 512) return rows(int4_rows_kernel<T, G, true, kMt, 1>, t, kMt, 1);
       return rows(int4_rows_kernel<T, G, true, kMt, 2>, t, kMt, 2);
     }
-    if (K % 8) return go(int4_few_rows_kernel<T, G, false, 4>, t);
-    if (split == 1) go(int4_few_rows_kernel<T, G, true, 1>, t);
-    else if (split == 2) go(int4_few_rows_kernel<T, G, true, 2>, t);
-    else go(int4_few_rows_kernel<T, G, true, 4>, t);
+    // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
+    // long rows are shared by eight waves.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
+    // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
+    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7.
+    if (K % 8) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
+    if (tiles < 384) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
+    if (tiles >= 1024 && (sizeof(T) == 4 || M > 8))
+      return kt < 16 ? go(int4_few_rows_kernel<T, G, true, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, true, 4, 8>, t, 4, 8);
+    return kt < 16 ? go(int4_few_rows_kernel<T, G, true, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, true, 2, 8>, t, 2, 8);
   };
   const auto pick = [&](auto* t) {
     if (group == 32) parts(t, std::integral_constant<int, 32>{});
