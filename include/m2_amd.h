@@ -379,11 +379,14 @@ int m2_encoder_layers_taps_fwd(const m2_layer_params* layers, int nlayers, const
  *   y (M, N) = act(x W^T + bias),  W[n, k] = (q - 8) * s,  q in 0 .. 15,  s bf16, one for each `group` (32, 64 or 128) values of a row
  * `weight` (m2_int4_weight_bytes, 0: unsupported; 16-byte aligned) holds tiles of 16 rows by 128 columns, all tiles of 16 rows behind one another:
  * 64 lanes times 16 bytes, lane 16 * (k / 8 % 4) + n % 16, with one 32-bit word for each of four steps of 32 columns, value j = k % 8 at bit
- * 16 * (j % 2) + 4 * (j / 2); then 16 rows times 128 / group scales.  Rows and columns beyond N and K hold q = 8 and s = 0.
+ * 16 * (j % 2) + 4 * (j / 2); then 16 rows times 128 / group scales.  Rows and columns beyond N and K hold q = 8 and s = 0.  Behind all tiles 16
+ * fp32 factors for each 16 rows: the power of two that takes the row's largest scale to [1 / 2, 1) (1 where that is 0 or not finite).
+ * `workspace`: m2_int4_workspace_bytes, 16-byte aligned (0: NULL does).
  * x: M rows of K values, `x_row` values apart, fp32 or bf16; y of the same type, dense; bias (N) fp32 or NULL; gelu: 0 none, 1 erf-GELU. */
 size_t m2_int4_weight_bytes(int N, int K, int group);
-int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, int M, int N, int K, int group,
-                       int gelu, int dtype, void* stream);
+size_t m2_int4_workspace_bytes(int M, int N, int K, int dtype);
+int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, void* workspace, int M, int N, int K,
+                       int group, int gelu, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Log probabilities of given tokens, entropies and the most likely alternatives from logits, and their gradient (the loss behind the

@@ -156,8 +156,10 @@ def _load() -> ctypes.CDLL:
     lib.m2_encoder_layers_taps_fwd.argtypes = [c_void_p, c_int] + [c_void_p] * 2 + [c_int] + [c_void_p] * 4 + [c_int] * 5 + [c_float, c_void_p]
     lib.m2_int4_weight_bytes.restype = c_size_t
     lib.m2_int4_weight_bytes.argtypes = [c_int] * 3
+    lib.m2_int4_workspace_bytes.restype = c_size_t
+    lib.m2_int4_workspace_bytes.argtypes = [c_int] * 4
     lib.m2_int4_linear_fwd.restype = c_int
-    lib.m2_int4_linear_fwd.argtypes = [c_void_p, c_long] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p]
+    lib.m2_int4_linear_fwd.argtypes = [c_void_p, c_long] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p]
     lib.m2_token_scores_workspace_bytes.restype = c_size_t
     lib.m2_token_scores_workspace_bytes.argtypes = [c_long, c_int, c_int]
     lib.m2_token_scores_fwd.restype = c_int
@@ -176,7 +178,7 @@ EXPORTS = ["m2_version", "m2_last_error", "m2_hyena_filter_workspace_bytes", "m2
            "m2_fftconv_fwd", "m2_dense_supported", "m2_dense_to_channels_fwd", "m2_dense_to_channels_rows_fwd", "m2_dense_channels_row", "m2_dense_from_channels_fwd", "m2_layernorm_to_channels_supported", "m2_layernorm_to_channels_fwd", "m2_blockdiag_glu_fwd", "m2_blockdiag_glu_few_rows", "m2_blockdiag_linear_fwd", "m2_blockdiag_linear_f32_fwd", "m2_mlp_fused_supported", "m2_mlp_fused_packed_bytes", "m2_mlp_fused_pack", "m2_mlp_fused_fwd", "m2_glu_stream_supported", "m2_glu_stream_packed_bytes", "m2_glu_stream_pack", "m2_glu_stream_fwd", "m2_layernorm_fwd", "m2_layernorm_bf16_fwd", "m2_input_forms_fwd", "m2_pooler_fwd",
            "m2_embed_layernorm_fwd", "m2_blockdiag_linear_layernorm_supported", "m2_blockdiag_linear_layernorm_fwd", "m2_encoder_layers_workspace_bytes", "m2_encoder_layers_fwd", "m2_encoder_layers_taps_fwd",
            "m2_split_bytes", "m2_split_rows_fwd", "m2_split_jobs_fwd", "m2_split_channels_fwd", "m2_split_to_channels_fwd", "m2_split_linear_fwd", "m2_split_glu_fwd",
-           "m2_int4_weight_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd"]
+           "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd"]
 
 
 def check(rc: int) -> None:

@@ -21,6 +21,7 @@ using std::optional;
 // The entry points of libm2_amd.so, which m2_amd/_lib.py has loaded.
 decltype(&m2_last_error) last_error;
 decltype(&m2_int4_weight_bytes) int4_weight_bytes;
+decltype(&m2_int4_workspace_bytes) int4_workspace_bytes;
 decltype(&m2_int4_linear_fwd) int4_linear_fwd;
 decltype(&m2_token_scores_workspace_bytes) token_scores_workspace_bytes;
 decltype(&m2_token_scores_fwd) token_scores_fwd;
@@ -30,13 +31,14 @@ template <typename F>
 void set(F& f, uintptr_t address) { f = reinterpret_cast<F>(address); }
 
 void bind(std::vector<uintptr_t> a) {
-  TORCH_CHECK(a.size() == 6, "six addresses");
+  TORCH_CHECK(a.size() == 7, "seven addresses");
   set(last_error, a[0]);
   set(int4_weight_bytes, a[1]);
-  set(int4_linear_fwd, a[2]);
-  set(token_scores_workspace_bytes, a[3]);
-  set(token_scores_fwd, a[4]);
-  set(token_scores_bwd, a[5]);
+  set(int4_workspace_bytes, a[2]);
+  set(int4_linear_fwd, a[3]);
+  set(token_scores_workspace_bytes, a[4]);
+  set(token_scores_fwd, a[5]);
+  set(token_scores_bwd, a[6]);
 }
 
 void check(int rc) { TORCH_CHECK(rc == M2_OK, "libm2_amd error ", rc, ": ", last_error()); }
@@ -93,7 +95,9 @@ Tensor int4_linear(const Tensor& x, const Tensor& weight, int64_t N, int64_t gro
   if (M == 0) return out;
   TORCH_CHECK_VALUE(M < INT_MAX, "x: below 2^31 rows, got ", M);
   const Rows r = rows_of(x, 1);
-  check(int4_linear_fwd(r.t.data_ptr(), r.row, weight.data_ptr(), bias ? bias->data_ptr<float>() : nullptr, out.data_ptr(), static_cast<int>(M), static_cast<int>(N),
+  const auto scratch = static_cast<int64_t>(int4_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), type));
+  const Tensor workspace = scratch ? at::empty({scratch}, weight.options()) : Tensor();
+  check(int4_linear_fwd(r.t.data_ptr(), r.row, weight.data_ptr(), bias ? bias->data_ptr<float>() : nullptr, out.data_ptr(), pointer(workspace), static_cast<int>(M), static_cast<int>(N),
                         static_cast<int>(K), static_cast<int>(group), gelu, type, current_stream()));
   return out;
 }

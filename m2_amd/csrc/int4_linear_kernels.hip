@@ -4,13 +4,14 @@
 //
 // Order of the weights in memory: tiles of 16 rows n by 128 columns k, those of the same rows behind one another.  A tile is 64 lanes times 16 bytes, lane l
 // = 16 (k / 8 % 4) + n % 16 with the eight k of each of the four steps of 32 in a 32-bit word, value j of the eight at bit 16 (j % 2) + 4 (j / 2); behind them
-// 16 rows times 128 / group scales.  K and N are padded with q = 8 and scale 0.
+// 16 rows times 128 / group scales.  K and N are padded with q = 8 and scale 0.  Behind all tiles a factor for each row, a power of two.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <type_traits>
 
 #include "m2_internal.h"
+#include "mfma_stream.h"
 
 namespace m2 {
 
@@ -20,17 +21,24 @@ constexpr int tile_bytes(int group) { return 64 * 16 + kTileN * (kTileK / group)
 
 __device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f)); }
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) u32x4_any;      // at any address of x's type
+typedef uint32_t __attribute__((ext_vector_type(2), aligned(2))) u32x2_any;
+
+// (q & mask) | bits as one instruction, which takes one scalar register and no literals: the compiler is kept from knowing the two constants.
+struct Codes {
+  uint32_t mask, bits;
+  __device__ __forceinline__ Codes(uint32_t m, uint32_t b) : mask(m), bits(b) { asm volatile("" : "+s"(mask), "+v"(bits)); }
+  __device__ __forceinline__ uint32_t operator()(uint32_t q) const { return (q & mask) | bits; }
+};
 
 // Eight codes as bf16 16 + q, exactly: 0x4180 is 16, and its last bits but three are worth 1 each.  What a row of x sums to, times 24, is taken off again.
-__device__ __forceinline__ bf16x8 codes(uint32_t q) {
-  const u32x4 v = {((q << 3) & 0x00780078u) | 0x41804180u, ((q >> 1) & 0x00780078u) | 0x41804180u, ((q >> 5) & 0x00780078u) | 0x41804180u,
-                   ((q >> 9) & 0x00780078u) | 0x41804180u};
-  return __builtin_bit_cast(bf16x8, v);
-}
+struct Bf16Codes : Codes {
+  __device__ __forceinline__ Bf16Codes() : Codes(0x00780078u, 0x41804180u) {}
+  __device__ __forceinline__ bf16x8 get(uint32_t q) const {
+    const Codes& c = *this;
+    return __builtin_bit_cast(bf16x8, u32x4{c(q << 3), c(q >> 1), c(q >> 5), c(q >> 9)});
+  }
+};
 __device__ __forceinline__ bf16x8 minus24() {
   const u32x4 v = {0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};
   return __builtin_bit_cast(bf16x8, v);
@@ -52,6 +60,10 @@ template <> struct Operand<uint16_t> {
   }
   __device__ __forceinline__ void keep(bool is) { v = is ? v : u32x4{0, 0, 0, 0}; }
   __device__ __forceinline__ bf16x8 get(int) const { return __builtin_bit_cast(bf16x8, v); }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
 };
 template <> struct Operand<float> {
   static constexpr int kRows = 4;
@@ -66,6 +78,10 @@ template <> struct Operand<float> {
     for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = i < n ? __float_as_uint(p[i]) : 0u;
   }
   __device__ __forceinline__ void keep(bool is) { v[0] = is ? v[0] : u32x4{0, 0, 0, 0}, v[1] = is ? v[1] : u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i / 4][i % 4]);
+  }
   __device__ __forceinline__ bf16x8 get(int lane) const {
     const uint32_t second = (lane & 3) > 0 ? 0xffff0000u : 0u, third = (lane & 3) > 1 ? 0xffff0000u : 0u;
     uint32_t f[8];
@@ -134,7 +150,7 @@ struct Step {
       for (int i = 0; i < 4; ++i) load_edge<T, EVEN>(x[i], row, k + i * 32, K);
     }
   }
-  __device__ __forceinline__ void add(floatx4 (&sum)[NT], int lane) const {
+  __device__ __forceinline__ void add(floatx4 (&sum)[NT], const Bf16Codes& codes, int lane) const {
     constexpr int kSteps = GROUP / 32;
 #pragma unroll
     for (int g = 0; g < kTileK / GROUP; ++g) {
@@ -149,7 +165,7 @@ struct Step {
       for (int t = 0; t < NT; ++t) {
         floatx4 c = c0;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes(q[t][g * kSteps + i]), c);
+        for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes.get(q[t][g * kSteps + i]), c);
         const float scale = s[t].get(g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(scale, c[i], sum[t][i]);
@@ -175,6 +191,7 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
   const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
+  const Bf16Codes codes;
   floatx4 sum[NT] = {};
   if (t0 < tiles) {
     const long apart = (long)kt * tile_bytes(GROUP);
@@ -184,7 +201,7 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
     if (part < kt) now.load(mine, apart, tiles - t0, row, part, K, lane);
     for (int b = part; b < kt; b += SPLIT) {
       if (b + SPLIT < kt) next.load(mine, apart, tiles - t0, row, b + SPLIT, K, lane);
-      now.add(sum, lane);
+      now.add(sum, codes, lane);
       now = next;
     }
   }
@@ -266,6 +283,7 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
   const unsigned char* mine[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) mine[t] = w + (long)min(t0 + t, tiles - 1) * kt * tile_bytes(GROUP);
+  const Bf16Codes codes;
   floatx4 sum[MT][NT] = {};
   Staged<T, EVEN, MT> x_now;
   u32x4 q[NT], q_next[NT];
@@ -304,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
       for (int t = 0; t < NT; ++t) {
         bf16x8 v[kSteps];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) v[i] = codes(q[t][g * kSteps + i]);
+        for (int i = 0; i < kSteps; ++i) v[i] = codes.get(q[t][g * kSteps + i]);
         const float scale = s[t].get(g);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -340,23 +358,243 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
   }
 }
 
+// Many rows.  Products of 16-bit floats are exact where x is: q - 8 has three bits and a scale eight, so (q - 8) s is a half-precision number of 11, and W needs
+// no sums of its own for the scales.  What half precision lacks is range: rows of W come with a power of two that takes their largest scale below 1 (behind the
+// tiles of `weight`), rows of x are taken to 2^14 .. 2^15 by one of their own, and the result is multiplied with both.  Values 2^-29 of their row's largest lose bits;
+// fp32 rows are two parts of 11 bits.
+//
+// int4_operand_kernel writes x in that form once, in the order the matrix instructions take it in: 1024 bytes (Operand) for 16 rows, 32 columns and a part.
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+template <typename T>
+__global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__ x, long x_row, half8* __restrict__ out, float* __restrict__ factor, int M, int K) {
+  constexpr int kParts = sizeof(T) / 2;
+  __shared__ float most_of[4];
+  const int tid = threadIdx.x, r = (int)blockIdx.x, kt = (K + kTileK - 1) / kTileK;
+  const T* row = x + (long)r * x_row;
+  const auto values = [&](int c, float (&v)[8]) {      // eight columns, 0 behind the last
+    Operand<T> o;
+    if (c * 8 + 8 <= K) o.load(row + c * 8); else o.one(row + c * 8, K - c * 8);
+    o.values(v);
+  };
+  constexpr int kHeld = 4;      // eighths that stay in registers between the two passes: rows of up to 8192
+  float held[kHeld][8], most = 0.f;
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h) {
+    if (h * 256 + tid < kt * 16) {
+      values(h * 256 + tid, held[h]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(held[h][i]));
+    }
+  }
+  for (int c = kHeld * 256 + tid; c < kt * 16; c += 256) {
+    float v[8];
+    values(c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+  }
+  for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if ((tid & 63) == 0) most_of[tid >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
+  // a row of zeros, or with an infinity, is taken as it is
+  const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
+  if (tid == 0) factor[r] = ldexpf(1.f, -e);
+  const auto write = [&](int c, const float (&v)[8]) {
+    half8 part[kParts];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = ldexpf(v[i], e);
+      part[0][i] = (_Float16)f;
+      if constexpr (kParts == 2) part[1][i] = (_Float16)(f - (float)part[0][i]);
+    }
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) out[((((long)(r / 16) * kt + c / 16) * kParts + p) * 4 + c / 4 % 4) * 64 + c % 4 * 16 + r % 16] = part[p];
+  };
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (h * 256 + tid < kt * 16) write(h * 256 + tid, held[h]);
+  for (int c = kHeld * 256 + tid; c < kt * 16; c += 256) {
+    float v[8];
+    values(c, v);
+    write(c, v);
+  }
+}
+
+// Eight codes times a scale as (16 + q) s - 24 s, exactly: 0x4c00 is 16 and its bits from the seventh are worth 1, and 24 s has ten bits.
+struct ScaledCodes : Codes {
+  __device__ __forceinline__ ScaledCodes() : Codes(0x03c003c0u, 0x4c004c00u) {}
+  __device__ __forceinline__ half8 get(uint32_t q, half2v s, half2v off) const {
+    const Codes& c = *this;
+    const auto pair = [&](uint32_t b) { return __builtin_elementwise_fma(__builtin_bit_cast(half2v, c(b)), s, off); };
+    const half2v v[4] = {pair(q << 6), pair(q << 2), pair(q >> 2), pair(q >> 6)};
+    return __builtin_bit_cast(half8, v);
+  }
+};
+__device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// A workgroup has MT times 16 rows of x and 4 NT tiles of W's rows, NT a wave.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in
+// registers, once for MT products.
+template <typename T, int GROUP, int MT, int NT>
+__global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const float* __restrict__ factor, const unsigned char* __restrict__ w,
+                                                                const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks, int col_blocks) {
+  constexpr int kParts = sizeof(T) / 2, kStage = MT * kParts * 4096, kSteps = GROUP / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK, row_tiles = (M + 15) / 16;
+  // workgroups of the same columns behind one another on the same XCD (they are dealt to the eight in turn)
+  const int at = (int)blockIdx.x / 8, col = at / row_blocks * 8 + (int)blockIdx.x % 8;
+  if (col >= col_blocks) return;
+  const int m0 = at % row_blocks * MT, t0 = (col * 4 + wave) * NT;
+  const unsigned char* mine[NT];
+  float row_factor[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int tile = min(t0 + t, tiles - 1);
+    mine[t] = w + (long)tile * kt * tile_bytes(GROUP);
+    row_factor[t] = reinterpret_cast<const float*>(w + (long)tiles * kt * tile_bytes(GROUP))[tile * 16 + (lane & 15)];
+  }
+  floatx4 sum[MT][NT] = {};
+  u32x4 q[NT], q_next[NT];
+  Scales<GROUP> s[NT], s_next[NT];
+  half2v scale[NT], off[NT];
+  const ScaledCodes codes;
+  const unsigned lds0 = (unsigned)(uintptr_t)staged;
+  const auto ask = [&](int b) {
+    // a wave fetches every fourth piece of 1024 bytes
+#pragma unroll
+    for (int i = 0; i < MT * kParts; ++i) {
+      const int piece = i * 4 + wave, m = piece / (4 * kParts);
+      const unsigned char* from = x + (((long)min(m0 + m, row_tiles - 1) * kt + b) * kParts * 4 + piece % (4 * kParts)) * 1024;
+      load_to_lds(lds0 + (b & 1) * kStage + piece * 1024, lane * 16, from);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const unsigned char* p = mine[t] + (long)b * tile_bytes(GROUP);
+      q_next[t] = *reinterpret_cast<const u32x4*>(p + lane * 16);
+      s_next[t].load(p, lane);
+    }
+  };
+  ask(0);
+  for (int b = 0; b < kt; ++b) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) q[t] = q_next[t], s[t] = s_next[t];
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);      // this tile of x is there, of this wave's pieces
+    __syncthreads();                           // of all; and nobody reads the other stage any more
+    if (b + 1 < kt) ask(b + 1);
+    const unsigned char* from = staged + (b & 1) * kStage + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      half8 a[kParts][MT];
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) a[p][m] = *reinterpret_cast<const half8*>(from + ((m * kParts + p) * 4 + i) * 1024);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (i % kSteps == 0) {
+          const _Float16 one = (_Float16)(s[t].get(i / kSteps) * row_factor[t]);
+          scale[t] = half2v{one, one};
+          off[t] = scale[t] * half2v{(_Float16)-24.f, (_Float16)-24.f};
+        }
+        const half8 v = codes.get(q[t][i], scale[t], off[t]);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) sum[m][t] = mfma(a[p][m], v, sum[m][t]);
+      }
+    }
+  }
+  // 16 rows at a time through shared memory, each wave by itself, so that a row's values leave together
+  constexpr int kRow = NT * 16 + 4;
+  __syncthreads();
+  float* const mine_out = reinterpret_cast<float*>(staged) + wave * 16 * kRow;
+  const int n0 = t0 * kTileN;
+  float bn[NT], fn[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    bn[t] = bias && n0 + t * 16 + (lane & 15) < N ? bias[n0 + t * 16 + (lane & 15)] : 0.f;
+    fn[t] = 1.f / row_factor[t];
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if ((m0 + m) * 16 >= M) break;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (lane >> 4) * 4 + i;
+      const float fm = factor[min((m0 + m) * 16 + row, M - 1)];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float y = sum[m][t][i] * (fm * fn[t]) + bn[t];
+        if (gelu) y = gelu_erf(y);
+        mine_out[row * kRow + t * 16 + (lane & 15)] = y;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    constexpr int kEach = NT * 4;      // values of a lane: a quarter of a row
+    const int row = lane >> 2, at_n = (lane & 3) * kEach, R = (m0 + m) * 16 + row;
+    float y[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i += 4) *reinterpret_cast<floatx4*>(y + i) = *reinterpret_cast<const floatx4*>(mine_out + row * kRow + at_n + i);
+    __builtin_amdgcn_wave_barrier();
+    if (R < M) {
+      T* to = out + (long)R * N + n0 + at_n;
+      const int left = N - n0 - at_n;
+      if (left >= kEach) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < kEach; i += 4)
+            *reinterpret_cast<u32x4_any*>(to + i) = u32x4_any{__float_as_uint(y[i]), __float_as_uint(y[i + 1]), __float_as_uint(y[i + 2]), __float_as_uint(y[i + 3])};
+        } else if constexpr (kEach >= 8) {
+#pragma unroll
+          for (int i = 0; i < kEach; i += 8)
+            *reinterpret_cast<u32x4_any*>(to + i) = u32x4_any{pack_bf16x2(y[i], y[i + 1]), pack_bf16x2(y[i + 2], y[i + 3]), pack_bf16x2(y[i + 4], y[i + 5]), pack_bf16x2(y[i + 6], y[i + 7])};
+        } else {
+          *reinterpret_cast<u32x2_any*>(to) = u32x2_any{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+          if (i < left) put(to, i, y[i], 0);
+      }
+    }
+  }
+}
+
 }  // namespace m2
 
 using namespace m2;
 
 extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
   if (N <= 0 || K <= 0 || (group != 32 && group != 64 && group != 128)) return 0;
-  return (size_t)((N + kTileN - 1L) / kTileN) * (size_t)((K + kTileK - 1L) / kTileK) * (size_t)tile_bytes(group);
+  const size_t tiles = (size_t)((N + kTileN - 1L) / kTileN);
+  return tiles * ((size_t)((K + kTileK - 1L) / kTileK) * (size_t)tile_bytes(group) + kTileN * sizeof(float));
 }
 
-extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, int M, int N, int K, int group, int gelu,
+// Whether x is written as half-precision operands first, 4 us that only a large product wins back.  us, the kernel of more rows / operands and the kernel of many:
+// 768 -> 30528 bf16 M = 64 10.8 / 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 39; 7168 -> 1792 M = 512 49 / 39; 960 -> 960 M = 200 7.5 / 11.3; fp32, whose rows are
+// two parts there and four places of 16 here, 768 -> 30522 M = 8 9.0 / 11.7, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 63.
+static bool many_rows(int M, int N, int K, int dtype) {
+  const double products = (double)M * N * K;
+  return dtype == M2_DTYPE_F32 ? M > 16 && products >= 4e8 : M > 128 && products >= 3e9;
+}
+
+extern "C" size_t m2_int4_workspace_bytes(int M, int N, int K, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || !many_rows(M, N, K, dtype)) return 0;
+  const size_t row_tiles = (size_t)((M + 15L) / 16), kt = (size_t)((K + kTileK - 1L) / kTileK);
+  return row_tiles * (kt * (dtype == M2_DTYPE_F32 ? 8192 : 4096) + 16 * sizeof(float));
+}
+
+extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, void* workspace, int M, int N, int K, int group, int gelu,
                                   int dtype, void* stream) {
   const char* who = "m2_int4_linear_fwd";
   if (!x || !weight || !out) return set_error(M2_ERR_ARG, "%s: null pointer", who);
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype must be M2_DTYPE_F32 or M2_DTYPE_BF16 (got %d)", who, dtype);
   if (M <= 0 || N <= 0 || K <= 0 || x_row < 0 || (gelu != 0 && gelu != 1)) return set_error(M2_ERR_ARG, "%s: M=%d N=%d K=%d x_row=%ld gelu=%d", who, M, N, K, x_row, gelu);
   if (group != 32 && group != 64 && group != 128) return set_error(M2_ERR_UNSUPPORTED, "%s: groups of 32, 64 or 128 values (got %d)", who, group);
-  if (!aligned16(weight)) return set_error(M2_ERR_UNSUPPORTED, "%s: the weight must be 16-byte aligned", who);
+  if (!aligned16(weight, workspace)) return set_error(M2_ERR_UNSUPPORTED, "%s: weight and workspace must be 16-byte aligned", who);
+  if (!workspace && m2_int4_workspace_bytes(M, N, K, dtype)) return set_error(M2_ERR_ARG, "%s: M=%d rows need a workspace", who, M);
   const uintptr_t size = dtype == M2_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)x % size || (uintptr_t)out % size || (uintptr_t)bias % 4) return set_error(M2_ERR_UNSUPPORTED, "%s: x, out and bias must be aligned to their type", who);
   hipStream_t st = (hipStream_t)stream;
@@ -366,6 +604,15 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((waves + each - 1) / each), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows)), dim3(64 * each), 0, st, (const T*)x, x_row,
                        (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
+  };
+  const auto many = [&](auto kernel, auto* t, int mt, int nt) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const int row_tiles = (M + 15) / 16, row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
+    float* factor = (float*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
+    hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, factor, M, K);
+    const int stage = 2 * mt * parts * 4096, leave = 4 * 16 * (nt * 16 + 4) * 4;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((col_blocks + 7) / 8 * 8 * row_blocks)), dim3(256), (size_t)(stage > leave ? stage : leave), st, (const unsigned char*)workspace, factor,
+                       (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu, row_blocks, col_blocks);
   };
   const auto rows = [&](auto kernel, auto* t, int mt, int nt) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -377,6 +624,13 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int G = decltype(g)::value;
     const int places = (M + Operand<T>::kRows - 1) / Operand<T>::kRows;      // times 16
+    if (many_rows(M, N, K, dtype)) {
+      // 64 rows by 128 of W (fp32: 32 by 128) where there are two rounds of such workgroups, else 32 by 64: 768 -> 30528 M = 512 62 us by 32 x 64, 45 by 32 x 128, 39 by
+      // 64 x 128 and 64 x 256, 42 by 128 x 128; fp32 82, 63, 66 and 65; 7168 -> 1792 39, 41, 51, 79 and 76
+      constexpr int kMt = sizeof(T) == 4 ? 2 : 4;
+      if (((M + 16L * kMt - 1) / (16 * kMt)) * ((tiles + 7) / 8) >= 2L * num_cus()) return many(int4_many_rows_kernel<T, G, kMt, 2>, t, kMt, 2);
+      return many(int4_many_rows_kernel<T, G, 2, 1>, t, 2, 1);
+    }
     if (places > 1) {
       constexpr int kMt = sizeof(T) == 4 ? 4 : 2;      // 32 rows of bf16, 16 of fp32
       const long blocks = (places + kMt - 1L) / kMt * ((tiles + 7) / 8);

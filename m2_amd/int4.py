@@ -119,12 +119,17 @@ def _in_tiles(codes: torch.Tensor, scales: torch.Tensor, K: int, group: int) -> 
     v = v.permute(0, 2, 4, 1, 3, 7, 5, 6)                     # nt, kt, eighth, row, step, half, r // 2, r % 2
     tiles = (v[..., 0] | (v[..., 1] << 4)).reshape(nt, kt, 1024)
     s = s.view(nt, 16, kt, 128 // group).permute(0, 2, 1, 3).contiguous().view(torch.uint8).view(nt, kt, -1)
-    return torch.cat((tiles, s), -1).reshape(-1)
+    # the power of two that takes a row's largest scale to [1 / 2, 1)
+    most = scales.float().abs().amax(1)
+    exponent = torch.where(torch.isfinite(most) & (most > 0), torch.frexp(most).exponent, torch.zeros_like(most, dtype=torch.int32))
+    factor = torch.ones(nt * 16, device=codes.device)
+    factor[:N] = torch.ldexp(factor[:N], -exponent.clamp(-120, 120))
+    return torch.cat((torch.cat((tiles, s), -1).reshape(-1), factor.view(torch.uint8)))
 
 
 def _out_of_tiles(weight: torch.Tensor, N: int, K: int, group: int) -> Tuple[torch.Tensor, torch.Tensor]:
     nt, kt = -(-N // 16), -(-K // 128)
-    w = weight.view(nt, kt, -1)
+    w = weight[:weight.numel() - nt * 16 * 4].view(nt, kt, -1)
     v = w[..., :1024].reshape(nt, kt, 4, 16, 4, 2, 2)         # nt, kt, eighth, row, step, half, r // 2
     v = torch.stack((v & 15, v >> 4), -1).permute(0, 3, 1, 4, 2, 6, 7, 5).reshape(nt * 16, kt * 128)[:N]
     s = w[..., 1024:].contiguous().view(torch.bfloat16).view(nt, kt, 16, 128 // group).permute(0, 2, 1, 3).reshape(nt * 16, -1)

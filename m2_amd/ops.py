@@ -20,7 +20,7 @@ Tensor = torch.Tensor
 
 # what the calls of Int4Linear and token_logprobs need of the library that _lib has loaded
 _answer_calls.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
-    "m2_last_error", "m2_int4_weight_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd")])
+    "m2_last_error", "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd")])
 
 
 # handle of the current stream of a device: 0.3 us, where torch.cuda.current_stream() makes an object in 3 us

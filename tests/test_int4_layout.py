@@ -20,7 +20,7 @@ def _code_at(weight, N, K, group, n, k):
 def test_codes_and_scales_lie_where_the_header_says(N, K, group):
     import m2_amd
     from m2_amd import ops
-    g = torch.Generator().manual_seed(N)
+    g = torch.Generator().manual_seed(N + 1)
     codes = torch.randint(0, 16, (N, K + K % 2), generator=g)
     scales = torch.rand(N, -(-K // group), generator=g).to(torch.bfloat16)
     lin = m2_amd.Int4Linear.from_packed((codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8), scales, K, group)
@@ -29,6 +29,9 @@ def test_codes_and_scales_lie_where_the_header_says(N, K, group):
     for n in range(N):
         for k in range(0, K, 7):
             assert _code_at(lin.weight, N, K, group, n, k) == (codes[n, k].item(), bits[n, k // group].item())
+    factor = lin.weight[-(-N // 16) * 16 * -4:].view(torch.float32)
+    most = scales.float().amax(1) * factor[:N]
+    assert (torch.frexp(factor).mantissa == 0.5).all() and ((most >= 0.5) & (most < 1) | (scales == 0).all(1)).all()
     last = (-(-N // 16) * 16 - 1, -(-K // 128) * 128 - 1)
     if N % 16 and K % 128:
         assert _code_at(lin.weight, N, K, group, *last) == (8, 0)
@@ -75,12 +78,17 @@ def test_modules_refuse_what_does_not_fit():
 def test_entry_points_refuse_before_a_launch():
     from m2_amd._lib import lib
     p, off = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
-    assert lib.m2_int4_weight_bytes(16, 128, 128) == 1024 + 32 and lib.m2_int4_weight_bytes(17, 129, 32) == 4 * (1024 + 128)
+    assert lib.m2_int4_weight_bytes(16, 128, 128) == 1024 + 32 + 64 and lib.m2_int4_weight_bytes(17, 129, 32) == 4 * (1024 + 128) + 128
     assert lib.m2_int4_weight_bytes(0, 128, 128) == 0 and lib.m2_int4_weight_bytes(4, 0, 32) == 0 and lib.m2_int4_weight_bytes(4, 4, 16) == 0
-    assert lib.m2_int4_weight_bytes(2 ** 31 - 1, 2 ** 31 - 1, 128) == 2 ** 27 * 2 ** 24 * 1056
+    assert lib.m2_int4_weight_bytes(2 ** 31 - 1, 2 ** 31 - 1, 128) == 2 ** 27 * (2 ** 24 * 1056 + 64)
 
-    def linear(x=p, x_row=64, w=p, bias=None, out=p, M=1, N=16, K=64, group=64, gelu=0, dtype=1):
-        return lib.m2_int4_linear_fwd(x, x_row, w, bias, out, M, N, K, group, gelu, dtype, None)
+    def linear(x=p, x_row=64, w=p, bias=None, out=p, M=1, N=16, K=64, group=64, gelu=0, dtype=1, workspace=None):
+        return lib.m2_int4_linear_fwd(x, x_row, w, bias, out, workspace, M, N, K, group, gelu, dtype, None)
+
+    need = lib.m2_int4_workspace_bytes
+    assert need(1, 30522, 64, 1) == need(0, 64, 64, 1) == need(4096, 64, 0, 1) == need(4096, 64, 64, 1) == 0
+    assert need(4097, 30522, 129, 1) == 257 * (2 * 4096 + 64) and need(4097, 30522, 129, 0) == 257 * (2 * 8192 + 64)
+    assert linear(M=4096, N=30522) == -1 and b"workspace" in lib.m2_last_error() and linear(M=4096, N=30522, workspace=off) == -2
 
     assert linear(x=None) == linear(w=None) == linear(out=None) == -1 and b"null" in lib.m2_last_error()
     assert linear(M=0) == linear(N=-1) == linear(K=0) == linear(x_row=-1) == linear(dtype=2) == linear(gelu=2) == -1
