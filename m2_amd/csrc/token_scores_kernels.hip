@@ -98,10 +98,19 @@ __device__ __forceinline__ float value_at(const char* x, const unsigned char* a,
 // The hardware's 2^x: one ulp, results below 2^-126 are 0.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Maximum, sum of exp(z - m) and sum of exp(z - m) (z - m).
+// Maximum, sum of exp(z - m) in two parts and sum of exp(z - m) (z - m).  Where one token has nearly all of the probability, log s and the entropy are what
+// the others add to 1: `low` keeps what the additions to s lose.
 struct Sums {
-  float m = kNegInf, s = 0.f, t = 0.f;
+  float m, s, t, low;
 };
+__device__ __forceinline__ Sums nothing() { return {kNegInf, 0.f, 0.f, 0.f}; }
+
+// a.s + a.low + v
+__device__ __forceinline__ void add_up(Sums& a, float v) {
+  const float s = a.s + v, other = s - a.s;
+  a.low += (a.s - (s - other)) + (v - other);
+  a.s = s;
+}
 
 // What sums relative to `from` become relative to `to` >= from.  Differences below -1e4 stand for all that exp takes to zero, -inf and
 // (-inf) - (-inf) among them, so that nothing times zero is NaN; a NaN in the sums stays one.
@@ -109,14 +118,8 @@ __device__ __forceinline__ void rescale(Sums& a, float to) {
   const float d = fmaxf(a.m - to, -1e4f), f = exp2_(d * kLog2e);
   a.t = f * fmaf(d, a.s, a.t);
   a.s *= f;
+  a.low *= f;
   a.m = to;
-}
-
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  rescale(a, m);
-  rescale(b, m);
-  return {m, a.s + b.s, a.t + b.t};
 }
 
 // The sums of LANES neighbours, in all of them.
@@ -128,9 +131,10 @@ __device__ __forceinline__ Sums join_lanes(Sums a) {
   rescale(a, m);
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) {
-    const float s = __shfl_xor(a.s, o), t = __shfl_xor(a.t, o);
-    a.s += s;
+    const float s = __shfl_xor(a.s, o), t = __shfl_xor(a.t, o), low = __shfl_xor(a.low, o);
     a.t += t;
+    a.low += low;
+    add_up(a, s);
   }
   return a;
 }
@@ -143,12 +147,18 @@ __device__ __forceinline__ float add_values(Sums& a, const float (&z)[N]) {
   for (int i = 1; i < N; ++i) c = fmaxf(c, z[i]);
   if (c > a.m) rescale(a, c);
   const float base = a.m == kNegInf ? 0.f : a.m;      // nothing but -inf (and NaN, which has to show) so far
+  float e[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float d = z[i] - base, e = exp2_(d * kLog2e);
-    a.s += e;
-    a.t = fmaf(e, fmaxf(d, -1e4f), a.t);
+    const float d = z[i] - base;
+    e[i] = exp2_(d * kLog2e);
+    a.t = fmaf(e[i], fmaxf(d, -1e4f), a.t);
   }
+#pragma unroll
+  for (int n = N / 2; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) e[i] += e[i + n];
+  add_up(a, e[0]);
   return c;
 }
 
@@ -394,7 +404,7 @@ __device__ __forceinline__ float token_value(long long t, int V, const char* x, 
 __device__ __forceinline__ void finish(const RowScores& out, long r, int top_k, long long id_given, float token, const Sums& all, const float* v, const int* id) {
   const int tid = threadIdx.x;
   const bool empty = all.s == 0.f, broken = all.s != all.s;      // broken: a NaN or +inf among the values
-  const float logs = empty ? 0.f : logf(all.s), nan = __builtin_nanf("");
+  const float logs = empty ? 0.f : log1pf((all.s - 1.f) + all.low), nan = __builtin_nanf("");
   if (tid == 0) {
     if (out.tokens) {
       const float lp = broken ? nan : token == kNegInf ? kNegInf : (token - all.m) - logs;
@@ -415,7 +425,7 @@ __device__ __forceinline__ void finish(const RowScores& out, long r, int top_k, 
 template <typename T, bool MASK, bool TOP, int THREADS>
 __global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, RowScores out, uint32_t first, int V, int top_k, int parts, PartScores* __restrict__ work) {
   constexpr int N = Row<T>::N, kWaves = THREADS / 64, kAhead = 4;
-  __shared__ float part_m[kWaves], part_s[kWaves], part_t[kWaves];
+  __shared__ Sums part_sums[kWaves];
   __shared__ Top<T, MASK, THREADS> top;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int nvec = V / N, each = (nvec + parts - 1) / parts;
@@ -426,7 +436,7 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, Row
   const char* x = row_of<T>(in, r);
   const unsigned char* a = MASK ? in.allowed + r * in.allowed_row : nullptr;
   const Span p = {min(part * each, nvec), min((part + 1) * each, nvec), part == parts - 1 ? nvec * N : V, V};
-  Sums mine;
+  Sums mine = nothing();
   int i = p.first + tid;
   Met met;
   const auto add = [&](const Vector<T, MASK>& q, int at) {
@@ -457,10 +467,9 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, Row
   }
   const float at_token = parts > 1 ? 0.f : token_value<T, MASK>(token, V, x, a);
   mine = join_lanes<64>(mine);
-  if (lane == 0) part_m[wave] = mine.m, part_s[wave] = mine.s, part_t[wave] = mine.t;
+  if (lane == 0) part_sums[wave] = mine;
   __syncthreads();
-  const int w = lane % kWaves;
-  const Sums all = join_lanes<kWaves>(Sums{part_m[w], part_s[w], part_t[w]});
+  const Sums all = join_lanes<kWaves>(part_sums[lane % kWaves]);
   if (TOP)
     if (all.s == all.s) top.find(x, a, p, met, top_k);
   if (parts > 1) {
@@ -483,7 +492,7 @@ __global__ __launch_bounds__(256) void token_scores_join_kernel(LogitRows in, Ro
   const uint32_t r = blockIdx.x;
   const PartScores* from = work + r * parts;
   const long long token = out.tokens && tid == 0 ? out.tokens[r] : 0;
-  const Sums all = join_lanes<kMaxParts>(tid % kMaxParts < parts ? from[tid % kMaxParts].sums : Sums{});
+  const Sums all = join_lanes<kMaxParts>(tid % kMaxParts < parts ? from[tid % kMaxParts].sums : nothing());
   if (top_k && all.s == all.s) {
     // larger values first, then lower ids: all keys are different, empty places are 0
     for (int i = tid; i < (parts + kTogether - 1) / kTogether * kTogether * kMaxTop; i += 256) {

@@ -193,6 +193,20 @@ def test_values_at_the_ends(gpu, dtype, V):
     compare(x, tokens, min(V, 6), grads=_grads(gpu, (12,), min(V, 6)))
 
 
+@pytest.mark.parametrize("rows,V", [(3, 30522), (700, 4000), (1, 200_003)])
+def test_one_token_has_nearly_all(gpu, rows, V):
+    """What the other tokens add to 1 is all of log s and of the entropy.  Eight values of a vector are added to the 1 among them in three steps, half a unit of
+    its last bit each, and all others apart from it; each of the others is off by its argument's rounding, 2 units for each e-fold, below 30 of them."""
+    import m2_amd
+    x = _logits(gpu, (rows, V), torch.float32, scale=1.0) - 6
+    x[:, V // 3] = torch.linspace(4, 22, rows, device=gpu)
+    r = m2_amd.token_logprobs(x, torch.full((rows,), V // 3, device=gpu), 1)
+    lp, h, ids, top, _ = definition(x, torch.full((rows,), V // 3), 1, None)
+    assert torch.equal(r.top_ids.cpu(), ids)
+    close(r.logprobs, lp, U * (4 + 64 * lp.abs()))
+    close(r.entropy, h, U * (4 + 128 * h))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V,levels", [(4096, 1), (4096, 2), (30522, 3), (30522, 40), (70001, 1)])
 def test_ties_go_to_the_lowest_id(gpu, dtype, V, levels):
