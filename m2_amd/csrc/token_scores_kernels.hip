@@ -139,12 +139,9 @@ __device__ __forceinline__ Sums join_lanes(Sums a) {
   return a;
 }
 
-// Returns the largest of the values.
+// `c`: the largest of the values.
 template <int N>
-__device__ __forceinline__ float add_values(Sums& a, const float (&z)[N]) {
-  float c = z[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) c = fmaxf(c, z[i]);
+__device__ __forceinline__ void add_values(Sums& a, const float (&z)[N], float c) {
   if (c > a.m) rescale(a, c);
   const float base = a.m == kNegInf ? 0.f : a.m;      // nothing but -inf (and NaN, which has to show) so far
   float e[N];
@@ -159,7 +156,6 @@ __device__ __forceinline__ float add_values(Sums& a, const float (&z)[N]) {
 #pragma unroll
     for (int i = 0; i < n; ++i) e[i] += e[i + n];
   add_up(a, e[0]);
-  return c;
 }
 
 // (value, id) before (other, other_id): larger value first, then the lower id.
@@ -439,18 +435,31 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, Row
   Sums mine = nothing();
   int i = p.first + tid;
   Met met;
-  const auto add = [&](const Vector<T, MASK>& q, int at) {
-    float z[N];
-    q.values(z);
-    const float c = add_values<N>(mine, z);
-    if (TOP) met.see(c, at);
+  // kTogether vectors at a time, with one look at the maximum and one addition to the sum
+  const auto add = [&](const auto* q, auto count, int at) {
+    constexpr int C = decltype(count)::value;
+    float z[C * N], c[C], all = kNegInf;
+#pragma unroll
+    for (int v = 0; v < C; ++v) {
+      float (&zv)[N] = *reinterpret_cast<float (*)[N]>(z + v * N);
+      q[v].values(zv);
+      c[v] = zv[0];
+#pragma unroll
+      for (int n = 1; n < N; ++n) c[v] = fmaxf(c[v], zv[n]);
+      if (TOP) met.see(c[v], at + v * THREADS);
+      all = fmaxf(all, c[v]);
+    }
+    add_values<C * N>(mine, z, all);
   };
+  constexpr int kTogether = 16 / N;
+  const std::integral_constant<int, kTogether> together;
+  const std::integral_constant<int, 1> one;
   for (; i + (kAhead - 1) * THREADS < p.end; i += kAhead * THREADS) {
     Vector<T, MASK> q[kAhead];
 #pragma unroll
     for (int c = 0; c < kAhead; ++c) q[c].load(x, a, i + c * THREADS);
 #pragma unroll
-    for (int c = 0; c < kAhead; ++c) add(q[c], i + c * THREADS);
+    for (int c = 0; c < kAhead; c += kTogether) add(q + c, together, i + c * THREADS);
   }
   // the last vectors: as many loads at a time
   Vector<T, MASK> q[kAhead - 1];
@@ -459,11 +468,11 @@ __global__ __launch_bounds__(THREADS) void token_scores_kernel(LogitRows in, Row
     if (i + c * THREADS < p.end) q[c].load(x, a, i + c * THREADS);
 #pragma unroll
   for (int c = 0; c < kAhead - 1; ++c)
-    if (i + c * THREADS < p.end) add(q[c], i + c * THREADS);
+    if (i + c * THREADS < p.end) add(q + c, one, i + c * THREADS);
   if (p.tail + tid < V) {
     const float z[1] = {value_at<T, MASK>(x, a, p.tail + tid)};
-    const float c = add_values<1>(mine, z);
-    if (TOP) met.see(c, kTail);
+    if (TOP) met.see(z[0], kTail);
+    add_values<1>(mine, z, z[0]);
   }
   const float at_token = parts > 1 ? 0.f : token_value<T, MASK>(token, V, x, a);
   mine = join_lanes<64>(mine);
