@@ -628,7 +628,9 @@ static int check_rows(const char* who, const void* logits, int inner, long outer
 
 using namespace m2;
 
-// Workgroups a row: a part should keep a workgroup of 1024 threads busy for a few vectors each, and there is no use for more parts than fill the chip.
+// Workgroups a row: the second kernel, which puts parts together, costs 4 us, so rows of fewer than 8192 vectors stay whole, and there is no use for more parts than
+// fill the chip.  us, 1 / 2 / 4 / 8 / 16 parts, 512 threads: 131072 fp32 top 32 1 row 18.1 / 16.8 / 14.0 / 13.0 / 14.9, 24 rows 18.8 / 17.4 / 14.8 / 13.7 / 16.8; 30528 bf16 top 5
+// 1 row 7.7 / 10.9 / 9.4 / 9.5 / 12.0.
 static int parts_of(long rows, int V, int dtype) {
   const long vectors = V / (dtype == M2_DTYPE_F32 ? 4 : 8);
   long parts = vectors / 4096;
@@ -662,8 +664,12 @@ extern "C" int m2_token_scores_fwd(const void* logits, int inner, long outer_str
   const auto pick = [&](auto* t, auto masked) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr bool M = decltype(masked)::value;
-    if (blocks <= 512) top_k ? go(token_scores_kernel<T, M, true, 1024>, 1024) : go(token_scores_kernel<T, M, false, 1024>, 1024);
-    else top_k ? go(token_scores_kernel<T, M, true, 256>, 256) : go(token_scores_kernel<T, M, false, 256>, 256);
+    // us, 512 / 256 / 128 threads a row, ten alternatives: 30528 bf16 16 rows 8.2 / 9.1 / -, 300 13.0 / 12.9 / 17.9, 4915 78 / 65 / 68; 4000 bf16 8000 rows 55 / 33 / 28; 16000
+    // bf16 4000 rows 47 / 38 / 36
+    const int threads = blocks <= num_cus() ? 512 : V / Row<T>::N <= 2048 && blocks > 4L * num_cus() ? 128 : 256;
+    if (threads == 512) top_k ? go(token_scores_kernel<T, M, true, 512>, 512) : go(token_scores_kernel<T, M, false, 512>, 512);
+    else if (threads == 256) top_k ? go(token_scores_kernel<T, M, true, 256>, 256) : go(token_scores_kernel<T, M, false, 256>, 256);
+    else top_k ? go(token_scores_kernel<T, M, true, 128>, 128) : go(token_scores_kernel<T, M, false, 128>, 128);
     if (parts > 1)
       hipLaunchKernelGGL((token_scores_join_kernel<T, M>), dim3((unsigned)rows), dim3(256), 0, st, in, out, V, top_k, parts, (const PartScores*)workspace);
   };
