@@ -47,7 +47,9 @@ class Int4Linear(nn.Module):
             raise ValueError(f"in_features and out_features must be positive, got {in_features}, {out_features}")
         self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
         nbytes = ops.int4_weight_bytes(out_features, in_features, group_size)
-        self.register_buffer("weight", torch.zeros(nbytes, dtype=torch.uint8, device=device))
+        weight = torch.zeros(nbytes, dtype=torch.uint8, device=device)      # scales 0: W = 0
+        weight[nbytes - -(-out_features // 16) * 64:].view(torch.float32).fill_(1)
+        self.register_buffer("weight", weight)
         self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32, device=device) if bias else None)
 
     @classmethod
