@@ -367,42 +367,46 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
+// Four rows a workgroup, so that what it writes are pieces of 64 bytes.
 template <typename T>
 __global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__ x, long x_row, half8* __restrict__ out, float* __restrict__ factor, int M, int K) {
-  constexpr int kParts = sizeof(T) / 2;
-  __shared__ float most_of[4];
-  const int tid = threadIdx.x, r = (int)blockIdx.x, kt = (K + kTileK - 1) / kTileK;
-  const T* row = x + (long)r * x_row;
-  const auto values = [&](int c, float (&v)[8]) {      // eight columns, 0 behind the last
-    Operand<T> o;
+  constexpr int kParts = sizeof(T) / 2, kHeld = 16 / kParts;      // kHeld: eighths that stay in registers between the two passes (rows of up to 8192, fp32 4096)
+  __shared__ float most_of[4][4];
+  const int tid = threadIdx.x, r = (int)blockIdx.x * 4 + (tid & 3), first = tid >> 2, kt = (K + kTileK - 1) / kTileK, end = r < M ? kt * 16 : 0;
+  const T* row = x + (long)min(r, M - 1) * x_row;
+  const auto load = [&](int c, Operand<T>& o) {      // eight columns, 0 behind the last
     if (c * 8 + 8 <= K) o.load(row + c * 8); else o.one(row + c * 8, K - c * 8);
-    o.values(v);
   };
-  constexpr int kHeld = 4;      // eighths that stay in registers between the two passes: rows of up to 8192
-  float held[kHeld][8], most = 0.f;
-#pragma unroll
-  for (int h = 0; h < kHeld; ++h) {
-    if (h * 256 + tid < kt * 16) {
-      values(h * 256 + tid, held[h]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(held[h][i]));
-    }
-  }
-  for (int c = kHeld * 256 + tid; c < kt * 16; c += 256) {
+  float most = 0.f;
+  const auto look = [&](const Operand<T>& o) {
     float v[8];
-    values(c, v);
+    o.values(v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+  };
+  Operand<T> held[kHeld];
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (first + h * 64 < end) load(first + h * 64, held[h]);
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+    if (first + h * 64 < end) look(held[h]);
+  for (int c = first + kHeld * 64; c < end; c += 64) {
+    Operand<T> o;
+    load(c, o);
+    look(o);
   }
-  for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-  if ((tid & 63) == 0) most_of[tid >> 6] = most;
+  for (int o = 32; o > 2; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+  if ((tid & 63) < 4) most_of[tid >> 6][tid & 3] = most;
   __syncthreads();
-  most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
+  most = fmaxf(fmaxf(most_of[0][tid & 3], most_of[1][tid & 3]), fmaxf(most_of[2][tid & 3], most_of[3][tid & 3]));
   // a row of zeros, or with an infinity, is taken as it is
   const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
-  if (tid == 0) factor[r] = ldexpf(1.f, -e);
-  const auto write = [&](int c, const float (&v)[8]) {
+  if (tid < 4 && r < M) factor[r] = ldexpf(1.f, -e);
+  const auto write = [&](int c, const Operand<T>& o) {
     half8 part[kParts];
+    float v[8];
+    o.values(v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float f = ldexpf(v[i], e);
@@ -414,11 +418,11 @@ __global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__
   };
 #pragma unroll
   for (int h = 0; h < kHeld; ++h)
-    if (h * 256 + tid < kt * 16) write(h * 256 + tid, held[h]);
-  for (int c = kHeld * 256 + tid; c < kt * 16; c += 256) {
-    float v[8];
-    values(c, v);
-    write(c, v);
+    if (first + h * 64 < end) write(first + h * 64, held[h]);
+  for (int c = first + kHeld * 64; c < end; c += 64) {
+    Operand<T> o;
+    load(c, o);
+    write(c, o);
   }
 }
 
@@ -609,7 +613,7 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     using T = std::remove_pointer_t<decltype(t)>;
     const int row_tiles = (M + 15) / 16, row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
     float* factor = (float*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
-    hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)M), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, factor, M, K);
+    hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, factor, M, K);
     const int stage = 2 * mt * parts * 4096, leave = 4 * 16 * (nt * 16 + 4) * 4;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((col_blocks + 7) / 8 * 8 * row_blocks)), dim3(256), (size_t)(stage > leave ? stage : leave), st, (const unsigned char*)workspace, factor,
                        (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu, row_blocks, col_blocks);
