@@ -445,6 +445,7 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
                                                                 const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks, int col_blocks) {
   constexpr int kParts = sizeof(T) / 2, kStage = MT * kParts * 4096, kSteps = GROUP / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages
+  __shared__ float factors[MT * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK, row_tiles = (M + 15) / 16;
   // workgroups of the same columns behind one another on the same XCD (they are dealt to the eight in turn)
@@ -459,6 +460,12 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
     mine[t] = w + (long)tile * kt * tile_bytes(GROUP);
     row_factor[t] = reinterpret_cast<const float*>(w + (long)tiles * kt * tile_bytes(GROUP))[tile * 16 + (lane & 15)];
   }
+  // what the end needs is asked for now
+  if (threadIdx.x < MT * 16) factors[threadIdx.x] = factor[min(m0 * 16 + (int)threadIdx.x, M - 1)];
+  const int n0 = t0 * kTileN;
+  float bn[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) bn[t] = bias && n0 + t * 16 + (lane & 15) < N ? bias[n0 + t * 16 + (lane & 15)] : 0.f;
   floatx4 sum[MT][NT] = {};
   u32x4 q[NT], q_next[NT];
   Scales<GROUP> s[NT], s_next[NT];
@@ -514,20 +521,16 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
   constexpr int kRow = NT * 16 + 4;
   __syncthreads();
   float* const mine_out = reinterpret_cast<float*>(staged) + wave * 16 * kRow;
-  const int n0 = t0 * kTileN;
-  float bn[NT], fn[NT];
+  float fn[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    bn[t] = bias && n0 + t * 16 + (lane & 15) < N ? bias[n0 + t * 16 + (lane & 15)] : 0.f;
-    fn[t] = 1.f / row_factor[t];
-  }
+  for (int t = 0; t < NT; ++t) fn[t] = 1.f / row_factor[t];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if ((m0 + m) * 16 >= M) break;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = (lane >> 4) * 4 + i;
-      const float fm = factor[min((m0 + m) * 16 + row, M - 1)];
+      const float fm = factors[m * 16 + row];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float y = sum[m][t][i] * (fm * fn[t]) + bn[t];
