@@ -6,6 +6,12 @@
 //
 // One pass over a row: every thread keeps the largest value it has met and both sums relative to it, and rescales them when a larger one comes.
 // The largest value itself, and differences to it, are kept (and not products with log2 e, which overflow for a mask of the type's lowest value).
+//
+// Many rows are bound by memory and, in bf16, by nine vector instructions a value, one of them exp at four times the cost of others, nearly as much: 8192 x 30522 bf16 91 us =
+// 5.5 TB/s with the vector unit busy 93 % of the cycles; 4915 x 30528 fp32 104 us = 5.8 TB/s, bf16 59 us = 5.1 TB/s, with ten alternatives 65, with 32 70; the gradient 95 us =
+// 6.3 TB/s of reads and writes (its reads are partly what the pass before has left in the last cache).  Few rows by latency: 1 x 30522 6.1 us, with five alternatives
+// 7.8 (a pass over the row 1.4 us, the sums of all threads 1.4, the bound of the alternatives 0.7, their vectors 1.0, their order 0.5); 615 rows, 2.4 for each
+// compute unit, 12 and with ten alternatives 16 us where memory would take 7.1.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
