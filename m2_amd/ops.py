@@ -13,8 +13,13 @@ from typing import Optional, Sequence
 import torch
 from torch.autograd.forward_ad import unpack_dual as _unpack_dual
 
-from . import _answer_calls, _lib
+from . import _lib
 from ._lib import HyenaFilterParams, SplitJob, M2_DTYPE_BF16, M2_DTYPE_F32, check, lib
+
+try:
+    from . import _answer_calls
+except ImportError as e:
+    raise ImportError(f"m2_amd/_answer_calls.so is missing or does not fit this torch ({e}): build it with `python m2_amd/build.py`") from e
 
 Tensor = torch.Tensor
 
