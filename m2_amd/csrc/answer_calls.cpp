@@ -49,6 +49,7 @@ void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 int type_of(const char* name, const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), name, ": must live on the GPU (m2_amd has no CPU path); got device ", t.device());
+  TORCH_CHECK_TYPE(t.layout() == at::kStrided, name, ": must be strided, got ", t.layout());
   TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, ": must be float32 or bfloat16, got ", t.scalar_type());
   return t.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16;
 }
@@ -61,6 +62,7 @@ struct Rows {
 };
 Rows rows_of(Tensor t, int distances) {
   const int64_t d = t.dim() - 1;
+  if (t.is_neg()) t = t.resolve_neg();      // a view whose memory holds the negatives (the imaginary part of a conjugate)
   if (t.size(d) > 1 && t.stride(d) != 1) t = t.contiguous();
   int64_t size[2] = {1, 1}, stride[2] = {0, 0};      // the innermost first
   int n = 0;
@@ -170,7 +172,7 @@ Found scores(const Tensor& logits, const Scores& s) {
 }
 
 // A gradient of one value a row: it may be one value for all of them.
-Tensor per_row(const Tensor& g) { return g.defined() ? g.reshape({-1}) : g; }
+Tensor per_row(const Tensor& g) { return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).reshape({-1}) : g; }
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -206,7 +208,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
       grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
       if (rows) {
         const Tensor g_lp = per_row(g_logprobs), g_h = per_row(g_entropy),
-                     g_top = g_alternatives.defined() ? g_alternatives.contiguous() : g_alternatives;
+                     g_top = g_alternatives.defined() ? (g_alternatives.is_neg() ? g_alternatives.resolve_neg() : g_alternatives).contiguous() : g_alternatives;
         const Rows r = rows_of(logits.detach(), 2);
         check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(tokens)), ctx->saved_data["ignore_index"].toInt(),
                                static_cast<const unsigned char*>(pointer(allowed)), ctx->saved_data["allowed_row"].toInt(), entropy.data_ptr<float>(), stats.data_ptr<float>(),

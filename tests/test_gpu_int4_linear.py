@@ -193,6 +193,17 @@ def test_ranges_of_rows_and_scales(gpu, dtype, N):
         assert ((lin(x).double() - y).abs() <= tol).all()
 
 
+def test_views_of_negatives(gpu):
+    """Rows whose memory holds the negatives of their values, as imaginary parts of conjugates do."""
+    import m2_amd
+    for M, K in ((3, 200), (20, 200), (2, 1)):
+        _, scales, packed, w = weights(gpu, 50, K, 32)
+        lin = m2_amd.Int4Linear.from_packed(packed, scales, K, 32)
+        x = rows(gpu, M, K, dtype=torch.float32)
+        for v in (torch._neg_view(-x), torch.complex(x, -x).conj().imag):
+            assert v.is_neg() and torch.equal(lin(v), lin(x))
+
+
 def test_what_is_around_stays(gpu):
     import m2_amd
     from m2_amd import ops

@@ -424,6 +424,42 @@ def test_captured_beside_eager_calls_and_streams(gpu, rows, V):
         assert all(torch.equal(a, b) for a, b in zip(eager, want[2]))
 
 
+def test_views_of_negatives(gpu):
+    """Logits and gradients whose memory holds the negatives of their values, as imaginary parts of conjugates do."""
+    import m2_amd
+
+    def negative_view(t):
+        v = torch.complex(t, -t).conj().imag
+        assert v.is_neg() and torch.equal(v, t)
+        return v
+
+    for rows, V in ((5, 300), (1, 70), (4, 1)):
+        x, t, (gl, gh, ga) = _logits(gpu, (rows, V), torch.float32, seed=5), _tokens(gpu, (rows,), V), _grads(gpu, (rows,), 1)
+        a, b = x.clone().requires_grad_(), torch._neg_view(-x).requires_grad_()
+        assert b.is_neg()
+        one, other = m2_amd.token_logprobs(a, t, 1), m2_amd.token_logprobs(b, t, 1)
+        assert all(torch.equal(p, q) for p, q in zip(one, other))
+        assert torch.equal(m2_amd.token_logprobs(negative_view(x), t).logprobs, one.logprobs)
+        ins = [torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], [v], g)[0]
+               for r, v, g in ((one, a, (gl, gh, ga)), (other, b, tuple(negative_view(g) for g in (gl, gh, ga))))]
+        assert torch.equal(ins[0], ins[1])
+
+
+def test_recomputed_in_the_backward_pass(gpu):
+    """Under activation checkpointing, whose hooks hand the saved tensors out again."""
+    import m2_amd
+    from torch.utils.checkpoint import checkpoint
+    h, w = torch.randn(6, 40, device=gpu), torch.randn(500, 40, device=gpu)
+    t = _tokens(gpu, (6,), 500)
+    grads = []
+    for again in (False, True):
+        v = w.clone().requires_grad_()
+        f = lambda: m2_amd.token_logprobs(h @ v.t(), t, 3)
+        r = checkpoint(f, use_reentrant=False) if again else f()
+        grads.append(torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + r.top_logprobs.sum(), [v])[0])
+    assert torch.equal(*grads)
+
+
 def test_refusals(gpu):
     import m2_amd
     f = m2_amd.token_logprobs
