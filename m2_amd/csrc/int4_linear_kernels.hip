@@ -203,13 +203,13 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
   __shared__ floatx4 sums[SPLIT > 1 ? waves_of(SPLIT) : 1][SPLIT > 1 ? NT : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
-  const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
+  const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT;
   const Bf16Codes codes;
   floatx4 sum[NT] = {};
   if (t0 < tiles) {
     const long apart = (long)kt * tile_bytes(GROUP);
     const unsigned char* mine = w + t0 * apart;
-    const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
+    const T* row = x + (long)min(Operand<T>::row(lane), M - 1) * x_row;
     Step<T, GROUP, EVEN, NT> now, next;
     if (part < kt) now.load(mine, apart, tiles - t0, row, part, K, lane);
     for (int b = part; b < kt; b += SPLIT) {
@@ -237,12 +237,12 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
     if (n >= N) continue;
     const float b = bias ? bias[n] : 0.f;
     if constexpr (sizeof(T) == 4) {
-      const int m = m0 + (lane >> 4);
+      const int m = lane >> 4;
       if (m < M) put(out, (long)m * N + n, (sum[t][2] + sum[t][1]) + sum[t][0] + b, gelu);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int m = m0 + (lane >> 4) * 4 + i;
+        const int m = (lane >> 4) * 4 + i;
         if (m < M) put(out, (long)m * N + n, sum[t][i] + b, gelu);
       }
     }
@@ -383,7 +383,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 // Four rows a workgroup, so that what it writes are pieces of 64 bytes.
 template <typename T>
-__global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__ x, long x_row, half8* __restrict__ out, float* __restrict__ factor, int M, int K) {
+__global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__ x, long x_row, half8* __restrict__ out, int* __restrict__ exponent, int M, int K) {
   constexpr int kParts = sizeof(T) / 2, kHeld = 16 / kParts;      // kHeld: eighths that stay in registers between the two passes (rows of up to 8192, fp32 4096)
   __shared__ float most_of[4][4];
   const int tid = threadIdx.x, r = (int)blockIdx.x * 4 + (tid & 3), first = tid >> 2, kt = (K + kTileK - 1) / kTileK, end = r < M ? kt * 16 : 0;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__
   most = fmaxf(fmaxf(most_of[0][tid & 3], most_of[1][tid & 3]), fmaxf(most_of[2][tid & 3], most_of[3][tid & 3]));
   // a row of zeros, or with an infinity, is taken as it is
   const int e = most > 0.f && most < __builtin_inff() ? 14 - ilogbf(most) : 0;
-  if (tid < 4 && r < M) factor[r] = ldexpf(1.f, -e);
+  if (tid < 4 && r < M) exponent[r] = -e;
   const auto write = [&](int c, const Operand<T>& o) {
     half8 part[kParts];
     float v[8];
@@ -455,11 +455,11 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __
 // A workgroup has MT times 16 rows of x and 4 NT tiles of W's rows, NT a wave.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in
 // registers, once for MT products.
 template <typename T, int GROUP, int MT, int NT>
-__global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const float* __restrict__ factor, const unsigned char* __restrict__ w,
+__global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const int* __restrict__ exponent, const unsigned char* __restrict__ w,
                                                                 const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks, int col_blocks) {
   constexpr int kParts = sizeof(T) / 2, kStage = MT * kParts * 4096, kSteps = GROUP / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages
-  __shared__ float factors[MT * 16];
+  __shared__ int exponents[MT * 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK, row_tiles = (M + 15) / 16;
   // workgroups of the same columns behind one another on the same XCD (they are dealt to the eight in turn)
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
     row_factor[t] = reinterpret_cast<const float*>(w + (long)tiles * kt * tile_bytes(GROUP))[tile * 16 + (lane & 15)];
   }
   // what the end needs is asked for now
-  if (threadIdx.x < MT * 16) factors[threadIdx.x] = factor[min(m0 * 16 + (int)threadIdx.x, M - 1)];
+  if (threadIdx.x < MT * 16) exponents[threadIdx.x] = exponent[min(m0 * 16 + (int)threadIdx.x, M - 1)];
   const int n0 = t0 * kTileN;
   float bn[NT];
 #pragma unroll
@@ -535,19 +535,20 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
   constexpr int kRow = NT * 16 + 4;
   __syncthreads();
   float* const mine_out = reinterpret_cast<float*>(staged) + wave * 16 * kRow;
-  float fn[NT];
+  // the powers of two are put together as exponents: as numbers their product may be out of range where the result is not
+  int en[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) fn[t] = 1.f / row_factor[t];
+  for (int t = 0; t < NT; ++t) en[t] = 127 - (int)(__float_as_uint(row_factor[t]) >> 23);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if ((m0 + m) * 16 >= M) break;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = (lane >> 4) * 4 + i;
-      const float fm = factors[m * 16 + row];
+      const int em = exponents[m * 16 + row];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float y = sum[m][t][i] * (fm * fn[t]) + bn[t];
+        float y = ldexpf(sum[m][t][i], em + en[t]) + bn[t];
         if (gelu) y = gelu_erf(y);
         mine_out[row * kRow + t * 16 + (lane & 15)] = y;
       }
@@ -604,7 +605,7 @@ static bool many_rows(int M, int N, int K, int dtype) {
 extern "C" size_t m2_int4_workspace_bytes(int M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || !many_rows(M, N, K, dtype)) return 0;
   const size_t row_tiles = (size_t)((M + 15L) / 16), kt = (size_t)((K + kTileK - 1L) / kTileK);
-  return row_tiles * (kt * (dtype == M2_DTYPE_F32 ? 8192 : 4096) + 16 * sizeof(float));
+  return row_tiles * (kt * (dtype == M2_DTYPE_F32 ? 8192 : 4096) + 16 * sizeof(int));
 }
 
 extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight, const float* bias, void* out, void* workspace, int M, int N, int K, int group, int gelu,
@@ -619,32 +620,42 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   const uintptr_t size = dtype == M2_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)x % size || (uintptr_t)out % size || (uintptr_t)bias % 4) return set_error(M2_ERR_UNSUPPORTED, "%s: x, out and bias must be aligned to their type", who);
   hipStream_t st = (hipStream_t)stream;
-  const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
+  const int tiles = (int)((N + kTileN - 1L) / kTileN), kt = (int)((K + kTileK - 1L) / kTileK);
+  // a launch holds below 2^32 threads
+  const auto fits = [](long blocks, long threads) { return blocks < (1L << 32) / threads; };
+  const auto too_large = [&] { return set_error(M2_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d are more workgroups than a launch holds", who, M, N, K); };
   const auto go = [&](auto kernel, auto* t, int nt, int split) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((waves + each - 1) / each), (unsigned)((M + Operand<T>::kRows - 1) / Operand<T>::kRows)), dim3(64 * each), 0, st, (const T*)x, x_row,
-                       (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
+    const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split), blocks = (waves + each - 1) / each;
+    if (!fits(blocks, 64 * each)) return too_large();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * each), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
+    return check_launch("int4_linear");
   };
   const auto many = [&](auto kernel, auto* t, int mt, int nt) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int row_tiles = (M + 15) / 16, row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
-    float* factor = (float*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
-    hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, factor, M, K);
+    const int row_tiles = (int)((M + 15L) / 16), row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
+    const long blocks = (col_blocks + 7L) / 8 * 8 * row_blocks;
+    if (!fits(blocks, 256) || !fits((M + 3L) / 4, 256)) return too_large();
+    int* exponent = (int*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
+    hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, exponent, M, K);
     const int stage = 2 * mt * parts * 4096, leave = 4 * 16 * (nt * 16 + 4) * 4;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((col_blocks + 7) / 8 * 8 * row_blocks)), dim3(256), (size_t)(stage > leave ? stage : leave), st, (const unsigned char*)workspace, factor,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), (size_t)(stage > leave ? stage : leave), st, (const unsigned char*)workspace, exponent,
                        (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu, row_blocks, col_blocks);
+    return check_launch("int4_linear");
   };
   const auto rows = [&](auto kernel, auto* t, int mt, int nt) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int each = mt * Operand<T>::kRows, row_blocks = (M + each - 1) / each;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 4L * nt - 1) / (4 * nt) * row_blocks)), dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias,
+    const int each = mt * Operand<T>::kRows, row_blocks = (int)((M + each - 1L) / each);
+    const long blocks = (tiles + 4L * nt - 1) / (4 * nt) * row_blocks;
+    if (!fits(blocks, 256)) return too_large();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias,
                        (T*)out, M, N, K, gelu, row_blocks);
+    return check_launch("int4_linear");
   };
   const auto parts = [&](auto* t, auto g) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int G = decltype(g)::value;
-    const int places = (M + Operand<T>::kRows - 1) / Operand<T>::kRows;      // times 16
+    const int places = (int)((M + Operand<T>::kRows - 1L) / Operand<T>::kRows);      // times 16
     if (many_rows(M, N, K, dtype)) {
       // 64 rows by 128 of W (fp32: 32 by 128) where there are two rounds of such workgroups, else 32 by 64: 768 -> 30528 M = 512 62 us by 32 x 64, 45 by 32 x 128, 39 by
       // 64 x 128 and 64 x 256, 42 by 128 x 128; fp32 82, 63, 66 and 65; 7168 -> 1792 39, 41, 51, 79 and 76
@@ -670,10 +681,9 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     return kt < 16 ? go(int4_few_rows_kernel<T, G, true, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, true, 2, 8>, t, 2, 8);
   };
   const auto pick = [&](auto* t) {
-    if (group == 32) parts(t, std::integral_constant<int, 32>{});
-    else if (group == 64) parts(t, std::integral_constant<int, 64>{});
-    else parts(t, std::integral_constant<int, 128>{});
+    if (group == 32) return parts(t, std::integral_constant<int, 32>{});
+    if (group == 64) return parts(t, std::integral_constant<int, 64>{});
+    return parts(t, std::integral_constant<int, 128>{});
   };
-  dtype == M2_DTYPE_F32 ? pick((float*)nullptr) : pick((uint16_t*)nullptr);
-  return check_launch("int4_linear");
+  return dtype == M2_DTYPE_F32 ? pick((float*)nullptr) : pick((uint16_t*)nullptr);
 }

@@ -37,7 +37,8 @@ class Int4Linear(nn.Module):
 
     x fp32 or bf16 (..., in_features) on the GPU, rows any distance apart; y of the same type (bf16 for fp32 input under CUDA autocast); products are exact,
     sums fp32, rounded once.  Large products of many rows take x as half-precision parts of its row's size: fp32 to 22 bits, and values 2^-29 of their row's
-    largest (scales 2^-17 of theirs) lose bits.  Rows of magnitudes above 2^115 may overflow inside a sum.  Weights are constants: an input that asks for gradients is refused.  `weight` holds codes and scales in the kernel's order
+    largest (scales 2^-17 of theirs) lose bits.  Rows of magnitudes above 2^115 may overflow inside a sum; a row
+    that holds an infinity or NaN has no finite result.  Weights are constants: an input that asks for gradients is refused.  `weight` holds codes and scales in the kernel's order
     (include/m2_amd.h); make it with `from_linear`, `from_weight` or `from_packed`."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, group_size: int = 64, device=None):
@@ -125,8 +126,9 @@ def _in_tiles(codes: torch.Tensor, scales: torch.Tensor, K: int, group: int) -> 
     # the power of two that takes a row's largest scale to [1 / 2, 1)
     most = scales.float().abs().amax(1)
     exponent = torch.where(torch.isfinite(most) & (most > 0), torch.frexp(most).exponent, torch.zeros_like(most, dtype=torch.int32))
-    factor = torch.ones(nt * 16, device=codes.device)
-    factor[:N] = torch.ldexp(factor[:N], -exponent.clamp(-120, 120))
+    factor = torch.full((nt * 16,), 127, dtype=torch.int32, device=codes.device)
+    factor[:N] -= exponent.clamp(-120, 120)
+    factor <<= 23      # as fp32; torch.ldexp multiplies by pow(2, e), which is not always a power of two on the GPU
     return torch.cat((torch.cat((tiles, s), -1).reshape(-1), factor.view(torch.uint8)))
 
 

@@ -193,6 +193,41 @@ def test_ranges_of_rows_and_scales(gpu, dtype, N):
         assert ((lin(x).double() - y).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_powers_that_cancel(gpu, dtype):
+    """Rows whose largest value, 2^115, meets codes that stand for zero, times scales of 2^38; rows of 2^-140 times scales of 2^60: what comes out is in range."""
+    import m2_amd
+    M, N, K, group = 200, 40_000, 512, 64
+    codes, scales, packed, w = weights(gpu, N, K, group)
+    codes[:, 0] = 8
+    packed = (codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8).to(gpu)
+    for big, small, power in ((2.0 ** 115, 2.0 ** 80, 38), (2.0 ** -140, 2.0 ** -140, 60)):
+        s = (scales.float() * 2.0 ** power).to(torch.bfloat16)
+        lin = m2_amd.Int4Linear.from_packed(packed, s, K, group)
+        x = (rows(gpu, M, K, dtype=torch.float32) * small).to(dtype)
+        x[:, 0] = big
+        y = x.double() @ ((codes.to(gpu) - 8).double() * s.double().repeat_interleave(group, 1)).t()
+        most = s.double().abs().amax(1)
+        size = x[:, 1:].double().abs().amax(1, keepdim=True) * most
+        # a row's values become multiples of 2^-24 where its largest is 2^14 or more: each is off by 2^-39 of the largest at most, and is taken 8 times a scale
+        largest = x.double().abs().amax(1, keepdim=True)
+        tol = 8 * U * 55 * math.sqrt(group) * math.sqrt(2 * K + 64) * size + K * 8 * 2.0 ** -39 * largest * most + torch.finfo(dtype).eps / 2 * y.abs()
+        got = lin(x).double()
+        assert torch.isfinite(got).all() and ((got - y).abs() <= tol).all()
+
+
+def test_factors_are_powers_of_two(gpu):
+    """Weights laid out on the GPU hold the same bytes as on the CPU, scales of all sizes."""
+    import m2_amd
+    exponents = torch.arange(-126, 128)
+    scales = torch.ldexp(torch.full((254,), 1.25), exponents).to(torch.bfloat16)[:, None]
+    codes = torch.randint(0, 256, (254, 16), dtype=torch.uint8, generator=torch.Generator().manual_seed(0))
+    a, b = (m2_amd.Int4Linear.from_packed(codes.to(d), scales.to(d), 32, 32).weight.cpu() for d in ("cpu", gpu))
+    assert torch.equal(a, b)
+    factor = b[-256 * 4:].view(torch.float32)
+    assert (torch.frexp(factor).mantissa == 0.5).all() and torch.equal(torch.frexp(factor[:254]).exponent, 1 - (exponents + 1).clamp(-120, 120).to(torch.int32))
+
+
 def test_views_of_negatives(gpu):
     """Rows whose memory holds the negatives of their values, as imaginary parts of conjugates do."""
     import m2_amd
@@ -296,3 +331,6 @@ def test_refusals(gpu):
         ops.int4_linear(x, lin.weight[:-1], 10, 64)
     with pytest.raises(ValueError):
         ops.int4_linear(x, lin.weight, 10, 48)
+    one = m2_amd.Int4Linear(1, 1, device=gpu)
+    with pytest.raises(RuntimeError, match="more workgroups than a launch holds"):
+        one(torch.zeros(1, 1, device=gpu, dtype=torch.bfloat16).expand(2 ** 30, 1))
