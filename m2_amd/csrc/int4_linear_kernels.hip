@@ -71,7 +71,13 @@ template <> struct Operand<uint16_t> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (2 * i < n ? p[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] << 16 : 0u);
   }
-  __device__ __forceinline__ void keep(bool is) { v = is ? v : u32x4{0, 0, 0, 0}; }
+  // the values from the n-th on, 0 behind them
+  __device__ __forceinline__ void drop(int n) {
+    if (n & 4) v = u32x4{v[2], v[3], 0, 0};
+    if (n & 2) v = u32x4{v[1], v[2], v[3], 0};
+    if (n & 1) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    if (n >= 8) v = u32x4{0, 0, 0, 0};
+  }
   __device__ __forceinline__ bf16x8 get(int) const { return __builtin_bit_cast(bf16x8, v); }
   __device__ __forceinline__ void values(float (&f)[8]) const {
 #pragma unroll
@@ -90,7 +96,12 @@ template <> struct Operand<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = i < n ? __float_as_uint(p[i]) : 0u;
   }
-  __device__ __forceinline__ void keep(bool is) { v[0] = is ? v[0] : u32x4{0, 0, 0, 0}, v[1] = is ? v[1] : u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ void drop(int n) {
+    if (n & 4) v[0] = v[1], v[1] = u32x4{0, 0, 0, 0};
+    if (n & 2) v[0] = u32x4{v[0][2], v[0][3], v[1][0], v[1][1]}, v[1] = u32x4{v[1][2], v[1][3], 0, 0};
+    if (n & 1) v[0] = u32x4{v[0][1], v[0][2], v[0][3], v[1][0]}, v[1] = u32x4{v[1][1], v[1][2], v[1][3], 0};
+    if (n >= 8) v[0] = v[1] = u32x4{0, 0, 0, 0};
+  }
   __device__ __forceinline__ void values(float (&f)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i / 4][i % 4]);
@@ -112,14 +123,16 @@ template <> struct Operand<float> {
   }
 };
 
-// The eight values of a row from column k on, 0 behind the last: where K is a multiple of eight (EVEN), all of them or none; else one by one.
-template <typename T, bool EVEN>
+// The eight values of a row from column k on, 0 behind the last.  They are the last of the eight that end with the row, so that nothing is read one by one: that
+// took 27.6 us for 16 x 1001 -> 30528, this way 9.3.  Rows of less than eight (SHORT) have no such eight.
+template <typename T, bool SHORT>
 __device__ __forceinline__ void load_edge(Operand<T>& to, const T* row, int k, int K) {
-  if (EVEN) {
-    to.load(row + (k < K ? k : 0));
-    to.keep(k < K);
-  } else {
+  if (SHORT) {
     to.one(row + k, K - k);
+  } else {
+    const int from = min(k, K - 8);
+    to.load(row + from);
+    to.drop(k - from);
   }
 }
 
@@ -141,7 +154,7 @@ struct Scales {
 };
 
 // 128 columns of x's rows and of NT tiles of W: what a wave has asked for, and what it makes of it.
-template <typename T, int GROUP, bool EVEN, int NT>
+template <typename T, int GROUP, bool SHORT, int NT>
 struct Step {
   u32x4 q[NT];
   Scales<GROUP> s[NT];
@@ -160,7 +173,7 @@ struct Step {
       for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) load_edge<T, EVEN>(x[i], row, k + i * 32, K);
+      for (int i = 0; i < 4; ++i) load_edge<T, SHORT>(x[i], row, k + i * 32, K);
     }
   }
   __device__ __forceinline__ void add(floatx4 (&sum)[NT], const Bf16Codes& codes, int lane) const {
@@ -197,20 +210,20 @@ constexpr int waves_of(int split) { return split > 4 ? split : 4; }
 
 // Up to 16 rows of bf16 or 4 of fp32.  A wave has NT tiles of 16 rows of W, and of their tiles of 128 columns every SPLIT-th; the SPLIT waves' sums meet in shared
 // memory.
-template <typename T, int GROUP, bool EVEN, int NT, int SPLIT>
+template <typename T, int GROUP, bool SHORT, int NT, int SPLIT>
 __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
                                                             T* __restrict__ out, int M, int N, int K, int gelu) {
   __shared__ floatx4 sums[SPLIT > 1 ? waves_of(SPLIT) : 1][SPLIT > 1 ? NT : 1][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
-  const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT;
+  const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
   const Bf16Codes codes;
   floatx4 sum[NT] = {};
   if (t0 < tiles) {
     const long apart = (long)kt * tile_bytes(GROUP);
     const unsigned char* mine = w + t0 * apart;
-    const T* row = x + (long)min(Operand<T>::row(lane), M - 1) * x_row;
-    Step<T, GROUP, EVEN, NT> now, next;
+    const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
+    Step<T, GROUP, SHORT, NT> now, next;
     if (part < kt) now.load(mine, apart, tiles - t0, row, part, K, lane);
     for (int b = part; b < kt; b += SPLIT) {
       if (b + SPLIT < kt) next.load(mine, apart, tiles - t0, row, b + SPLIT, K, lane);
@@ -237,12 +250,12 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
     if (n >= N) continue;
     const float b = bias ? bias[n] : 0.f;
     if constexpr (sizeof(T) == 4) {
-      const int m = lane >> 4;
+      const int m = m0 + (lane >> 4);
       if (m < M) put(out, (long)m * N + n, (sum[t][2] + sum[t][1]) + sum[t][0] + b, gelu);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int m = (lane >> 4) * 4 + i;
+        const int m = m0 + (lane >> 4) * 4 + i;
         if (m < M) put(out, (long)m * N + n, sum[t][i] + b, gelu);
       }
     }
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
 // columns after the other in two buffers, in the operand's order: 64 lanes times 16 bytes for each 16 places and 32 columns.  A lane's place among
 // the 16 of its eighth is turned by the number of the eighth, so that the threads that write a row's sixteen eighths meet in no bank; readers are permuted
 // among themselves.
-template <typename T, bool EVEN, int MT>
+template <typename T, bool SHORT, int MT>
 struct Staged {
   static constexpr int kRows = MT * Operand<T>::kRows, kBytes = MT * 4 * 1024, kEach = kRows / 16;      // kEach: eighths of a thread
   static_assert(kRows % 16 == 0, "a row for every 16 threads");
@@ -263,7 +276,7 @@ struct Staged {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const T* row = x + (long)min(m0 + (int)(threadIdx.x >> 4) + 16 * i, M - 1) * x_row;
-      if ((b + 1) * kTileK <= K) v[i].load(row + k); else load_edge<T, EVEN>(v[i], row, k, K);
+      if ((b + 1) * kTileK <= K) v[i].load(row + k); else load_edge<T, SHORT>(v[i], row, k, K);
     }
   }
   __device__ __forceinline__ void store(unsigned char* to) const {
@@ -285,20 +298,20 @@ struct Staged {
   }
 };
 
-template <typename T, int GROUP, bool EVEN, int MT, int NT>
+template <typename T, int GROUP, bool SHORT, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
                                                         T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks) {
   constexpr int kSteps = GROUP / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char staged[2][Staged<T, EVEN, MT>::kBytes];
+  __shared__ __attribute__((aligned(16))) unsigned char staged[2][Staged<T, SHORT, MT>::kBytes];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
-  const int m0 = (int)(blockIdx.x % row_blocks) * Staged<T, EVEN, MT>::kRows, t0 = ((int)(blockIdx.x / row_blocks) * 4 + wave) * NT;
+  const int m0 = (int)(blockIdx.x % row_blocks) * Staged<T, SHORT, MT>::kRows, t0 = ((int)(blockIdx.x / row_blocks) * 4 + wave) * NT;
   const unsigned char* mine[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) mine[t] = w + (long)min(t0 + t, tiles - 1) * kt * tile_bytes(GROUP);
   const Bf16Codes codes;
   floatx4 sum[MT][NT] = {};
-  Staged<T, EVEN, MT> x_now;
+  Staged<T, SHORT, MT> x_now;
   u32x4 q[NT], q_next[NT];
   Scales<GROUP> s[NT], s_next[NT];
   const auto ask = [&](int b) {
@@ -327,7 +340,7 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
         c0[m] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-          a[m][i] = Staged<T, EVEN, MT>::read(from, m, g * kSteps + i, lane);
+          a[m][i] = Staged<T, SHORT, MT>::read(from, m, g * kSteps + i, lane);
           c0[m] = mfma(a[m][i], minus24(), c0[m]);
         }
       }
@@ -666,19 +679,19 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     if (places > 1) {
       constexpr int kMt = sizeof(T) == 4 ? 4 : 2;      // 32 rows of bf16, 16 of fp32
       const long blocks = (places + kMt - 1L) / kMt * ((tiles + 7) / 8);
-      if (K % 8) return rows(int4_rows_kernel<T, G, false, kMt, 1>, t, kMt, 1);
-      if (blocks < 512) return rows(int4_rows_kernel<T, G, true, kMt, 1>, t, kMt, 1);
-      return rows(int4_rows_kernel<T, G, true, kMt, 2>, t, kMt, 2);
+      if (K < 8) return rows(int4_rows_kernel<T, G, true, kMt, 1>, t, kMt, 1);
+      if (blocks < 512) return rows(int4_rows_kernel<T, G, false, kMt, 1>, t, kMt, 1);
+      return rows(int4_rows_kernel<T, G, false, kMt, 2>, t, kMt, 2);
     }
     // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
     // long rows are shared by eight waves.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
     // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
     // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7.
-    if (K % 8) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
-    if (tiles < 384) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
+    if (K < 8) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
+    if (tiles < 384) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
     if (tiles >= 1024 && (sizeof(T) == 4 || M > 8))
-      return kt < 16 ? go(int4_few_rows_kernel<T, G, true, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, true, 4, 8>, t, 4, 8);
-    return kt < 16 ? go(int4_few_rows_kernel<T, G, true, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, true, 2, 8>, t, 2, 8);
+      return kt < 16 ? go(int4_few_rows_kernel<T, G, false, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, false, 4, 8>, t, 4, 8);
+    return kt < 16 ? go(int4_few_rows_kernel<T, G, false, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, false, 2, 8>, t, 2, 8);
   };
   const auto pick = [&](auto* t) {
     if (group == 32) return parts(t, std::integral_constant<int, 32>{});
