@@ -271,19 +271,19 @@ struct Staged {
   static constexpr int kRows = MT * Operand<T>::kRows, kBytes = MT * 4 * 1024, kEach = kRows / 16;      // kEach: eighths of a thread
   static_assert(kRows % 16 == 0, "a row for every 16 threads");
   Operand<T> v[kEach];
-  __device__ __forceinline__ void load(const T* x, long x_row, int m0, int M, int b, int K) {
-    const int k = b * kTileK + (threadIdx.x & 15) * 8;
+  __device__ __forceinline__ void load(const T* x, long x_row, int m0, int M, int b, int K, int tid) {
+    const int k = b * kTileK + (tid & 15) * 8;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const T* row = x + (long)min(m0 + (int)(threadIdx.x >> 4) + 16 * i, M - 1) * x_row;
+      const T* row = x + (long)min(m0 + (tid >> 4) + 16 * i, M - 1) * x_row;
       if ((b + 1) * kTileK <= K) v[i].load(row + k); else load_edge<T, SHORT>(v[i], row, k, K);
     }
   }
-  __device__ __forceinline__ void store(unsigned char* to) const {
-    const int c = threadIdx.x & 15;
+  __device__ __forceinline__ void store(unsigned char* to, int tid) const {
+    const int c = tid & 15;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int row = (int)(threadIdx.x >> 4) + 16 * i;
+      const int row = (tid >> 4) + 16 * i;
       constexpr int kPlaces = sizeof(T) == 4 ? 3 : 1, kSpread = sizeof(T) == 4 ? 4 : 1;
 #pragma unroll
       for (int part = 0; part < kPlaces; ++part) {
@@ -298,12 +298,12 @@ struct Staged {
   }
 };
 
-template <typename T, int GROUP, bool SHORT, int MT, int NT>
-__global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
+template <typename T, int GROUP, bool SHORT, int MT, int NT, int SPLIT>
+__global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
                                                         T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks) {
   constexpr int kSteps = GROUP / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char staged[2][Staged<T, SHORT, MT>::kBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) unsigned char staged[SPLIT][2][Staged<T, SHORT, MT>::kBytes];
+  const int tid = threadIdx.x & 255, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
   const int m0 = (int)(blockIdx.x % row_blocks) * Staged<T, SHORT, MT>::kRows, t0 = ((int)(blockIdx.x / row_blocks) * 4 + wave) * NT;
   const unsigned char* mine[NT];
@@ -321,16 +321,23 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
       q_next[t] = *reinterpret_cast<const u32x4*>(p + lane * 16);
       s_next[t].load(p, lane);
     }
-    x_now.load(x, x_row, m0, M, b, K);
+    x_now.load(x, x_row, m0, M, b, K, tid);
   };
-  ask(0);
-  x_now.store(staged[0]);
+  if (part < kt) {
+    ask(part);
+    x_now.store(staged[part][0], tid);
+  }
   __syncthreads();
-  for (int b = 0; b < kt; ++b) {
+  for (int n = 0, b = part; n * SPLIT < kt; ++n, b += SPLIT) {
+    const bool more = b + SPLIT < kt;
+    if (SPLIT > 1 && b >= kt) {      // other parts have a tile more
+      __syncthreads();
+      break;
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) q[t] = q_next[t], s[t] = s_next[t];
-    if (b + 1 < kt) ask(b + 1);
-    const unsigned char* from = staged[b & 1];
+    if (more) ask(b + SPLIT);
+    const unsigned char* from = staged[part][n & 1];
 #pragma unroll
     for (int g = 0; g < kTileK / GROUP; ++g) {
       bf16x8 a[MT][kSteps];
@@ -360,7 +367,17 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
         }
       }
     }
-    if (b + 1 < kt) x_now.store(staged[(b + 1) & 1]);
+    if (more) x_now.store(staged[part][(n + 1) & 1], tid);
+    __syncthreads();
+  }
+  if (SPLIT > 1) {
+    // the parts' sums meet where their rows were; each part takes a share of the tiles on
+    static_assert(NT <= 2, "sums fit into a part's two stages");
+    floatx4* const mine_sums = reinterpret_cast<floatx4*>(staged[part]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) mine_sums[(m * NT + t) * 256 + tid] = sum[m][t];
     __syncthreads();
   }
 #pragma unroll
@@ -370,6 +387,12 @@ __global__ __launch_bounds__(256, 2) void int4_rows_kernel(const T* __restrict__
     const float bn = bias ? bias[n] : 0.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      if (SPLIT > 1) {
+        if ((m * NT + t) % SPLIT != part) continue;
+        sum[m][t] = reinterpret_cast<const floatx4*>(staged[0])[(m * NT + t) * 256 + tid];
+#pragma unroll
+        for (int p = 1; p < SPLIT; ++p) sum[m][t] += reinterpret_cast<const floatx4*>(staged[p])[(m * NT + t) * 256 + tid];
+      }
       if constexpr (sizeof(T) == 4) {
         const int row = m0 + m * 4 + (lane >> 4);
         if (row < M) put(out, (long)row * N + n, (sum[m][t][2] + sum[m][t][1]) + sum[m][t][0] + bn, gelu);
@@ -467,13 +490,13 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __
 
 // A workgroup has MT times 16 rows of x and 4 NT tiles of W's rows, NT a wave.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in
 // registers, once for MT products.
-template <typename T, int GROUP, int MT, int NT>
-__global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const int* __restrict__ exponent, const unsigned char* __restrict__ w,
+template <typename T, int GROUP, int MT, int NT, int SPLIT>
+__global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const int* __restrict__ exponent, const unsigned char* __restrict__ w,
                                                                 const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks, int col_blocks) {
   constexpr int kParts = sizeof(T) / 2, kStage = MT * kParts * 4096, kSteps = GROUP / 32;
-  extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages
+  extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages a part
   __shared__ int exponents[MT * 16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK, row_tiles = (M + 15) / 16;
   // workgroups of the same columns behind one another on the same XCD (they are dealt to the eight in turn)
   const int at = (int)blockIdx.x / 8, col = at / row_blocks * 8 + (int)blockIdx.x % 8;
@@ -498,14 +521,14 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
   Scales<GROUP> s[NT], s_next[NT];
   half2v scale[NT], off[NT];
   const ScaledCodes codes;
-  const unsigned lds0 = (unsigned)(uintptr_t)staged;
-  const auto ask = [&](int b) {
+  const unsigned lds0 = (unsigned)(uintptr_t)staged + part * 2 * kStage;
+  const auto ask = [&](int b, int stage) {
     // a wave fetches every fourth piece of 1024 bytes
 #pragma unroll
     for (int i = 0; i < MT * kParts; ++i) {
       const int piece = i * 4 + wave, m = piece / (4 * kParts);
       const unsigned char* from = x + (((long)min(m0 + m, row_tiles - 1) * kt + b) * kParts * 4 + piece % (4 * kParts)) * 1024;
-      load_to_lds(lds0 + (b & 1) * kStage + piece * 1024, lane * 16, from);
+      load_to_lds(lds0 + stage * kStage + piece * 1024, lane * 16, from);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -514,14 +537,15 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
       s_next[t].load(p, lane);
     }
   };
-  ask(0);
-  for (int b = 0; b < kt; ++b) {
+  if (part < kt) ask(part, 0);
+  for (int n = 0, b = part; n * SPLIT < kt; ++n, b += SPLIT) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) q[t] = q_next[t], s[t] = s_next[t];
     __builtin_amdgcn_s_waitcnt(kWaitVm0);      // this tile of x is there, of this wave's pieces
     __syncthreads();                           // of all; and nobody reads the other stage any more
-    if (b + 1 < kt) ask(b + 1);
-    const unsigned char* from = staged + (b & 1) * kStage + lane * 16;
+    if (SPLIT > 1 && b >= kt) break;           // other parts have a tile more
+    if (b + SPLIT < kt) ask(b + SPLIT, (n + 1) & 1);
+    const unsigned char* from = staged + (part * 2 + (n & 1)) * kStage + lane * 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       half8 a[kParts][MT];
@@ -547,7 +571,16 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
   // 16 rows at a time through shared memory, each wave by itself, so that a row's values leave together
   constexpr int kRow = NT * 16 + 4;
   __syncthreads();
-  float* const mine_out = reinterpret_cast<float*>(staged) + wave * 16 * kRow;
+  if (SPLIT > 1) {      // the parts' sums meet where their rows were
+    static_assert(NT <= 2 * kParts, "sums fit into a part's two stages");
+    floatx4* const sums = reinterpret_cast<floatx4*>(staged + part * 2 * kStage) + (threadIdx.x & 255);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sums[(m * NT + t) * 256] = sum[m][t];
+    __syncthreads();
+  }
+  float* const mine_out = reinterpret_cast<float*>(staged + (SPLIT > 1 ? SPLIT * 2 * kStage : 0)) + (threadIdx.x >> 6) * 16 * kRow;
   // the powers of two are put together as exponents: as numbers their product may be out of range where the result is not
   int en[NT];
 #pragma unroll
@@ -555,6 +588,16 @@ __global__ __launch_bounds__(256, 2) void int4_many_rows_kernel(const unsigned c
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if ((m0 + m) * 16 >= M) break;
+    if (SPLIT > 1) {
+      if (m % SPLIT != part) continue;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const floatx4* sums = reinterpret_cast<const floatx4*>(staged) + (m * NT + t) * 256 + (threadIdx.x & 255);
+        sum[m][t] = sums[0];
+#pragma unroll
+        for (int p = 1; p < SPLIT; ++p) sum[m][t] += sums[p * 2 * kStage / 16];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = (lane >> 4) * 4 + i;
@@ -607,16 +650,64 @@ extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
   return tiles * ((size_t)((K + kTileK - 1L) / kTileK) * (size_t)tile_bytes(group) + kTileN * sizeof(float));
 }
 
-// Whether x is written as half-precision operands first, 4 us that only a large product wins back.  us, the kernel of more rows / operands and the kernel of many:
-// 768 -> 30528 bf16 M = 64 10.8 / 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 39; 7168 -> 1792 M = 512 49 / 39; 960 -> 960 M = 200 7.5 / 11.3; fp32, whose rows are
-// two parts there and four places of 16 here, 768 -> 30522 M = 8 9.0 / 11.7, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 63.
-static bool many_rows(int M, int N, int K, int dtype) {
+// Which kernel a product runs on, with how many times 16 places of rows (MT) and tiles of 16 rows of W (NT) a wave, and how many parts of K.
+//
+// What a wave takes for a tile of 128 columns is mostly waiting, so the smallest workgroups of one round over the chip win, and K is split as far as registers and
+// shared memory go.  us, as it was before (32 rows of bf16 or 16 of fp32 a workgroup, K whole) / the few rows' kernel over MT = 1, NT = 1 / 2 / 4 / rows 2 1 4 / many 4 1 4 / many
+// 4 2 2, bf16, K -> N:
+//   1792 -> 1792 M = 32 10.0 / 4.0 / 5.1 / 7.0 / 7.0; M = 128 10.2 / 9.6 / 7.0 / 7.1 / 7.3 / 12.9; M = 256 11.5 / 15.4 / 12.2 / 10.4 / 8.1 / 13.4
+//   4096 -> 2000 M = 64 20.4 / 11.3 / 8.3 / 8.8 / 12.1 / 17.9; M = 256 22.7 / 35 / 23 / 16.9 / 13.9 / 21.0; M = 512 28.7 / 68 / 43 / 32 / 26.9 / 24.3
+//   7168 -> 1792 M = 128 34.6 / 30.5 / 18.6 / 13.4 / 19.1 / 27.6; M = 512 41.7 / 101 / 57 / 46 / 37.6 / 33.6 / 45
+//   4096 -> 8192 M = 64 23 / 36 / 22 / 16.9 / 14.0 / 19.2; M = 128 27 / 67 / 40 / 31 / 26 / 21.8 / 27.6; M = 256 41 / - / - / 58 / 49 / 38 / 31.5
+// fp32 (rows 4 1 2 / many 1 1 4 / 2 1 4 / 2 2 2):
+//   5672 -> 1200 M = 8 32 / 8.2 / 9.4 / 12.4 / 26.6; M = 64 36 / 28 / 21 / 25 / 27.8 / 22.4 / 27.1; M = 256 40 / - / - / 64 / 59 / 39 / 32.1 / 41
+//   4096 -> 8192 M = 32 26.6 / 56 / 37 / 34 / 23.2 / 18.3 / 20.9; M = 64 29 / - / - / - / 46 / 29.3 / 23.6 / 29.7; M = 128 38 / - / - / - / 88 / 50 / 39.5 / 33.9
+// Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 10.8 /
+// 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 37; 1792 -> 4096 M = 256 12.9 / 14.6; fp32 1792 -> 1792 M = 64 10.5 / 11.4, 4096 -> 2000 M = 64 21.4 / 17.5, 768 -> 30522 M = 16
+// 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 60.
+struct Plan {
+  enum Kernel { kFew, kRows, kMany } kernel;
+  int mt, nt, split;
+};
+static Plan plan_of(int M, int N, int K, int dtype) {
+  const bool f32 = dtype == M2_DTYPE_F32;
+  const long tiles = (N + kTileN - 1L) / kTileN, kt = (K + kTileK - 1L) / kTileK, round = num_cus();
+  const long places = f32 ? (M + 3L) / 4 : (M + 15L) / 16;      // times 16 places of an operand
+  const auto blocks = [&](int rows, int columns) { return (M + rows - 1L) / rows * ((tiles + columns - 1) / columns); };      // of `rows` rows and `columns` tiles
+  if (places == 1) {
+    // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
+    // long rows are shared by eight waves.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
+    // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
+    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7.
+    if (K < 8 || tiles < 384) return {Plan::kFew, 1, 1, 8};
+    return {Plan::kFew, 1, tiles >= 1024 && (f32 || M > 8) ? 4 : 2, kt < 16 ? 4 : 8};
+  }
+  if (K >= 8)
+    for (int nt = 1; nt <= 4; nt *= 2)
+      if (places * ((tiles + nt - 1) / nt) <= round) return {Plan::kFew, 1, nt, 8};
   const double products = (double)M * N * K;
-  return dtype == M2_DTYPE_F32 ? M > 16 && products >= 4e8 : M > 128 && products >= 3e9;
+  if (f32) {
+    if (products >= 4e8) {
+      if (blocks(16, 4) <= round) return {Plan::kMany, 1, 1, 4};
+      if (blocks(32, 4) <= round) return {Plan::kMany, 2, 1, 4};
+      if (blocks(32, 8) <= round) return {Plan::kMany, 2, 2, 2};
+      return {Plan::kMany, 2, 2, 1};
+    }
+    if (K >= 8 && blocks(16, 4) <= round) return {Plan::kRows, 4, 1, 2};
+    return {Plan::kRows, 4, K >= 8 && blocks(16, 8) >= 2 * round ? 2 : 1, 1};
+  }
+  if (K >= 8 && blocks(32, 4) <= round) return {Plan::kRows, 2, 1, 4};
+  if (M > 64 && products >= 3e9) {
+    if (blocks(64, 4) <= round) return {Plan::kMany, 4, 1, 4};
+    if (blocks(64, 8) <= round) return {Plan::kMany, 4, 2, 2};
+    return {Plan::kMany, 4, 2, 1};
+  }
+  if (K >= 8 && blocks(32, 4) <= 2 * round) return {Plan::kRows, 2, 1, 2};
+  return {Plan::kRows, 2, K >= 8 && blocks(32, 8) >= 2 * round ? 2 : 1, 1};
 }
 
 extern "C" size_t m2_int4_workspace_bytes(int M, int N, int K, int dtype) {
-  if (M <= 0 || N <= 0 || K <= 0 || !many_rows(M, N, K, dtype)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || plan_of(M, N, K, dtype).kernel != Plan::kMany) return 0;
   const size_t row_tiles = (size_t)((M + 15L) / 16), kt = (size_t)((K + kTileK - 1L) / kTileK);
   return row_tiles * (kt * (dtype == M2_DTYPE_F32 ? 8192 : 4096) + 16 * sizeof(int));
 }
@@ -639,59 +730,60 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   const auto too_large = [&] { return set_error(M2_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d are more workgroups than a launch holds", who, M, N, K); };
   const auto go = [&](auto kernel, auto* t, int nt, int split) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split), blocks = (waves + each - 1) / each;
-    if (!fits(blocks, 64 * each)) return too_large();
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * each), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
+    const long waves = (tiles + nt - 1L) / nt * split, each = waves_of(split), blocks = (waves + each - 1) / each, places = (M + Operand<T>::kRows - 1L) / Operand<T>::kRows;
+    if (!fits(blocks * places, 64 * each)) return too_large();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)places), dim3(64 * each), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
     return check_launch("int4_linear");
   };
-  const auto many = [&](auto kernel, auto* t, int mt, int nt) {
+  const auto many = [&](auto kernel, auto* t, int mt, int nt, int split) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int row_tiles = (int)((M + 15L) / 16), row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
     const long blocks = (col_blocks + 7L) / 8 * 8 * row_blocks;
-    if (!fits(blocks, 256) || !fits((M + 3L) / 4, 256)) return too_large();
+    if (!fits(blocks, 256 * split) || !fits((M + 3L) / 4, 256)) return too_large();
     int* exponent = (int*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
+    const int stages = split * 2 * mt * parts * 4096, leave = split * 4 * 16 * (nt * 16 + 4) * 4, lds = split > 1 ? stages + leave : stages > leave ? stages : leave;
+    if (lds > 64 * 1024) {
+      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return set_error(M2_ERR_LAUNCH, "hipFuncSetAttribute(int4_many_rows): %s", hipGetErrorString(e));
+    }
     hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, exponent, M, K);
-    const int stage = 2 * mt * parts * 4096, leave = 4 * 16 * (nt * 16 + 4) * 4;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), (size_t)(stage > leave ? stage : leave), st, (const unsigned char*)workspace, exponent,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256 * split), (size_t)lds, st, (const unsigned char*)workspace, exponent,
                        (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu, row_blocks, col_blocks);
     return check_launch("int4_linear");
   };
-  const auto rows = [&](auto kernel, auto* t, int mt, int nt) {
+  const auto rows = [&](auto kernel, auto* t, int mt, int nt, int split) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int each = mt * Operand<T>::kRows, row_blocks = (int)((M + each - 1L) / each);
     const long blocks = (tiles + 4L * nt - 1) / (4 * nt) * row_blocks;
-    if (!fits(blocks, 256)) return too_large();
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias,
+    if (!fits(blocks, 256 * split)) return too_large();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256 * split), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias,
                        (T*)out, M, N, K, gelu, row_blocks);
     return check_launch("int4_linear");
   };
+  const Plan p = plan_of(M, N, K, dtype);
   const auto parts = [&](auto* t, auto g) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int G = decltype(g)::value;
-    const int places = (int)((M + Operand<T>::kRows - 1L) / Operand<T>::kRows);      // times 16
-    if (many_rows(M, N, K, dtype)) {
-      // 64 rows by 128 of W (fp32: 32 by 128) where there are two rounds of such workgroups, else 32 by 64: 768 -> 30528 M = 512 62 us by 32 x 64, 45 by 32 x 128, 39 by
-      // 64 x 128 and 64 x 256, 42 by 128 x 128; fp32 82, 63, 66 and 65; 7168 -> 1792 39, 41, 51, 79 and 76
-      constexpr int kMt = sizeof(T) == 4 ? 2 : 4;
-      if (((M + 16L * kMt - 1) / (16 * kMt)) * ((tiles + 7) / 8) >= 2L * num_cus()) return many(int4_many_rows_kernel<T, G, kMt, 2>, t, kMt, 2);
-      return many(int4_many_rows_kernel<T, G, 2, 1>, t, 2, 1);
+    constexpr bool kF32 = sizeof(T) == 4;
+    if (p.kernel == Plan::kFew) {
+      if (K < 8) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
+      if (p.nt == 1) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
+      if (p.nt == 2) return p.split == 4 ? go(int4_few_rows_kernel<T, G, false, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, false, 2, 8>, t, 2, 8);
+      return p.split == 4 ? go(int4_few_rows_kernel<T, G, false, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, false, 4, 8>, t, 4, 8);
     }
-    if (places > 1) {
-      constexpr int kMt = sizeof(T) == 4 ? 4 : 2;      // 32 rows of bf16, 16 of fp32
-      const long blocks = (places + kMt - 1L) / kMt * ((tiles + 7) / 8);
-      if (K < 8) return rows(int4_rows_kernel<T, G, true, kMt, 1>, t, kMt, 1);
-      if (blocks < 512) return rows(int4_rows_kernel<T, G, false, kMt, 1>, t, kMt, 1);
-      return rows(int4_rows_kernel<T, G, false, kMt, 2>, t, kMt, 2);
+    if (p.kernel == Plan::kRows) {
+      constexpr int kMt = kF32 ? 4 : 2;
+      if (K < 8) return rows(int4_rows_kernel<T, G, true, kMt, 1, 1>, t, kMt, 1, 1);
+      if (p.nt == 2) return rows(int4_rows_kernel<T, G, false, kMt, 2, 1>, t, kMt, 2, 1);
+      if (p.split == 1) return rows(int4_rows_kernel<T, G, false, kMt, 1, 1>, t, kMt, 1, 1);
+      if (kF32 || p.split == 2) return rows(int4_rows_kernel<T, G, false, kMt, 1, 2>, t, kMt, 1, 2);
+      if constexpr (!kF32) return rows(int4_rows_kernel<T, G, false, kMt, 1, 4>, t, kMt, 1, 4);
     }
-    // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
-    // long rows are shared by eight waves.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
-    // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
-    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7.
-    if (K < 8) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
-    if (tiles < 384) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
-    if (tiles >= 1024 && (sizeof(T) == 4 || M > 8))
-      return kt < 16 ? go(int4_few_rows_kernel<T, G, false, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, false, 4, 8>, t, 4, 8);
-    return kt < 16 ? go(int4_few_rows_kernel<T, G, false, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, false, 2, 8>, t, 2, 8);
+    constexpr int kMt = kF32 ? 2 : 4;
+    if (p.nt == 2) return p.split == 1 ? many(int4_many_rows_kernel<T, G, kMt, 2, 1>, t, kMt, 2, 1) : many(int4_many_rows_kernel<T, G, kMt, 2, 2>, t, kMt, 2, 2);
+    if constexpr (kF32)
+      if (p.mt == 1) return many(int4_many_rows_kernel<T, G, 1, 1, 4>, t, 1, 1, 4);
+    return many(int4_many_rows_kernel<T, G, kMt, 1, 4>, t, kMt, 1, 4);
   };
   const auto pick = [&](auto* t) {
     if (group == 32) return parts(t, std::integral_constant<int, 32>{});

@@ -60,6 +60,17 @@ def test_against_fp64(gpu, dtype, group, M, N, K):
     check(m2_amd.Int4Linear.from_packed(packed, scales, K, group)(x), x, w, scales, group)
 
 
+@pytest.mark.parametrize("M,N", [(20, 1200), (64, 1200), (120, 1200), (256, 1200), (512, 1200), (300, 1800), (100, 10_000), (50, 6000), (50, 20_000), (130, 30_522)])
+@pytest.mark.parametrize("K", [5, 100, 300, 520, 1000, 1403])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parts_of_long_rows(gpu, dtype, M, N, K):
+    """Sizes that are shared out differently, over rows, columns and parts of K, parts with no tile among them."""
+    import m2_amd
+    _, scales, packed, w = weights(gpu, N, K, 64)
+    x = rows(gpu, M, K, dtype=dtype)
+    check(m2_amd.Int4Linear.from_packed(packed, scales, K, 64)(x), x, w, scales, 64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("M,N", [(1, 70), (6, 70), (40, 70), (200, 70), (300, 51001)])
 def test_rows_any_distance_apart(gpu, dtype, M, N):
