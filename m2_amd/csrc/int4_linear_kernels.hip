@@ -676,11 +676,13 @@ static Plan plan_of(int M, int N, int K, int dtype) {
   const auto blocks = [&](int rows, int columns) { return (M + rows - 1L) / rows * ((tiles + columns - 1) / columns); };      // of `rows` rows and `columns` tiles
   if (places == 1) {
     // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
-    // long rows are shared by eight waves.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
+    // long rows are shared by eight waves, short ones by four where there are many tiles.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
     // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
-    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7.
+    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7;
+    // groups of 32, 1792 -> 15000 M = 1 7.3 / 6.9 / 6.4 / 8.0 / 6.9, 768 -> 17000 fp32 M = 1 7.6 / 5.7 / 5.4 / 6.9 / 7.2, 1536 -> 30522 fp32 M = 4 15.2 / 11.5 / 10.9 / 10.0 / 11.1.
     if (K < 8 || tiles < 384) return {Plan::kFew, 1, 1, 8};
-    return {Plan::kFew, 1, tiles >= 1024 && (f32 || M > 8) ? 4 : 2, kt < 16 ? 4 : 8};
+    const bool many = tiles >= 1536 || (kt >= 16 && tiles >= 1024);
+    return {Plan::kFew, 1, many && (f32 || M > 8) ? 4 : 2, kt < 16 && many ? 4 : 8};
   }
   if (K >= 8)
     for (int nt = 1; nt <= 4; nt *= 2)
