@@ -262,8 +262,8 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
   }
 }
 
-// More rows: a workgroup has MT times 16 places of rows (as Operand) and 4 NT tiles of W's rows, NT a wave.  x goes through shared memory, one tile of 128
-// columns after the other in two buffers, in the operand's order: 64 lanes times 16 bytes for each 16 places and 32 columns.  A lane's place among
+// More rows: a workgroup has MT times 16 places of rows (as Operand) and 4 NT tiles of W's rows, NT a wave, SPLIT times (every SPLIT-th tile of 128
+// columns, with sums that meet at the end).  x goes through shared memory, one tile of 128 columns after the other in two buffers, in the operand's order: 64 lanes times 16 bytes for each 16 places and 32 columns.  A lane's place among
 // the 16 of its eighth is turned by the number of the eighth, so that the threads that write a row's sixteen eighths meet in no bank; readers are permuted
 // among themselves.
 template <typename T, bool SHORT, int MT>
@@ -488,20 +488,20 @@ struct ScaledCodes : Codes {
 };
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// A workgroup has MT times 16 rows of x and 4 NT tiles of W's rows, NT a wave.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in
-// registers, once for MT products.
-template <typename T, int GROUP, int MT, int NT, int SPLIT>
-__global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const int* __restrict__ exponent, const unsigned char* __restrict__ w,
+// A workgroup has MT times 16 rows of x and WAVES NT tiles of W's rows, NT a wave, SPLIT times: every SPLIT-th tile of 128 columns, with sums that meet at
+// the end.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in registers, once for MT products.
+template <typename T, int GROUP, int MT, int NT, int SPLIT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPLIT / 4 : 2) void int4_many_rows_kernel(const unsigned char* __restrict__ x, const int* __restrict__ exponent, const unsigned char* __restrict__ w,
                                                                 const float* __restrict__ bias, T* __restrict__ out, int M, int N, int K, int gelu, int row_blocks, int col_blocks) {
   constexpr int kParts = sizeof(T) / 2, kStage = MT * kParts * 4096, kSteps = GROUP / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char staged[];      // two stages a part
   __shared__ int exponents[MT * 16];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES;
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK, row_tiles = (M + 15) / 16;
   // workgroups of the same columns behind one another on the same XCD (they are dealt to the eight in turn)
   const int at = (int)blockIdx.x / 8, col = at / row_blocks * 8 + (int)blockIdx.x % 8;
   if (col >= col_blocks) return;
-  const int m0 = at % row_blocks * MT, t0 = (col * 4 + wave) * NT;
+  const int m0 = at % row_blocks * MT, t0 = (col * WAVES + wave) * NT;
   const unsigned char* mine[NT];
   float row_factor[NT];
 #pragma unroll
@@ -523,10 +523,10 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_many_
   const ScaledCodes codes;
   const unsigned lds0 = (unsigned)(uintptr_t)staged + part * 2 * kStage;
   const auto ask = [&](int b, int stage) {
-    // a wave fetches every fourth piece of 1024 bytes
+    // pieces of 1024 bytes, dealt to the waves
 #pragma unroll
-    for (int i = 0; i < MT * kParts; ++i) {
-      const int piece = i * 4 + wave, m = piece / (4 * kParts);
+    for (int i = 0; i < MT * kParts * 4 / WAVES; ++i) {
+      const int piece = i * WAVES + wave, m = piece / (4 * kParts);
       const unsigned char* from = x + (((long)min(m0 + m, row_tiles - 1) * kt + b) * kParts * 4 + piece % (4 * kParts)) * 1024;
       load_to_lds(lds0 + stage * kStage + piece * 1024, lane * 16, from);
     }
@@ -572,12 +572,12 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_many_
   constexpr int kRow = NT * 16 + 4;
   __syncthreads();
   if (SPLIT > 1) {      // the parts' sums meet where their rows were
-    static_assert(NT <= 2 * kParts, "sums fit into a part's two stages");
-    floatx4* const sums = reinterpret_cast<floatx4*>(staged + part * 2 * kStage) + (threadIdx.x & 255);
+    static_assert(SPLIT == 1 || NT * WAVES <= 8 * kParts, "sums fit into a part's two stages");
+    floatx4* const sums = reinterpret_cast<floatx4*>(staged + part * 2 * kStage) + threadIdx.x % (64 * WAVES);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sums[(m * NT + t) * 256] = sum[m][t];
+      for (int t = 0; t < NT; ++t) sums[(m * NT + t) * 64 * WAVES] = sum[m][t];
     __syncthreads();
   }
   float* const mine_out = reinterpret_cast<float*>(staged + (SPLIT > 1 ? SPLIT * 2 * kStage : 0)) + (threadIdx.x >> 6) * 16 * kRow;
@@ -592,7 +592,7 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_many_
       if (m % SPLIT != part) continue;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const floatx4* sums = reinterpret_cast<const floatx4*>(staged) + (m * NT + t) * 256 + (threadIdx.x & 255);
+        const floatx4* sums = reinterpret_cast<const floatx4*>(staged) + (m * NT + t) * 64 * WAVES + threadIdx.x % (64 * WAVES);
         sum[m][t] = sums[0];
 #pragma unroll
         for (int p = 1; p < SPLIT; ++p) sum[m][t] += sums[p * 2 * kStage / 16];
@@ -664,10 +664,11 @@ extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
 //   4096 -> 8192 M = 32 26.6 / 56 / 37 / 34 / 23.2 / 18.3 / 20.9; M = 64 29 / - / - / - / 46 / 29.3 / 23.6 / 29.7; M = 128 38 / - / - / - / 88 / 50 / 39.5 / 33.9
 // Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 10.8 /
 // 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 37; 1792 -> 4096 M = 256 12.9 / 14.6; fp32 1792 -> 1792 M = 64 10.5 / 11.4, 4096 -> 2000 M = 64 21.4 / 17.5, 768 -> 30522 M = 16
-// 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 60.
+// 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 56.  Its workgroups have 4 NT tiles, and 8 NT where as much of the chip is used: 768 -> 30528 M = 256 19.7 / 19.1, 1792 -> 16000 M = 512 36.4 /
+// 35.4, 7168 -> 30528 M = 150 93 / 109 (717 and 360 workgroups), 768 -> 30528 fp32 M = 512 56.8 (32 rows by 4 NT) / 51.0 (64 by 8 NT), 4096 -> 8192 fp32 M = 256 43.6 / 58, 512 75 / 67.
 struct Plan {
   enum Kernel { kFew, kRows, kMany } kernel;
-  int mt, nt, split;
+  int mt, nt, split, waves = 4;      // waves: of kMany, times split
 };
 static Plan plan_of(int M, int N, int K, int dtype) {
   const bool f32 = dtype == M2_DTYPE_F32;
@@ -693,6 +694,7 @@ static Plan plan_of(int M, int N, int K, int dtype) {
       if (blocks(16, 4) <= round) return {Plan::kMany, 1, 1, 4};
       if (blocks(32, 4) <= round) return {Plan::kMany, 2, 1, 4};
       if (blocks(32, 8) <= round) return {Plan::kMany, 2, 2, 2};
+      if (blocks(64, 16) >= round) return {Plan::kMany, 4, 2, 1, 8};
       return {Plan::kMany, 2, 2, 1};
     }
     if (K >= 8 && blocks(16, 4) <= round) return {Plan::kRows, 4, 1, 2};
@@ -702,7 +704,9 @@ static Plan plan_of(int M, int N, int K, int dtype) {
   if (M > 64 && products >= 3e9) {
     if (blocks(64, 4) <= round) return {Plan::kMany, 4, 1, 4};
     if (blocks(64, 8) <= round) return {Plan::kMany, 4, 2, 2};
-    return {Plan::kMany, 4, 2, 1};
+    // what of its last round over the chip is in use
+    const auto use = [&](long b) { return (double)b / (double)((b + round - 1) / round * round); };
+    return {Plan::kMany, 4, 2, 1, use(blocks(64, 16)) > 0.9 * use(blocks(64, 8)) ? 8 : 4};
   }
   if (K >= 8 && blocks(32, 4) <= 2 * round) return {Plan::kRows, 2, 1, 2};
   return {Plan::kRows, 2, K >= 8 && blocks(32, 8) >= 2 * round ? 2 : 1, 1};
@@ -737,19 +741,19 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)places), dim3(64 * each), 0, st, (const T*)x, x_row, (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu);
     return check_launch("int4_linear");
   };
-  const auto many = [&](auto kernel, auto* t, int mt, int nt, int split) {
+  const auto many = [&](auto kernel, auto* t, int mt, int nt, int split, int waves) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int row_tiles = (int)((M + 15L) / 16), row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + 4 * nt - 1) / (4 * nt), parts = (int)sizeof(T) / 2;
+    const int row_tiles = (int)((M + 15L) / 16), row_blocks = (row_tiles + mt - 1) / mt, col_blocks = (tiles + waves * nt - 1) / (waves * nt), parts = (int)sizeof(T) / 2;
     const long blocks = (col_blocks + 7L) / 8 * 8 * row_blocks;
-    if (!fits(blocks, 256 * split) || !fits((M + 3L) / 4, 256)) return too_large();
+    if (!fits(blocks, 64 * waves * split) || !fits((M + 3L) / 4, 256)) return too_large();
     int* exponent = (int*)((unsigned char*)workspace + (size_t)row_tiles * kt * parts * 4096);
-    const int stages = split * 2 * mt * parts * 4096, leave = split * 4 * 16 * (nt * 16 + 4) * 4, lds = split > 1 ? stages + leave : stages > leave ? stages : leave;
+    const int stages = split * 2 * mt * parts * 4096, leave = split * waves * 16 * (nt * 16 + 4) * 4, lds = split > 1 ? stages + leave : stages > leave ? stages : leave;
     if (lds > 64 * 1024) {
       const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e != hipSuccess) return set_error(M2_ERR_LAUNCH, "hipFuncSetAttribute(int4_many_rows): %s", hipGetErrorString(e));
     }
     hipLaunchKernelGGL((int4_operand_kernel<T>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, (const T*)x, x_row, (half8*)workspace, exponent, M, K);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256 * split), (size_t)lds, st, (const unsigned char*)workspace, exponent,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * waves * split), (size_t)lds, st, (const unsigned char*)workspace, exponent,
                        (const unsigned char*)weight, bias, (T*)out, M, N, K, gelu, row_blocks, col_blocks);
     return check_launch("int4_linear");
   };
@@ -782,10 +786,15 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
       if constexpr (!kF32) return rows(int4_rows_kernel<T, G, false, kMt, 1, 4>, t, kMt, 1, 4);
     }
     constexpr int kMt = kF32 ? 2 : 4;
-    if (p.nt == 2) return p.split == 1 ? many(int4_many_rows_kernel<T, G, kMt, 2, 1>, t, kMt, 2, 1) : many(int4_many_rows_kernel<T, G, kMt, 2, 2>, t, kMt, 2, 2);
-    if constexpr (kF32)
-      if (p.mt == 1) return many(int4_many_rows_kernel<T, G, 1, 1, 4>, t, 1, 1, 4);
-    return many(int4_many_rows_kernel<T, G, kMt, 1, 4>, t, kMt, 1, 4);
+    if (p.nt == 2 && p.split == 2) return many(int4_many_rows_kernel<T, G, kMt, 2, 2, 4>, t, kMt, 2, 2, 4);
+    if (p.nt == 2 && p.waves == 8) return many(int4_many_rows_kernel<T, G, 4, 2, 1, 8>, t, 4, 2, 1, 8);
+    if constexpr (kF32) {
+      if (p.nt == 2) return many(int4_many_rows_kernel<T, G, 2, 2, 1, 4>, t, 2, 2, 1, 4);
+      if (p.mt == 1) return many(int4_many_rows_kernel<T, G, 1, 1, 4, 4>, t, 1, 1, 4, 4);
+    }
+    if constexpr (!kF32)
+      if (p.nt == 2) return many(int4_many_rows_kernel<T, G, 4, 2, 1, 4>, t, 4, 2, 1, 4);
+    return many(int4_many_rows_kernel<T, G, kMt, 1, 4, 4>, t, kMt, 1, 4, 4);
   };
   const auto pick = [&](auto* t) {
     if (group == 32) return parts(t, std::integral_constant<int, 32>{});
