@@ -2,11 +2,14 @@
 //
 // Their calls are a few microseconds of GPU time for a row or a handful of them, and checks, output tensors and the call through ctypes took
 // 10 to 17 us in Python (torch's own linear: 19), a gradient 100: here the same checks raise the same errors.  us a call, one stream, back to back, Python / here:
-// Int4Linear 768 x 768 11.8 / 7.5; token_logprobs 1 x 30522 17.0 / 8.7, 1 x 30522 fp32 with its gradient 118 / 66 (most of it torch's own backward pass).
+// Int4Linear 768 x 768 11.8 / 6.4 (the launch itself 3.0, the output tensor 0.7); token_logprobs 1 x 30522 17.0 / 7.9, 1 x 30522 fp32 with its gradient 118 / 66
+// (most of it torch's own backward pass).
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
@@ -30,7 +33,7 @@ decltype(&m2_token_scores_bwd) token_scores_bwd;
 template <typename F>
 void set(F& f, uintptr_t address) { f = reinterpret_cast<F>(address); }
 
-void bind(std::vector<uintptr_t> a) {
+void bind(const std::vector<uintptr_t>& a) {
   TORCH_CHECK(a.size() == 7, "seven addresses");
   set(last_error, a[0]);
   set(int4_weight_bytes, a[1]);
@@ -226,24 +229,95 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 
-using Results = std::tuple<optional<Tensor>, Tensor, optional<Tensor>, optional<Tensor>>;      // logprobs, entropy, ids, log probabilities of the alternatives
-
-optional<Tensor> given(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
-
-Results token_logprobs(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
+// The four results: log probabilities, entropy, ids and log probabilities of the alternatives; undefined where not asked for.
+std::array<Tensor, 4> token_logprobs(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     const variable_list v = TokenLogprobs::apply(logits, tokens, top_k, allowed, ignore_index);
     const bool has = tokens.has_value();
-    return {has ? given(v[1]) : std::nullopt, v[0], top_k ? given(v[1 + has]) : std::nullopt, top_k ? given(v[2 + has]) : std::nullopt};
+    return {has ? v[1] : Tensor(), v[0], top_k ? v[1 + has] : Tensor(), top_k ? v[2 + has] : Tensor()};
   }
-  const Found f = scores(logits, arguments(logits, tokens, top_k, allowed, ignore_index));
-  return {given(f.logprobs), f.entropy, given(f.ids), given(f.top)};
+  Found f = scores(logits, arguments(logits, tokens, top_k, allowed, ignore_index));
+  return {std::move(f.logprobs), std::move(f.entropy), std::move(f.ids), std::move(f.top)};
 }
+
+// Arguments come by position, without pybind's conversions (1.1 us a call).
+const Tensor& tensor(const char* name, PyObject* o) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": expected a tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+optional<Tensor> tensor_or_none(const char* name, PyObject* o) { return o == Py_None ? std::nullopt : optional<Tensor>(tensor(name, o)); }
+int64_t integer(PyObject* o) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+// Refuses what a kernel that is given a tensor's memory would answer wrongly: tensors that are no plain ones, transforms of functions (vmap, jvp, ...), traces,
+// forward-mode gradients, and (unless grad_ok) gradients.
+const Tensor& values(const char* name, PyObject* o, bool grad_ok) {
+  TORCH_CHECK_TYPE(THPVariable_CheckExact(o), name, ": expected a plain tensor, got ", Py_TYPE(o)->tp_name);
+  const Tensor& t = THPVariable_Unpack(o);
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !torch::jit::tracer::isTracing() && !t._fw_grad(0).defined(), name,
+              ": function transforms, traces and forward-mode gradients are not supported");
+  TORCH_CHECK(grad_ok || !t.requires_grad() || !at::GradMode::is_enabled(), name,
+              ": this operator has no gradient; call it under torch.no_grad() or on a detached tensor");
+  return t;
+}
+
+PyObject* object_of(Tensor t) {
+  if (!t.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(t));
+}
+
+// (x, weight, N, group, bias or None, gelu) -> y
+PyObject* py_int4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 6, "int4_linear: six arguments");
+  const Tensor &x = values("x", args[0], false), &weight = tensor("weight", args[1]);
+  const int64_t N = integer(args[2]), group = integer(args[3]);
+  const optional<Tensor> bias = tensor_or_none("bias", args[4]);
+  const bool gelu = args[5] == Py_True;
+  Tensor y;
+  {
+    const pybind11::gil_scoped_release free;
+    y = int4_linear(x, weight, N, group, bias, gelu);
+  }
+  return object_of(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// (logits, tokens or None, top_k, allowed or None, ignore_index) -> four results, None where not asked for
+PyObject* py_token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 5, "token_logprobs: five arguments");
+  const Tensor& logits = values("logits", args[0], true);
+  const optional<Tensor> tokens = tensor_or_none("tokens", args[1]), allowed = tensor_or_none("allowed", args[3]);
+  const int64_t top_k = integer(args[2]), ignore_index = integer(args[4]);
+  std::array<Tensor, 4> found;
+  {
+    const pybind11::gil_scoped_release free;
+    found = token_logprobs(logits, tokens, top_k, allowed, ignore_index);
+  }
+  auto results = pybind11::reinterpret_steal<pybind11::object>(PyTuple_New(4));
+  if (!results) throw python_error();
+  for (int i = 0; i < 4; ++i) {
+    PyObject* o = object_of(std::move(found[i]));
+    if (!o) throw python_error();
+    PyTuple_SET_ITEM(results.ptr(), i, o);
+  }
+  return results.release().ptr();
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef fast[] = {
+    {"int4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_int4_linear)), METH_FASTCALL, nullptr},
+    {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_token_logprobs)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
 
 }  // namespace
 
 PYBIND11_MODULE(_answer_calls, m) {
   m.def("bind", torch::wrap_pybind_function(bind));
-  m.def("int4_linear", torch::wrap_pybind_function_no_gil(int4_linear));
-  m.def("token_logprobs", torch::wrap_pybind_function_no_gil(token_logprobs));
+  if (PyModule_AddFunctions(m.ptr(), fast) != 0) throw pybind11::error_already_set();
 }

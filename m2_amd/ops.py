@@ -11,7 +11,6 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.forward_ad import unpack_dual as _unpack_dual
 
 from . import _lib
 from ._lib import HyenaFilterParams, SplitJob, M2_DTYPE_BF16, M2_DTYPE_F32, check, lib
@@ -749,25 +748,12 @@ def blockdiag_linear_layernorm(x: Tensor, w: Tensor, bias: Optional[Tensor], res
     return o32, o16, ot
 
 
-def require_values(t: Tensor, name: str, grad_ok: bool = False) -> None:
-    """Refuses what a kernel that is given a tensor's memory would answer wrongly: tensors that are no plain ones, transforms of functions (vmap, jvp,
-    ...), traces, forward-mode gradients, and (unless grad_ok) gradients."""
-    if type(t) not in (torch.Tensor, torch.nn.Parameter):
-        raise TypeError(f"{name}: expected a plain tensor, got {type(t).__name__}")
-    c = torch._C
-    if c._are_functorch_transforms_active() or c._get_tracing_state() is not None or _unpack_dual(t).tangent is not None:
-        raise RuntimeError(f"{name}: function transforms, traces and forward-mode gradients are not supported")
-    if not grad_ok and t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name}: this operator has no gradient; call it under torch.no_grad() or on a detached tensor")
-
-
 def int4_weight_bytes(N: int, K: int, group: int) -> int:
     return lib.m2_int4_weight_bytes(N, K, group)
 
 
 def int4_linear(x: Tensor, weight: Tensor, N: int, group: int, bias: Optional[Tensor] = None, activation: Optional[str] = None) -> Tensor:
     """act(x W^T + bias): x (..., K) fp32 or bf16, weight uint8 in the order of m2_int4_linear_fwd, bias (N) fp32 -> (..., N) of x's type."""
-    require_values(x, "x")
     if activation is not None and activation != "gelu":
         raise ValueError(f'activation must be None or "gelu", got {activation!r}')
     return _answer_calls.int4_linear(x, weight, N, group, bias, activation is not None)
@@ -776,5 +762,4 @@ def int4_linear(x: Tensor, weight: Tensor, N: int, group: int, bias: Optional[Te
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed: Optional[Tensor], ignore_index: int):
     """-> (log probabilities of `tokens` | None, entropies, alternatives' ids | None, their log probabilities | None), with a gradient where the logits ask for one;
     see scores.token_logprobs."""
-    require_values(logits, "logits", grad_ok=True)
     return _answer_calls.token_logprobs(logits, tokens, top_k, allowed, ignore_index)
