@@ -6,9 +6,11 @@
 // (most of it torch's own backward pass).
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -177,32 +179,29 @@ Found scores(const Tensor& logits, const Scores& s) {
 // A gradient of one value a row: it may be one value for all of them.
 Tensor per_row(const Tensor& g) { return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).reshape({-1}) : g; }
 
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
-struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed,
-                               int64_t ignore_index) {
-    const Scores s = arguments(logits, tokens, top_k, allowed, ignore_index);
-    const Found f = scores(logits, s);
-    ctx->save_for_backward({logits, s.tokens, s.allowed, f.entropy, f.stats, f.ids});
-    ctx->saved_data["top_k"] = top_k;
-    ctx->saved_data["ignore_index"] = ignore_index;
-    ctx->saved_data["allowed_row"] = s.allowed_row;
-    ctx->set_materialize_grads(false);
-    if (f.ids.defined()) ctx->mark_non_differentiable({f.ids});
-    variable_list out = {f.entropy};      // all outputs are defined: the entropy, the log probabilities where there are tokens, alternatives' ids and log probabilities
-    if (s.tokens.defined()) out.push_back(f.logprobs);
-    if (top_k) out.push_back(f.ids), out.push_back(f.top);
-    return out;
+// The graph's node.  Its inputs are the gradients of entropy, log probabilities and alternatives' log probabilities, undefined where there is none.
+struct TokenLogprobsBackward : torch::autograd::Node {
+  SavedVariable logits_, tokens_, allowed_, entropy_, stats_, ids_;
+  int64_t top_k = 0, ignore_index = 0, allowed_row = 0;
+  bool released = false;
+
+  std::string name() const override { return "TokenLogprobsBackward"; }
+
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* v : {&logits_, &tokens_, &allowed_, &entropy_, &stats_, &ids_}) v->reset_data();
+    released = true;
   }
 
-  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    const auto saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &tokens = saved[1], &allowed = saved[2], &entropy = saved[3], &stats = saved[4], &ids = saved[5];
-    const int64_t top_k = ctx->saved_data["top_k"].toInt();
-    const Tensor g_entropy = g[0], g_logprobs = tokens.defined() ? g[1] : Tensor(), g_alternatives = top_k ? g.back() : Tensor();
-    if (!g_entropy.defined() && !g_logprobs.defined() && !g_alternatives.defined()) return variable_list(5);
+  variable_list apply(variable_list&& g) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
+    const Tensor logits = logits_.unpack(), tokens = tokens_.unpack(), allowed = allowed_.unpack(), entropy = entropy_.unpack(shared_from_this()), stats = stats_.unpack(),
+                 ids = ids_.unpack();
+    if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return variable_list(1);
     Tensor grad;
     {
       const at::AutoDispatchBelowADInplaceOrView below;
@@ -210,11 +209,10 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
       const int64_t V = logits.size(-1), rows = logits.numel() / V;
       grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
       if (rows) {
-        const Tensor g_lp = per_row(g_logprobs), g_h = per_row(g_entropy),
-                     g_top = g_alternatives.defined() ? (g_alternatives.is_neg() ? g_alternatives.resolve_neg() : g_alternatives).contiguous() : g_alternatives;
-        const Rows r = rows_of(logits.detach(), 2);
-        check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(tokens)), ctx->saved_data["ignore_index"].toInt(),
-                               static_cast<const unsigned char*>(pointer(allowed)), ctx->saved_data["allowed_row"].toInt(), entropy.data_ptr<float>(), stats.data_ptr<float>(),
+        const Tensor g_h = per_row(g[0]), g_lp = per_row(g[1]), g_top = g[2].defined() ? (g[2].is_neg() ? g[2].resolve_neg() : g[2]).contiguous() : g[2];
+        const Rows r = rows_of(logits, 2);
+        check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(tokens)), ignore_index,
+                               static_cast<const unsigned char*>(pointer(allowed)), allowed_row, entropy.data_ptr<float>(), stats.data_ptr<float>(),
                                static_cast<const long long*>(pointer(ids)), static_cast<const float*>(pointer(g_lp)), g_lp.defined() ? g_lp.stride(0) : 0,
                                static_cast<const float*>(pointer(g_h)), g_h.defined() ? g_h.stride(0) : 0, static_cast<const float*>(pointer(g_top)), grad.data_ptr(), V, rows,
                                static_cast<int>(V), static_cast<int>(top_k), logits.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16, current_stream()));
@@ -225,18 +223,33 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
       grad.set_requires_grad(true);
       grad = (*node)({grad})[0];
     }
-    return {grad, Tensor(), Tensor(), Tensor(), Tensor()};
+    return {grad};
   }
 };
 
+Found scores_with_graph(const Tensor& logits, const Scores& s) {
+  const std::shared_ptr<TokenLogprobsBackward> node(new TokenLogprobsBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(logits));
+  Found f;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    f = scores(logits, s);
+  }
+  torch::autograd::set_history(variable_list{f.entropy, f.logprobs, f.top}, node);
+  node->logits_ = SavedVariable(logits, false);
+  node->tokens_ = SavedVariable(s.tokens, false);
+  node->allowed_ = SavedVariable(s.allowed, false);
+  node->entropy_ = SavedVariable(f.entropy, true);
+  node->stats_ = SavedVariable(f.stats, false);
+  node->ids_ = SavedVariable(f.ids, false);
+  node->top_k = s.top_k, node->ignore_index = s.ignore_index, node->allowed_row = s.allowed_row;
+  return f;
+}
+
 // The four results: log probabilities, entropy, ids and log probabilities of the alternatives; undefined where not asked for.
 std::array<Tensor, 4> token_logprobs(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
-  if (logits.requires_grad() && at::GradMode::is_enabled()) {
-    const variable_list v = TokenLogprobs::apply(logits, tokens, top_k, allowed, ignore_index);
-    const bool has = tokens.has_value();
-    return {has ? v[1] : Tensor(), v[0], top_k ? v[1 + has] : Tensor(), top_k ? v[2 + has] : Tensor()};
-  }
-  Found f = scores(logits, arguments(logits, tokens, top_k, allowed, ignore_index));
+  const Scores s = arguments(logits, tokens, top_k, allowed, ignore_index);
+  Found f = logits.requires_grad() && at::GradMode::is_enabled() ? scores_with_graph(logits, s) : scores(logits, s);
   return {std::move(f.logprobs), std::move(f.entropy), std::move(f.ids), std::move(f.top)};
 }
 
