@@ -1,19 +1,22 @@
 // y = act(x W^T + b) for few rows x, W (N, K) in 4 bits with a bf16 scale for each group of a row: W[n, k] = (q - 8) s, q in 0 .. 15.
 //
 // Few rows are bound by the weight, N K / 2 bytes and 2 N K / group of scales: 12.5 MB and 2.4 us for the word embeddings at K = 768, beside 3 us that any launch of
-// a few dependent loads takes.  Many rows are bound by what their instructions take: of 33 us at M = 512 the matrix unit is busy 28 % and the vector unit, which makes W
-// out of the codes, 42 % of the cycles, and on this chip the two hardly overlap.  Kernel times, MI355X (floor: bytes at 5.3 TB/s, products at 1.27 PFLOP/s):
+// a few dependent loads takes.  Many rows are bound by several things alike, which hardly overlap: of 33 us at M = 512 making W out of the codes takes 7, fetching x and W 7,
+// the products 12 (as copies of the kernel without one or two of these say; the matrix unit is busy 27 % of the cycles, the vector unit 42 %), and workgroups twice as wide or high, 64 x 64
+// instead of 64 x 32 to a wave, or another order of the instructions change nothing.  Kernel times, MI355X (floor: bytes at 5.3 TB/s, products at 1.27 PFLOP/s):
 //
 //   M x K -> N              us (floor)             M x K -> N                  us (floor)
-//   1 x 768 -> 30528        5.7 (2.4)              64 x 768 -> 30528           11.0 (3.1)
-//   16 x 768 -> 30528       7.3 (2.6)              128 x 768 -> 30528          17.1 (4.7)
-//   13 x 1536 -> 30522      8.2 (4.9)              512 x 768 -> 30528          33.1 + 4.6 (18.9)
-//   1 x 7168 -> 16384       11.7 (11.4)            4096 x 1792 -> 1792         37.6 + 9.5 (20.7)
-//   16 x 7168 -> 16384      13.6 (11.5)            40 x 768 -> 30522, fp32     13.7 + 4.2 (4.4)
-//   3 x 960 -> 960, fp32    3.5 (0.1)              512 x 768 -> 30528, fp32    57.9 + 4.9 (56: three products of bf16 parts)
+//   1 x 768 -> 30528        5.1 (2.4)              64 x 768 -> 30528           11.2 (3.1)
+//   16 x 768 -> 30528       7.2 (2.6)              128 x 768 -> 30528          11.9 + 4.2 (4.7)
+//   16 x 1001 -> 30522      9.2 (3.3)              512 x 768 -> 30528          33.4 + 4.5 (18.9)
+//   13 x 1536 -> 30522      8.0 (4.7)              4096 x 1792 -> 1792         34.9 + 9.5 (20.7)
+//   1 x 7168 -> 16384       11.8 (11.4)            40 x 768 -> 30522, fp32     11.7 + 4.2 (3.5)
+//   16 x 7168 -> 16384      13.7 (11.6)            512 x 768 -> 30528, fp32    51.4 + 4.9 (37.8: two products of half-precision parts)
+//   3 x 960 -> 960, fp32    3.6 (0.1)              8 x 5672 -> 1200, fp32      7.9 (0.7)
+//   64 x 4096 -> 2000       8.3 (1.0)              512 x 7168 -> 1792          23.5 + 8.3 (10.4)
 //
-// A product runs on one of three kernels: few rows (up to 16 of bf16, 4 of fp32) straight from memory, more of them with x in shared memory, many (many_rows) with x
-// as half-precision operands, which a launch of its own writes (behind the +).
+// A product runs on one of three kernels (plan_of): up to 16 rows of bf16 or 4 of fp32 straight from memory, and more of them so where W is small; more rows with x in shared
+// memory; large products with x as half-precision operands, which a launch of its own writes (behind the +).
 //
 // Order of the weights in memory: tiles of 16 rows n by 128 columns k, those of the same rows behind one another.  A tile is 64 lanes times 16 bytes, lane l
 // = 16 (k / 8 % 4) + n % 16 with the eight k of each of the four steps of 32 in a 32-bit word, value j of the eight at bit 16 (j % 2) + 4 (j / 2); behind them
@@ -208,7 +211,7 @@ __device__ __forceinline__ void put(T* out, long at, float y, int gelu) {
 
 constexpr int waves_of(int split) { return split > 4 ? split : 4; }
 
-// Up to 16 rows of bf16 or 4 of fp32.  A wave has NT tiles of 16 rows of W, and of their tiles of 128 columns every SPLIT-th; the SPLIT waves' sums meet in shared
+// Up to 16 rows of bf16 or 4 of fp32 (blockIdx.y of them).  A wave has NT tiles of 16 rows of W, and of their tiles of 128 columns every SPLIT-th; the SPLIT waves' sums meet in shared
 // memory.
 template <typename T, int GROUP, bool SHORT, int NT, int SPLIT>
 __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(const T* __restrict__ x, long x_row, const unsigned char* __restrict__ w, const float* __restrict__ bias,
