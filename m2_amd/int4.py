@@ -103,7 +103,7 @@ class Int4Linear(nn.Module):
         if x.dtype == torch.float32 and not _fp32_path(x):
             x = x.to(torch.bfloat16)
         buffers = self._buffers      # (nn.Module's own look-up takes 0.35 us for each)
-        bias = buffers["bias"]
+        bias = buffers["bias"] if "bias" in buffers else self.bias
         if bias is not None and bias.dtype != torch.float32:
             bias = bias.float()
         return ops.int4_linear(x, buffers["weight"], self.out_features, self.group_size, bias, activation)

@@ -71,6 +71,16 @@ def test_parts_of_long_rows(gpu, dtype, M, N, K):
     check(m2_amd.Int4Linear.from_packed(packed, scales, K, 64)(x), x, w, scales, 64)
 
 
+@pytest.mark.parametrize("M,N,K", [(100, 1200, 3403), (512, 1200, 5003), (256, 4000, 3003), (512, 4096, 1792), (300, 30_522, 400), (64, 8192, 4096)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_parts_of_large_products(gpu, dtype, M, N, K):
+    import m2_amd
+    for group in (32, 128):
+        _, scales, packed, w = weights(gpu, N, K, group)
+        x, bias = rows(gpu, M, K, dtype=dtype), rows(gpu, N, dtype=torch.float32)
+        check(m2_amd.Int4Linear.from_packed(packed, scales, K, group, bias)(x, activation="gelu"), x, w, scales, group, bias, "gelu")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("M,N", [(1, 70), (6, 70), (40, 70), (200, 70), (300, 51001)])
 def test_rows_any_distance_apart(gpu, dtype, M, N):

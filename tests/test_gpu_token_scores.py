@@ -445,6 +445,39 @@ def test_views_of_negatives(gpu):
         assert torch.equal(ins[0], ins[1])
 
 
+def test_graph_is_kept_and_let_go(gpu):
+    """A second backward pass where the graph is kept is the first; where it is not, and where what is saved has changed, it is refused."""
+    import m2_amd
+    x, t = _logits(gpu, (4, 600), torch.float32), _tokens(gpu, (4,), 600)
+    g = _grads(gpu, (4,), 3)
+
+    def call():
+        v = x.clone().requires_grad_()
+        return v, m2_amd.token_logprobs(v, t, 3)
+
+    v, r = call()
+    outs = [r.logprobs, r.entropy, r.top_logprobs]
+    assert not r.top_ids.requires_grad and all(o.requires_grad and not o.is_leaf for o in outs)
+    first = torch.autograd.grad(outs, [v], g, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(outs, [v], g)[0], first)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(outs, [v], g)
+    for change in ("logits", "entropy", "ids", "tokens"):
+        v, r = call()
+        with torch.no_grad():
+            {"logits": v, "entropy": r.entropy, "ids": r.top_ids, "tokens": t}[change].add_(0)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad([r.logprobs], [v], g[:1])
+    seen = []
+    v, r = call()
+    r.entropy.register_hook(lambda h: seen.append(h) or 2 * h)
+    r.logprobs.retain_grad()
+    (r.entropy.sum() + (r.logprobs * g[0]).sum()).backward()
+    a, b = call()
+    assert len(seen) == 1 and torch.equal(r.logprobs.grad, g[0])
+    assert torch.equal(v.grad, torch.autograd.grad([b.logprobs, b.entropy], [a], [g[0], torch.full((4,), 2.0, device=gpu)])[0])
+
+
 def test_recomputed_in_the_backward_pass(gpu):
     """Under activation checkpointing, whose hooks hand the saved tensors out again."""
     import m2_amd
