@@ -10,7 +10,7 @@
 //   16 x 768 -> 30528       7.2 (2.6)              128 x 768 -> 30528          11.9 + 4.2 (4.7)
 //   16 x 1001 -> 30522      9.2 (3.3)              512 x 768 -> 30528          33.4 + 4.5 (18.9)
 //   13 x 1536 -> 30522      8.0 (4.7)              4096 x 1792 -> 1792         34.9 + 9.5 (20.7)
-//   1 x 7168 -> 16384       11.8 (11.4)            40 x 768 -> 30522, fp32     11.7 + 4.2 (3.5)
+//   1 x 7168 -> 16384       11.8 (11.4)            40 x 768 -> 30522, fp32     10.0 + 4.2 (3.5)
 //   16 x 7168 -> 16384      13.7 (11.6)            512 x 768 -> 30528, fp32    51.4 + 4.9 (37.8: two products of half-precision parts)
 //   3 x 960 -> 960, fp32    3.6 (0.1)              8 x 5672 -> 1200, fp32      7.9 (0.7)
 //   64 x 4096 -> 2000       8.3 (1.0)              512 x 7168 -> 1792          23.5 + 8.3 (10.4)
@@ -665,6 +665,8 @@ extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
 // fp32 (rows 4 1 2 / many 1 1 4 / 2 1 4 / 2 2 2):
 //   5672 -> 1200 M = 8 32 / 8.2 / 9.4 / 12.4 / 26.6; M = 64 36 / 28 / 21 / 25 / 27.8 / 22.4 / 27.1; M = 256 40 / - / - / 64 / 59 / 39 / 32.1 / 41
 //   4096 -> 8192 M = 32 26.6 / 56 / 37 / 34 / 23.2 / 18.3 / 20.9; M = 64 29 / - / - / - / 46 / 29.3 / 23.6 / 29.7; M = 128 38 / - / - / - / 88 / 50 / 39.5 / 33.9
+// many 2 2 1 / 2 2 2 / 3 2 2 / 4 2 2, groups of 32: 768 -> 30522 M = 32 12.9 / 12.9 / 14.0 / 15.0, M = 48 16.4 / 19.1 / 14.8 / 15.7, M = 64 17.0 / 19.6 / 22.2 / 16.5, 1536 -> 16000 M = 96
+// 26.0 / 26.5 / 20.1 / 22.6, M = 128 25.5 / 28.2 / 31.6 / 23.5.
 // Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 10.8 /
 // 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 37; 1792 -> 4096 M = 256 12.9 / 14.6; fp32 1792 -> 1792 M = 64 10.5 / 11.4, 4096 -> 2000 M = 64 21.4 / 17.5, 768 -> 30522 M = 16
 // 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 56.  Its workgroups have 4 NT tiles, and 8 NT where as much of the chip is used: 768 -> 30528 M = 256 19.7 / 19.1, 1792 -> 16000 M = 512 36.4 /
@@ -696,7 +698,8 @@ static Plan plan_of(int M, int N, int K, int dtype) {
     if (products >= 4e8) {
       if (blocks(16, 4) <= round) return {Plan::kMany, 1, 1, 4};
       if (blocks(32, 4) <= round) return {Plan::kMany, 2, 1, 4};
-      if (blocks(32, 8) <= round) return {Plan::kMany, 2, 2, 2};
+      for (int mt = 2; mt <= 4; ++mt)
+        if (blocks(16 * mt, 8) <= round) return {Plan::kMany, mt, 2, 2};
       if (blocks(64, 16) >= round) return {Plan::kMany, 4, 2, 1, 8};
       return {Plan::kMany, 2, 2, 1};
     }
@@ -789,7 +792,10 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
       if constexpr (!kF32) return rows(int4_rows_kernel<T, G, false, kMt, 1, 4>, t, kMt, 1, 4);
     }
     constexpr int kMt = kF32 ? 2 : 4;
-    if (p.nt == 2 && p.split == 2) return many(int4_many_rows_kernel<T, G, kMt, 2, 2, 4>, t, kMt, 2, 2, 4);
+    if (p.nt == 2 && p.split == 2) {
+      if (p.mt == 4) return many(int4_many_rows_kernel<T, G, 4, 2, 2, 4>, t, 4, 2, 2, 4);
+      if constexpr (kF32) return p.mt == 3 ? many(int4_many_rows_kernel<T, G, 3, 2, 2, 4>, t, 3, 2, 2, 4) : many(int4_many_rows_kernel<T, G, 2, 2, 2, 4>, t, 2, 2, 2, 4);
+    }
     if (p.nt == 2 && p.waves == 8) return many(int4_many_rows_kernel<T, G, 4, 2, 1, 8>, t, 4, 2, 1, 8);
     if constexpr (kF32) {
       if (p.nt == 2) return many(int4_many_rows_kernel<T, G, 2, 2, 1, 4>, t, 2, 2, 1, 4);

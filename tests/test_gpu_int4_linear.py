@@ -71,7 +71,7 @@ def test_parts_of_long_rows(gpu, dtype, M, N, K):
     check(m2_amd.Int4Linear.from_packed(packed, scales, K, 64)(x), x, w, scales, 64)
 
 
-@pytest.mark.parametrize("M,N,K", [(100, 1200, 3403), (512, 1200, 5003), (256, 4000, 3003), (512, 4096, 1792), (300, 30_522, 400), (64, 8192, 4096)])
+@pytest.mark.parametrize("M,N,K", [(100, 1200, 3403), (512, 1200, 5003), (256, 4000, 3003), (512, 4096, 1792), (300, 30_522, 400), (64, 8192, 4096), (40, 30_522, 500), (64, 30_522, 300), (90, 16_000, 800), (128, 16_000, 400), (128, 30_522, 400)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_parts_of_large_products(gpu, dtype, M, N, K):
     import m2_amd
