@@ -208,6 +208,23 @@ def test_one_token_has_nearly_all(gpu, rows, V):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V", [(1, 30522), (30, 30522), (700, 4003), (3000, 900), (2, 262147), (5, 17)])
+def test_entropy_where_one_token_has_nearly_all(gpu, dtype, rows, V):
+    """To its own last bits.  Each e^d is off by the rounding of d log2 e below 2^5, 2^-20 ln 2, by that constant's, 2^-26 of it, and by an ulp: 20 U in all; three sums of positive numbers
+    in five steps each, U each; what stands beside a 1 loses four times U of that 1 and is mended where the rest is below 1 / 16, so up to 64 U of it."""
+    import m2_amd
+    x = _logits(gpu, (rows, V), torch.float32, scale=1.0) - 6
+    at = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(V)).to(gpu)
+    if rows > 4:
+        at[:3] = torch.tensor([0, V - 1, V - 2])
+    x = x.scatter(1, at[:, None], torch.linspace(6, 14, rows, device=gpu)[:, None]).to(dtype)
+    _, h, _, _, _ = definition(x, at.cpu(), 1, None)
+    for top in (0, 3):
+        r = m2_amd.token_logprobs(x, at, top)
+        close(r.entropy, h, U * (20 + 15 + 64) * h)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V,levels", [(4096, 1), (4096, 2), (30522, 3), (30522, 40), (70001, 1)])
 def test_ties_go_to_the_lowest_id(gpu, dtype, V, levels):
     g = torch.Generator().manual_seed(V + levels)
