@@ -88,7 +88,7 @@ Tensor int4_linear(const Tensor& x, const Tensor& weight, int64_t N, int64_t gro
   const int type = type_of("x", x);
   TORCH_CHECK_VALUE(x.dim() > 0, "x: expected (..., K), got a single value");
   const int64_t K = x.size(-1);
-  TORCH_CHECK_VALUE(N > 0 && N < INT_MAX && K > 0 && K < INT_MAX, "x ", x.sizes(), " and N = ", N, ": sizes must be positive and below 2^31");
+  TORCH_CHECK_VALUE(N > 0 && N <= 1 << 30 && K > 0 && K <= 1 << 30, "x ", x.sizes(), " and N = ", N, ": sizes must be positive and at most 2^30");
   const auto bytes = static_cast<int64_t>(int4_weight_bytes(static_cast<int>(N), static_cast<int>(K), static_cast<int>(group)));
   TORCH_CHECK(weight.device() == x.device() && (!bias || bias->device() == x.device()), "weight and bias must live on x's device, ", x.device());
   TORCH_CHECK_VALUE(bytes > 0 && weight.scalar_type() == at::kByte && weight.is_contiguous() && weight.numel() == bytes, "weight: expected ", bytes, " bytes for (", N, ", ", K,

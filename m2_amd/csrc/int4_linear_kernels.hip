@@ -32,6 +32,7 @@
 namespace m2 {
 
 constexpr int kTileK = 128, kTileN = 16;
+constexpr int kMaxSize = 1 << 30;      // of N and K: what a workgroup's last tiles count to behind them stays below 2^31
 
 constexpr int tile_bytes(int group) { return 64 * 16 + kTileN * (kTileK / group) * 2; }
 
@@ -730,6 +731,7 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
   if (!x || !weight || !out) return set_error(M2_ERR_ARG, "%s: null pointer", who);
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype must be M2_DTYPE_F32 or M2_DTYPE_BF16 (got %d)", who, dtype);
   if (M <= 0 || N <= 0 || K <= 0 || x_row < 0 || (gelu != 0 && gelu != 1)) return set_error(M2_ERR_ARG, "%s: M=%d N=%d K=%d x_row=%ld gelu=%d", who, M, N, K, x_row, gelu);
+  if (N > kMaxSize || K > kMaxSize) return set_error(M2_ERR_UNSUPPORTED, "%s: N and K of at most 2^30 (N=%d K=%d)", who, N, K);
   if (group != 32 && group != 64 && group != 128) return set_error(M2_ERR_UNSUPPORTED, "%s: groups of 32, 64 or 128 values (got %d)", who, group);
   if (!aligned16(weight, workspace)) return set_error(M2_ERR_UNSUPPORTED, "%s: weight and workspace must be 16-byte aligned", who);
   if (!workspace && m2_int4_workspace_bytes(M, N, K, dtype)) return set_error(M2_ERR_ARG, "%s: M=%d rows need a workspace", who, M);

@@ -14,6 +14,7 @@ from . import ops
 from .blockdiag import _fp32_path
 
 GROUPS = (32, 64, 128)
+MAX_SIZE = 2 ** 30
 
 
 def quantize_int4(weight: torch.Tensor, group_size: int = 64) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -45,8 +46,8 @@ class Int4Linear(nn.Module):
         super().__init__()
         if group_size not in GROUPS:
             raise ValueError(f"group_size must be one of {GROUPS}, got {group_size}")
-        if in_features <= 0 or out_features <= 0:
-            raise ValueError(f"in_features and out_features must be positive, got {in_features}, {out_features}")
+        if not (0 < in_features <= MAX_SIZE and 0 < out_features <= MAX_SIZE):
+            raise ValueError(f"in_features and out_features must be positive and at most 2^30, got {in_features}, {out_features}")
         self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
         nbytes = ops.int4_weight_bytes(out_features, in_features, group_size)
         weight = torch.zeros(nbytes, dtype=torch.uint8, device=device)      # scales 0: W = 0
