@@ -109,11 +109,26 @@ Tensor int4_linear(const Tensor& x, const Tensor& weight, int64_t N, int64_t gro
   return out;
 }
 
+// Which tokens a row may use, as the kernels read it: V bytes for all rows (row 0), or rows `row` bytes apart.
+struct Allowed {
+  Tensor t;
+  int64_t row = 0;
+};
+Allowed allowed_of(const Tensor& t, int64_t V) {
+  if (t.dim() == 1) return {t.contiguous(), 0};      // one list (or the only row's)
+  Rows r = rows_of(t, 1);
+  // rows that overlap (one list expanded to all) are one list where there is nothing else
+  if (r.row == 0 && r.inner > 1) return {std::move(r.t), 0};
+  if (r.inner == 1 || r.row >= V) return {std::move(r.t), std::max(V, r.row)};
+  return {t.contiguous(), V};
+}
+
 // What both directions take of the arguments.
 struct Scores {
   int type;
-  int64_t V, rows, top_k, ignore_index, allowed_row = 0;
-  Tensor tokens, allowed;
+  int64_t V, rows, top_k, ignore_index;
+  Tensor tokens;
+  Allowed allowed;
 };
 Scores arguments(const Tensor& logits, const optional<Tensor>& tokens, int64_t top_k, const optional<Tensor>& allowed, int64_t ignore_index) {
   Scores s;
@@ -135,15 +150,7 @@ Scores arguments(const Tensor& logits, const optional<Tensor>& tokens, int64_t t
     const bool one = allowed->dim() == 1 && allowed->size(0) == s.V;
     TORCH_CHECK_VALUE(allowed->scalar_type() == at::kBool && (one || allowed->sizes() == logits.sizes()) && allowed->device() == logits.device(), "allowed: expected bool (",
                       s.V, ") or ", logits.sizes(), " on ", logits.device(), ", got ", allowed->scalar_type(), " ", allowed->sizes(), " on ", allowed->device());
-    if (one) {
-      s.allowed = allowed->contiguous();
-    } else {
-      const Rows r = rows_of(*allowed, 1);
-      // rows that overlap (one list expanded to all) are one list where there is nothing else
-      const bool shared = r.row == 0 && r.inner > 1;
-      s.allowed = shared || r.row >= s.V || r.inner == 1 ? r.t : allowed->contiguous();
-      s.allowed_row = shared ? 0 : std::max(s.V, s.allowed.is_same(r.t) ? r.row : s.V);
-    }
+    s.allowed = allowed_of(*allowed, s.V);
   }
   return s;
 }
@@ -170,11 +177,14 @@ Found scores(const Tensor& logits, const Scores& s) {
   const auto bytes = static_cast<int64_t>(token_scores_workspace_bytes(s.rows, static_cast<int>(s.V), s.type));
   const Tensor workspace = bytes ? at::empty({bytes}, f32.dtype(at::kByte)) : Tensor();
   check(token_scores_fwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(s.tokens)), s.ignore_index,
-                         static_cast<const unsigned char*>(pointer(s.allowed)), s.allowed_row, static_cast<float*>(pointer(f.logprobs)), f.entropy.data_ptr<float>(),
+                         static_cast<const unsigned char*>(pointer(s.allowed.t)), s.allowed.row, static_cast<float*>(pointer(f.logprobs)), f.entropy.data_ptr<float>(),
                          f.stats.data_ptr<float>(), static_cast<long long*>(pointer(f.ids)), static_cast<float*>(pointer(f.top)), pointer(workspace), s.rows,
                          static_cast<int>(s.V), static_cast<int>(s.top_k), s.type, current_stream()));
   return f;
 }
+
+// The values one behind the other.
+Tensor dense(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
 
 // A gradient of one value a row: it may be one value for all of them.
 Tensor per_row(const Tensor& g) { return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).reshape({-1}) : g; }
@@ -185,7 +195,8 @@ using torch::autograd::variable_list;
 // The graph's node.  Its inputs are the gradients of entropy, log probabilities and alternatives' log probabilities, undefined where there is none.
 struct TokenLogprobsBackward : torch::autograd::Node {
   SavedVariable logits_, tokens_, allowed_, entropy_, stats_, ids_;
-  int64_t top_k = 0, ignore_index = 0, allowed_row = 0;
+  int type = 0;
+  int64_t V = 0, rows = 0, top_k = 0, ignore_index = 0;
   bool released = false;
 
   std::string name() const override { return "TokenLogprobsBackward"; }
@@ -199,23 +210,36 @@ struct TokenLogprobsBackward : torch::autograd::Node {
   variable_list apply(variable_list&& g) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     TORCH_CHECK(!released, torch::autograd::ERR_BACKWARD_TWICE);
-    const Tensor logits = logits_.unpack(), tokens = tokens_.unpack(), allowed = allowed_.unpack(), entropy = entropy_.unpack(shared_from_this()), stats = stats_.unpack(),
-                 ids = ids_.unpack();
+    // Hooks on saved tensors (torch.autograd.graph.saved_tensors_hooks) may hand out others than were saved, of another layout or anything at all.
+    const Tensor logits = logits_.unpack();
+    TORCH_CHECK(logits.defined() && logits.is_cuda() && logits.layout() == at::kStrided && logits.scalar_type() == (type == M2_DTYPE_F32 ? at::kFloat : at::kBFloat16) &&
+                    logits.dim() > 0 && logits.size(-1) == V && logits.numel() == rows * V, "token_logprobs: the saved logits came back as other ones");
+    const auto saved = [&](const char* name, Tensor t, at::ScalarType dtype, int64_t numel) {
+      TORCH_CHECK(!t.defined() || (t.device() == logits.device() && t.layout() == at::kStrided && t.scalar_type() == dtype && (numel < 0 || t.numel() == numel)), "token_logprobs: the saved ",
+                  name, " came back as another tensor");
+      return t;
+    };
+    const Tensor tokens = saved("tokens", tokens_.unpack(), at::kLong, rows), allowed = saved("allowed tokens", allowed_.unpack(), at::kBool, -1),
+                 entropy = saved("entropies", entropy_.unpack(shared_from_this()), at::kFloat, rows), stats = saved("sums", stats_.unpack(), at::kFloat, 2 * rows),
+                 ids = saved("ids", ids_.unpack(), at::kLong, rows * top_k);
+    TORCH_CHECK(!allowed.defined() || (allowed.dim() > 0 && allowed.size(-1) == V && (allowed.dim() == 1 || allowed.numel() == rows * V)),
+                "token_logprobs: the saved allowed tokens came back as another tensor");
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return variable_list(1);
     Tensor grad;
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(logits.device());
-      const int64_t V = logits.size(-1), rows = logits.numel() / V;
       grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
       if (rows) {
-        const Tensor g_h = per_row(g[0]), g_lp = per_row(g[1]), g_top = g[2].defined() ? (g[2].is_neg() ? g[2].resolve_neg() : g[2]).contiguous() : g[2];
+        const Tensor g_h = per_row(g[0]), g_lp = per_row(g[1]), g_top = dense(g[2]);
+        const Tensor token = dense(tokens), h = dense(entropy), sums = dense(stats), id = dense(ids);
+        const Allowed mask = allowed.defined() ? allowed_of(allowed, V) : Allowed();
         const Rows r = rows_of(logits, 2);
-        check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(tokens)), ignore_index,
-                               static_cast<const unsigned char*>(pointer(allowed)), allowed_row, entropy.data_ptr<float>(), stats.data_ptr<float>(),
-                               static_cast<const long long*>(pointer(ids)), static_cast<const float*>(pointer(g_lp)), g_lp.defined() ? g_lp.stride(0) : 0,
+        check(token_scores_bwd(r.t.data_ptr(), static_cast<int>(r.inner), r.outer, r.row, static_cast<const long long*>(pointer(token)), ignore_index,
+                               static_cast<const unsigned char*>(pointer(mask.t)), mask.row, h.data_ptr<float>(), sums.data_ptr<float>(),
+                               static_cast<const long long*>(pointer(id)), static_cast<const float*>(pointer(g_lp)), g_lp.defined() ? g_lp.stride(0) : 0,
                                static_cast<const float*>(pointer(g_h)), g_h.defined() ? g_h.stride(0) : 0, static_cast<const float*>(pointer(g_top)), grad.data_ptr(), V, rows,
-                               static_cast<int>(V), static_cast<int>(top_k), logits.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16, current_stream()));
+                               static_cast<int>(V), static_cast<int>(top_k), type, current_stream()));
       }
     }
     if (at::GradMode::is_enabled()) {      // a graph of the backward pass is made: what is asked of it later has to fail
@@ -238,11 +262,11 @@ Found scores_with_graph(const Tensor& logits, const Scores& s) {
   torch::autograd::set_history(variable_list{f.entropy, f.logprobs, f.top}, node);
   node->logits_ = SavedVariable(logits, false);
   node->tokens_ = SavedVariable(s.tokens, false);
-  node->allowed_ = SavedVariable(s.allowed, false);
+  node->allowed_ = SavedVariable(s.allowed.t, false);
   node->entropy_ = SavedVariable(f.entropy, true);
   node->stats_ = SavedVariable(f.stats, false);
   node->ids_ = SavedVariable(f.ids, false);
-  node->top_k = s.top_k, node->ignore_index = s.ignore_index, node->allowed_row = s.allowed_row;
+  node->type = s.type, node->V = s.V, node->rows = s.rows, node->top_k = s.top_k, node->ignore_index = s.ignore_index;
   return f;
 }
 
