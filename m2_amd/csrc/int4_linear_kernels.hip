@@ -41,24 +41,19 @@ __device__ __forceinline__ float gelu_erf(float v) { return 0.5f * v * (1.0f + e
 typedef uint32_t __attribute__((ext_vector_type(4), aligned(2))) u32x4_any;      // at any address of x's type
 typedef uint32_t __attribute__((ext_vector_type(2), aligned(2))) u32x2_any;
 
-// (q & mask) | bits as one instruction, which takes one scalar register and no literals: the compiler is kept from knowing the two constants.
-struct Codes {
-  uint32_t mask, bits;
-  __device__ __forceinline__ Codes(uint32_t m, uint32_t b) : mask(m), bits(b) { asm volatile("" : "+s"(mask), "+v"(bits)); }
-  __device__ __forceinline__ uint32_t operator()(uint32_t q) const { return (q & mask) | bits; }
-};
-
-// Eight codes as bf16 16 + q, exactly: 0x4180 is 16, and its last bits but three are worth 1 each.  What a row of x sums to, times 24, is taken off again.
-struct Bf16Codes : Codes {
-  __device__ __forceinline__ Bf16Codes() : Codes(0x00780078u, 0x41804180u) {}
-  __device__ __forceinline__ bf16x8 get(uint32_t q) const {
-    const Codes& c = *this;
-    return __builtin_bit_cast(bf16x8, u32x4{c(q << 3), c(q >> 1), c(q >> 5), c(q >> 9)});
-  }
-};
-__device__ __forceinline__ bf16x8 minus24() {
-  const u32x4 v = {0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};
-  return __builtin_bit_cast(bf16x8, v);
+// Eight codes as bf16 (q - 8) / 16, exactly; results are multiplied by 16 at the end.  The instruction takes the low four bits of a byte as a signed number to fp32, and q with its top bit turned
+// is q - 8; the upper halves of two are put together.  Nothing has to be taken off a sum again, so that a value on a code of zero leaves it as it was.  16 + q, whose bits are quicker to make (8
+// instructions instead of 14), less 24 times the sum of x kept 24 times a row's largest value in the sum: rows of one value 2^16 times the others, on a code of zero, were off by 2^-9.5 of the
+// result, and rows of one sign, at groups of 128, by 5e-7 of it (rms; 5e-8 this way).  That costs 16 x 768 -> 30528 6.3 -> 6.7 us, 1 x 7168 -> 16384 11.9 -> 12.5, fp32 13.6 -> 15.1.
+__device__ __forceinline__ bf16x8 codes_of(uint32_t q) {
+  // (asm: what the compiler makes of the bytes otherwise are shifts of their own)
+  uint32_t low = q ^ 0x88888888u, high;
+  asm("" : "+v"(low));
+  high = low >> 4;
+  asm("" : "+v"(high));
+  const auto value = [](uint32_t b) { return __float_as_uint(__builtin_amdgcn_cvt_off_f32_i4((int)b)); };
+  const auto pair = [&](uint32_t even, uint32_t odd) { return __builtin_amdgcn_perm(value(odd), value(even), 0x07060302u); };
+  return __builtin_bit_cast(bf16x8, u32x4{pair(low & 0xff, low >> 16 & 0xff), pair(high & 0xff, high >> 16 & 0xff), pair(low >> 8 & 0xff, low >> 24), pair(high >> 8 & 0xff, high >> 24)});
 }
 __device__ __forceinline__ floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
@@ -111,14 +106,14 @@ template <> struct Operand<float> {
     for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(v[i / 4][i % 4]);
   }
   __device__ __forceinline__ bf16x8 get(int lane) const {
-    const uint32_t second = (lane & 3) > 0 ? 0xffff0000u : 0u, third = (lane & 3) > 1 ? 0xffff0000u : 0u;
+    // part p is what x has in its first 8 (p + 1) bits and not in its first 8 p
+    const int p = lane & 3;
+    const uint32_t upto = p > 1 ? 0xffffffffu : p > 0 ? 0xffffff00u : 0xffff0000u, before = p > 1 ? 0xffffff00u : p > 0 ? 0xffff0000u : 0u;
     uint32_t f[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float x = __uint_as_float(v[i / 4][i % 4]);
-      x -= __uint_as_float(__float_as_uint(x) & second);
-      x -= __uint_as_float(__float_as_uint(x) & third);
-      f[i] = __float_as_uint(x);
+      const uint32_t x = v[i / 4][i % 4];
+      f[i] = __float_as_uint(__uint_as_float(x & upto) - __uint_as_float(x & before));
     }
     u32x4 o;
 #pragma unroll
@@ -164,6 +159,8 @@ struct Step {
   Scales<GROUP> s[NT];
   Operand<T> x[4];
   // `w`: the first tile's part, the others' `apart` bytes behind one another; those from `tiles` on are the last one again
+  // and `EDGE`: whether this may be the end of a row
+  template <bool EDGE>
   __device__ __forceinline__ void load(const unsigned char* w, long apart, int tiles, const T* row, int b, int K, int lane) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -172,7 +169,7 @@ struct Step {
       s[t].load(p, lane);
     }
     const int k = b * kTileK + (lane >> 4) * 8;
-    if ((b + 1) * kTileK <= K) {
+    if (!EDGE || (b + 1) * kTileK <= K) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i].load(row + k + i * 32);
     } else {
@@ -180,22 +177,18 @@ struct Step {
       for (int i = 0; i < 4; ++i) load_edge<T, SHORT>(x[i], row, k + i * 32, K);
     }
   }
-  __device__ __forceinline__ void add(floatx4 (&sum)[NT], const Bf16Codes& codes, int lane) const {
+  __device__ __forceinline__ void add(floatx4 (&sum)[NT], int lane) const {
     constexpr int kSteps = GROUP / 32;
 #pragma unroll
     for (int g = 0; g < kTileK / GROUP; ++g) {
       bf16x8 a[kSteps];
-      floatx4 c0 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        a[i] = x[g * kSteps + i].get(lane);
-        c0 = mfma(a[i], minus24(), c0);
-      }
+      for (int i = 0; i < kSteps; ++i) a[i] = x[g * kSteps + i].get(lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        floatx4 c = c0;
+        floatx4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes.get(q[t][g * kSteps + i]), c);
+        for (int i = 0; i < kSteps; ++i) c = mfma(a[i], codes_of(q[t][g * kSteps + i]), c);
         const float scale = s[t].get(g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(scale, c[i], sum[t][i]);
@@ -221,18 +214,21 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (N + kTileN - 1) / kTileN, kt = (K + kTileK - 1) / kTileK;
   const int t0 = ((int)blockIdx.x * (waves_of(SPLIT) / SPLIT) + wave / SPLIT) * NT, part = wave % SPLIT, m0 = (int)blockIdx.y * Operand<T>::kRows;
-  const Bf16Codes codes;
   floatx4 sum[NT] = {};
   if (t0 < tiles) {
     const long apart = (long)kt * tile_bytes(GROUP);
     const unsigned char* mine = w + t0 * apart;
     const T* row = x + (long)min(m0 + Operand<T>::row(lane), M - 1) * x_row;
     Step<T, GROUP, SHORT, NT> now, next;
-    if (part < kt) now.load(mine, apart, tiles - t0, row, part, K, lane);
-    for (int b = part; b < kt; b += SPLIT) {
-      if (b + SPLIT < kt) next.load(mine, apart, tiles - t0, row, b + SPLIT, K, lane);
-      now.add(sum, codes, lane);
-      now = next;
+    // from the last tile to the first, so that the end of a row is no matter of the loop
+    if (part < kt) {
+      int b = part + (kt - 1 - part) / SPLIT * SPLIT;
+      now.template load<true>(mine, apart, tiles - t0, row, b, K, lane);
+      for (; b >= 0; b -= SPLIT) {
+        if (b >= SPLIT) next.template load<false>(mine, apart, tiles - t0, row, b - SPLIT, K, lane);
+        now.add(sum, lane);
+        now = next;
+      }
     }
   }
   if (SPLIT > 1) {
@@ -255,12 +251,12 @@ __global__ __launch_bounds__(64 * waves_of(SPLIT)) void int4_few_rows_kernel(con
     const float b = bias ? bias[n] : 0.f;
     if constexpr (sizeof(T) == 4) {
       const int m = m0 + (lane >> 4);
-      if (m < M) put(out, (long)m * N + n, (sum[t][2] + sum[t][1]) + sum[t][0] + b, gelu);
+      if (m < M) put(out, (long)m * N + n, fmaf(16.f, (sum[t][2] + sum[t][1]) + sum[t][0], b), gelu);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int m = m0 + (lane >> 4) * 4 + i;
-        if (m < M) put(out, (long)m * N + n, sum[t][i] + b, gelu);
+        if (m < M) put(out, (long)m * N + n, fmaf(16.f, sum[t][i], b), gelu);
       }
     }
   }
@@ -313,7 +309,6 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_
   const unsigned char* mine[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) mine[t] = w + (long)min(t0 + t, tiles - 1) * kt * tile_bytes(GROUP);
-  const Bf16Codes codes;
   floatx4 sum[MT][NT] = {};
   Staged<T, SHORT, MT> x_now;
   u32x4 q[NT], q_next[NT];
@@ -345,25 +340,19 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_
 #pragma unroll
     for (int g = 0; g < kTileK / GROUP; ++g) {
       bf16x8 a[MT][kSteps];
-      floatx4 c0[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        c0[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          a[m][i] = Staged<T, SHORT, MT>::read(from, m, g * kSteps + i, lane);
-          c0[m] = mfma(a[m][i], minus24(), c0[m]);
-        }
-      }
+        for (int i = 0; i < kSteps; ++i) a[m][i] = Staged<T, SHORT, MT>::read(from, m, g * kSteps + i, lane);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         bf16x8 v[kSteps];
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) v[i] = codes.get(q[t][g * kSteps + i]);
+        for (int i = 0; i < kSteps; ++i) v[i] = codes_of(q[t][g * kSteps + i]);
         const float scale = s[t].get(g);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          floatx4 c = c0[m];
+          floatx4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) c = mfma(a[m][i], v[i], c);
 #pragma unroll
@@ -399,12 +388,12 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_
       }
       if constexpr (sizeof(T) == 4) {
         const int row = m0 + m * 4 + (lane >> 4);
-        if (row < M) put(out, (long)row * N + n, (sum[m][t][2] + sum[m][t][1]) + sum[m][t][0] + bn, gelu);
+        if (row < M) put(out, (long)row * N + n, fmaf(16.f, (sum[m][t][2] + sum[m][t][1]) + sum[m][t][0], bn), gelu);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = m0 + m * 16 + (lane >> 4) * 4 + i;
-          if (row < M) put(out, (long)row * N + n, sum[m][t][i] + bn, gelu);
+          if (row < M) put(out, (long)row * N + n, fmaf(16.f, sum[m][t][i], bn), gelu);
         }
       }
     }
@@ -479,6 +468,13 @@ __global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__
     write(c, o);
   }
 }
+
+// (q & mask) | bits as one instruction, which takes one scalar register and no literals: the compiler is kept from knowing the two constants.
+struct Codes {
+  uint32_t mask, bits;
+  __device__ __forceinline__ Codes(uint32_t m, uint32_t b) : mask(m), bits(b) { asm volatile("" : "+s"(mask), "+v"(bits)); }
+  __device__ __forceinline__ uint32_t operator()(uint32_t q) const { return (q & mask) | bits; }
+};
 
 // Eight codes times a scale as (16 + q) s - 24 s, exactly: 0x4c00 is 16 and its bits from the seventh are worth 1, and 24 s has ten bits.
 struct ScaledCodes : Codes {
