@@ -382,6 +382,7 @@ int m2_encoder_layers_taps_fwd(const m2_layer_params* layers, int nlayers, const
  * 16 * (j % 2) + 4 * (j / 2); then 16 rows times 128 / group scales.  Rows and columns beyond N and K hold q = 8 and s = 0.  Behind all tiles 16
  * fp32 factors for each 16 rows: the power of two that takes the row's largest scale to [1 / 2, 1) (1 where that is 0 or not finite).
  * `workspace`: m2_int4_workspace_bytes, 16-byte aligned (0: NULL does).  N and K are at most 2^30.
+ * Results below 2^-122 may be multiples of 2^-145.
  * x: M rows of K values, `x_row` values apart, fp32 or bf16; y of the same type, dense; bias (N) fp32 or NULL; gelu: 0 none, 1 erf-GELU. */
 size_t m2_int4_weight_bytes(int N, int K, int group);
 size_t m2_int4_workspace_bytes(int M, int N, int K, int dtype);

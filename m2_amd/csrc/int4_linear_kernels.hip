@@ -401,10 +401,10 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_
 }
 
 // Many rows.  Products of 16-bit floats are exact where x is: q - 8 has three bits and a scale eight, so (q - 8) s is a half-precision number of 11, and W needs
-// no sums of its own for the scales.  What half precision lacks is range: rows of W come with a power of two that takes their largest scale below 1 (behind the
-// tiles of `weight`), rows of x are taken to 2^14 .. 2^15 by one of their own, and the result is multiplied with both.  Values 2^-29 of their row's largest lose bits;
+// no sums of its own for the scales.  What half precision lacks is range: rows of W come with a power of two that takes their largest scale below 2^11 (behind the
+// tiles of `weight`, scale_factor), rows of x are taken to 2^14 .. 2^15 by one of their own, and the result is multiplied with both.  Values 2^-29 of their row's largest lose bits;
 // fp32 rows are two parts of 11 bits.  Scales below
-// 2^-17 of their row's largest lose bits, below 2^-24 of the largest product.
+// 2^-27 of their row's largest lose bits (2^-36 of that at most).
 //
 // int4_operand_kernel writes x in that form once, in the order the matrix instructions take it in: 1024 bytes (Operand) for 16 rows, 32 columns and a part.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -488,6 +488,10 @@ struct ScaledCodes : Codes {
 };
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// What a row's scales are multiplied with: its factor takes the largest to [1 / 2, 1), 2^11 more to [2^10, 2^11), as high as 24 times a scale goes, so that those 2^-27 of it are exact too.
+// (The factor ends at 2^-120, where scales may be 2^8 yet, and 2^120.)
+__device__ __forceinline__ float scale_factor(float f) { return f > 0x1p-120f ? fminf(f, 0x1p116f) * 0x1p11f : f * 4.f; }
+
 // A workgroup has MT times 16 rows of x and WAVES NT tiles of W's rows, NT a wave, SPLIT times: every SPLIT-th tile of 128 columns, with sums that meet at
 // the end.  x comes straight into shared memory, a tile of 128 columns ahead; W is made in registers, once for MT products.
 template <typename T, int GROUP, int MT, int NT, int SPLIT, int WAVES>
@@ -508,7 +512,7 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
   for (int t = 0; t < NT; ++t) {
     const int tile = min(t0 + t, tiles - 1);
     mine[t] = w + (long)tile * kt * tile_bytes(GROUP);
-    row_factor[t] = reinterpret_cast<const float*>(w + (long)tiles * kt * tile_bytes(GROUP))[tile * 16 + (lane & 15)];
+    row_factor[t] = scale_factor(reinterpret_cast<const float*>(w + (long)tiles * kt * tile_bytes(GROUP))[tile * 16 + (lane & 15)]);
   }
   // what the end needs is asked for now
   if (threadIdx.x < MT * 16) exponents[threadIdx.x] = exponent[min(m0 * 16 + (int)threadIdx.x, M - 1)];

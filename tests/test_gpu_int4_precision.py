@@ -71,3 +71,27 @@ def test_errors_are_those_of_sums(gpu, group, M, N, K, kind):
     err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
     n = K if many(M, N, K, torch.float32) else min(group, K)
     assert err <= 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)), err
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(3, 2000, 512), (20, 40000, 512), (200, 40000, 512), (64, 16000, 1500), (512, 3000, 1000)])
+def test_scales_far_below_their_rows_largest(gpu, dtype, group, M, N, K):
+    """Rows that have nothing where scales are large get what the small scales give, to the errors of their sums and the result's rounding.  bf16 scales of 8 bits have
+    them all in half precision down to 2^-27 of the largest (half a unit of its last place is 2^-25 where that is 2^10, and their last bit 2^-8 of them).
+    Where rows are few a result is 16 times a sum that is kept in steps of 2^-149: each of the additions of groups and parts is off by up to 2^-150 more, times 16 2^-146.  That shows below 2^-122."""
+    for power, offset in ((20, 0), (26, 0), (26, 100), (22, -110), (20, 125)):
+        codes, scales = weights(gpu, N, K, group)
+        s = scales.float() / 0.021 * 2.0 ** offset
+        s[:, 0] = 2.0 ** offset
+        s[:, 1:] = s[:, 1:] * 2.0 ** (1 - power) + 2.0 ** (offset - power)
+        scales = s.to(torch.bfloat16)
+        lin, w = make(gpu, codes, scales, group)
+        x = rows(gpu, M, K, dtype)
+        x[:, :group] = 0
+        y = x.double() @ w.t()
+        err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
+        n = K if many(M, N, K, dtype) else min(group, K)
+        tol = 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)) + (torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0)
+        tol += 2.0 ** -146 * (math.ceil(K / group) + 8) / y.pow(2).mean().sqrt()
+        assert err <= tol, (power, offset, err)
