@@ -402,9 +402,10 @@ __global__ __launch_bounds__(256 * SPLIT, SPLIT > 2 ? SPLIT : 2) void int4_rows_
 
 // Many rows.  Products of 16-bit floats are exact where x is: q - 8 has three bits and a scale eight, so (q - 8) s is a half-precision number of 11, and W needs
 // no sums of its own for the scales.  What half precision lacks is range: rows of W come with a power of two that takes their largest scale below 2^11 (behind the
-// tiles of `weight`, scale_factor), rows of x are taken to 2^14 .. 2^15 by one of their own, and the result is multiplied with both.  Values 2^-29 of their row's largest lose bits;
-// fp32 rows are two parts of 11 bits.  Scales below
-// 2^-27 of their row's largest lose bits (2^-36 of that at most).
+// tiles of `weight`, scale_factor), rows of x are taken to 2^14 .. 2^15 by one of their own, and the result is multiplied with both.  bf16 values below 2^-31 of their row's largest lose bits
+// (2^-39 of that at most).  fp32 rows are two parts: x rounded to 11 bits, and 2^11 times what is left, with sums of its own, rounded to 11 bits too, so that a value is off by 2^-23 of itself at most, and
+// those below 2^-27 of their row's largest by 2^-50 of that.  (With both in one sum, the second part lost bits from 2^-17 of the largest on: rows with one value 2^24 times the others, on a code of
+// zero, were off by 2^-15.8 of the result, now 2^-22.)  Scales below 2^-27 of their row's largest lose bits (2^-36 of that at most).
 //
 // int4_operand_kernel writes x in that form once, in the order the matrix instructions take it in: 1024 bytes (Operand) for 16 rows, 32 columns and a part.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(256) void int4_operand_kernel(const T* __restrict__
     for (int i = 0; i < 8; ++i) {
       const float f = ldexpf(v[i], e);
       part[0][i] = (_Float16)f;
-      if constexpr (kParts == 2) part[1][i] = (_Float16)(f - (float)part[0][i]);
+      if constexpr (kParts == 2) part[1][i] = (_Float16)((f - (float)part[0][i]) * 0x1p11f);
     }
 #pragma unroll
     for (int p = 0; p < kParts; ++p) out[((((long)(r / 16) * kt + c / 16) * kParts + p) * 4 + c / 4 % 4) * 64 + c % 4 * 16 + r % 16] = part[p];
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
   float bn[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) bn[t] = bias && n0 + t * 16 + (lane & 15) < N ? bias[n0 + t * 16 + (lane & 15)] : 0.f;
-  floatx4 sum[MT][NT] = {};
+  floatx4 sum[kParts][MT][NT] = {};
   u32x4 q[NT], q_next[NT];
   Scales<GROUP> s[NT], s_next[NT];
   half2v scale[NT], off[NT];
@@ -568,10 +569,18 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
 #pragma unroll
         for (int p = 0; p < kParts; ++p)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) sum[m][t] = mfma(a[p][m], v, sum[m][t]);
+          for (int m = 0; m < MT; ++m) sum[p][m][t] = mfma(a[p][m], v, sum[p][m][t]);
       }
     }
   }
+  // the parts of x together: the second is 2^11 times what it stands for
+  if constexpr (kParts == 2)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[0][m][t][i] = fmaf(sum[1][m][t][i], 0x1p-11f, sum[0][m][t][i]);
   // 16 rows at a time through shared memory, each wave by itself, so that a row's values leave together
   constexpr int kRow = NT * 16 + 4;
   __syncthreads();
@@ -581,7 +590,7 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sums[(m * NT + t) * 64 * WAVES] = sum[m][t];
+      for (int t = 0; t < NT; ++t) sums[(m * NT + t) * 64 * WAVES] = sum[0][m][t];
     __syncthreads();
   }
   float* const mine_out = reinterpret_cast<float*>(staged + (SPLIT > 1 ? SPLIT * 2 * kStage : 0)) + (threadIdx.x >> 6) * 16 * kRow;
@@ -597,9 +606,9 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const floatx4* sums = reinterpret_cast<const floatx4*>(staged) + (m * NT + t) * 64 * WAVES + threadIdx.x % (64 * WAVES);
-        sum[m][t] = sums[0];
+        sum[0][m][t] = sums[0];
 #pragma unroll
-        for (int p = 1; p < SPLIT; ++p) sum[m][t] += sums[p * 2 * kStage / 16];
+        for (int p = 1; p < SPLIT; ++p) sum[0][m][t] += sums[p * 2 * kStage / 16];
       }
     }
 #pragma unroll
@@ -608,7 +617,7 @@ __global__ __launch_bounds__(64 * WAVES * SPLIT, WAVES * SPLIT > 8 ? WAVES * SPL
       const int em = exponents[m * 16 + row];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float y = ldexpf(sum[m][t][i], em + en[t]) + bn[t];
+        float y = ldexpf(sum[0][m][t][i], em + en[t]) + bn[t];
         if (gelu) y = gelu_erf(y);
         mine_out[row * kRow + t * 16 + (lane & 15)] = y;
       }
@@ -671,7 +680,9 @@ extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
 // Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 10.8 /
 // 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 37; 1792 -> 4096 M = 256 12.9 / 14.6; fp32 1792 -> 1792 M = 64 10.5 / 11.4, 4096 -> 2000 M = 64 21.4 / 17.5, 768 -> 30522 M = 16
 // 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 56.  Its workgroups have 4 NT tiles, and 8 NT where as much of the chip is used: 768 -> 30528 M = 256 19.7 / 19.1, 1792 -> 16000 M = 512 36.4 /
-// 35.4, 7168 -> 30528 M = 150 93 / 109 (717 and 360 workgroups), 768 -> 30528 fp32 M = 512 56.8 (32 rows by 4 NT) / 51.0 (64 by 8 NT), 4096 -> 8192 fp32 M = 256 43.6 / 58, 512 75 / 67.
+// 35.4, 7168 -> 30528 M = 150 93 / 109 (717 and 360 workgroups), 4096 -> 8192 fp32 M = 256 43.6 / 58, 512 75 / 67.
+// fp32 of 64 rows by 8 NT takes 144 registers with its two sums, so that one workgroup has a compute unit; 48 rows 120, which two share: 512 rows, 64 / 48: 768 -> 30528 64.8 / 59.5 (960 and 1320
+// workgroups), 7168 -> 16384 220 / 228 (512, 704), 4096 -> 8192 70.9 / 84.8 (256, 352).
 struct Plan {
   enum Kernel { kFew, kRows, kMany } kernel;
   int mt, nt, split, waves = 4;      // waves: of kMany, times split
@@ -701,7 +712,7 @@ static Plan plan_of(int M, int N, int K, int dtype) {
       if (blocks(32, 4) <= round) return {Plan::kMany, 2, 1, 4};
       for (int mt = 2; mt <= 4; ++mt)
         if (blocks(16 * mt, 8) <= round) return {Plan::kMany, mt, 2, 2};
-      if (blocks(64, 16) >= round) return {Plan::kMany, 4, 2, 1, 8};
+      if (blocks(64, 16) >= round) return {Plan::kMany, blocks(64, 16) > 2 * round ? 3 : 4, 2, 1, 8};
       return {Plan::kMany, 2, 2, 1};
     }
     if (K >= 8 && blocks(16, 4) <= round) return {Plan::kRows, 4, 1, 2};
@@ -798,6 +809,8 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
       if (p.mt == 4) return many(int4_many_rows_kernel<T, G, 4, 2, 2, 4>, t, 4, 2, 2, 4);
       if constexpr (kF32) return p.mt == 3 ? many(int4_many_rows_kernel<T, G, 3, 2, 2, 4>, t, 3, 2, 2, 4) : many(int4_many_rows_kernel<T, G, 2, 2, 2, 4>, t, 2, 2, 2, 4);
     }
+    if constexpr (kF32)
+      if (p.nt == 2 && p.waves == 8 && p.mt == 3) return many(int4_many_rows_kernel<T, G, 3, 2, 1, 8>, t, 3, 2, 1, 8);
     if (p.nt == 2 && p.waves == 8) return many(int4_many_rows_kernel<T, G, 4, 2, 1, 8>, t, 4, 2, 1, 8);
     if constexpr (kF32) {
       if (p.nt == 2) return many(int4_many_rows_kernel<T, G, 2, 2, 1, 4>, t, 2, 2, 1, 4);

@@ -37,8 +37,9 @@ class Int4Linear(nn.Module):
     """y = act(x W^T + bias), W (out_features, in_features) as (code - 8) * scale.
 
     x fp32 or bf16 (..., in_features) on the GPU, rows any distance apart; y of the same type (bf16 for fp32 input under CUDA autocast); products are exact,
-    sums fp32, rounded once.  Large products of many rows take x as half-precision parts of its row's size: fp32 to 22 bits, and values 2^-29 of their row's
-    largest (scales 2^-17 of theirs) lose bits.  Rows of magnitudes above 2^115 may overflow inside a sum; a row
+    sums fp32, rounded once.  Large products of many rows take x as half-precision parts of its row's size: fp32
+    values are rounded to 23 bits, and what is far below its row's largest loses more (fp32 values from 2^-27 of it on, by 2^-50 of it; bf16 from 2^-31 on, by 2^-39; scales from 2^-27 of theirs
+    on, by 2^-36).  Rows of magnitudes above 2^115 may overflow inside a sum; a row
     that holds an infinity or NaN has no finite result.  Weights are constants: an input that asks for gradients is refused.  `weight` holds codes and scales in the kernel's order
     (include/m2_amd.h); make it with `from_linear`, `from_weight` or `from_packed`."""
 

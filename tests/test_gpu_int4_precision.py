@@ -95,3 +95,20 @@ def test_scales_far_below_their_rows_largest(gpu, dtype, group, M, N, K):
         tol = 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)) + (torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0)
         tol += 2.0 ** -146 * (math.ceil(K / group) + 8) / y.pow(2).mean().sqrt()
         assert err <= tol, (power, offset, err)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(3, 2000, 512), (20, 40000, 512), (200, 40000, 512), (64, 16000, 1500), (512, 3000, 1000), (130, 30522, 640), (256, 8192, 1024), (512, 8192, 700), (512, 30522, 400)])
+def test_fp32_values_far_below_their_rows_largest(gpu, group, M, N, K):
+    """A few large values on codes of zero.  In half precision the others are off by 2 U of themselves where they are 2^-27 of the largest or more (the root mean square of that is
+    the 1 that is added), smaller ones by 2^-50 of it: 2^-26 at most here, beside rows of size 1."""
+    for power in (12, 18, 22, 24):
+        codes, scales = weights(gpu, N, K, group)
+        codes[:, [0, K // 2, K - 1]] = 8
+        lin, w = make(gpu, codes, scales, group)
+        x = rows(gpu, M, K)
+        x[:, [0, K // 2, K - 1]] = 2.0 ** power
+        y = x.double() @ w.t()
+        err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
+        n = K if many(M, N, K, torch.float32) else min(group, K)
+        assert err <= 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)), (power, err)
