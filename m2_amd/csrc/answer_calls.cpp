@@ -59,6 +59,9 @@ int type_of(const char* name, const Tensor& t) {
   return t.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16;
 }
 
+// The values one behind the other.
+Tensor dense(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
+
 // t (..., n): row r of its leading dimensions lies (r / inner) * outer + (r % inner) * row values behind the first, in t or a copy of it: one is made where
 // a row's values lie apart, or the rows at more than `distances` (1 or 2) distances.
 struct Rows {
@@ -104,7 +107,8 @@ Tensor int4_linear(const Tensor& x, const Tensor& weight, int64_t N, int64_t gro
   const Rows r = rows_of(x, 1);
   const auto scratch = static_cast<int64_t>(int4_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), type));
   const Tensor workspace = scratch ? at::empty({scratch}, weight.options()) : Tensor();
-  check(int4_linear_fwd(r.t.data_ptr(), r.row, weight.data_ptr(), bias ? bias->data_ptr<float>() : nullptr, out.data_ptr(), pointer(workspace), static_cast<int>(M), static_cast<int>(N),
+  const Tensor offsets = bias ? dense(*bias) : Tensor();
+  check(int4_linear_fwd(r.t.data_ptr(), r.row, weight.data_ptr(), static_cast<const float*>(pointer(offsets)), out.data_ptr(), pointer(workspace), static_cast<int>(M), static_cast<int>(N),
                         static_cast<int>(K), static_cast<int>(group), gelu, type, current_stream()));
   return out;
 }
@@ -144,7 +148,7 @@ Scores arguments(const Tensor& logits, const optional<Tensor>& tokens, int64_t t
   if (tokens) {
     TORCH_CHECK_VALUE(tokens->scalar_type() == at::kLong && tokens->sizes() == lead && tokens->device() == logits.device(), "tokens: expected int64 ", lead, " on ",
                       logits.device(), ", got ", tokens->scalar_type(), " ", tokens->sizes(), " on ", tokens->device());
-    s.tokens = tokens->contiguous();
+    s.tokens = dense(*tokens);
   }
   if (allowed) {
     const bool one = allowed->dim() == 1 && allowed->size(0) == s.V;
@@ -182,9 +186,6 @@ Found scores(const Tensor& logits, const Scores& s) {
                          static_cast<int>(s.V), static_cast<int>(s.top_k), s.type, current_stream()));
   return f;
 }
-
-// The values one behind the other.
-Tensor dense(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
 
 // A gradient of one value a row: it may be one value for all of them.
 Tensor per_row(const Tensor& g) { return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).reshape({-1}) : g; }
