@@ -313,7 +313,7 @@ PyObject* py_int4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 6, "int4_linear: six arguments");
   const Tensor &x = values("x", args[0], false), &weight = tensor("weight", args[1]);
   const int64_t N = integer(args[2]), group = integer(args[3]);
-  const optional<Tensor> bias = tensor_or_none("bias", args[4]);
+  const optional<Tensor> bias = args[4] == Py_None ? std::nullopt : optional<Tensor>(values("bias", args[4], false));
   const bool gelu = args[5] == Py_True;
   Tensor y;
   {

@@ -25,3 +25,23 @@ def test_bias_and_tokens_of_negatives(gpu, dtype, M):
     a, b = (m2_amd.token_logprobs(logits, t) for t in (tokens, torch._neg_view(-tokens)))
     assert torch.equal(a.logprobs, b.logprobs)
     assert torch.equal(*(torch.autograd.grad(r.logprobs.sum(), logits)[0] for r in (a, b)))
+
+
+def test_bias_that_asks_for_gradients_is_refused(gpu):
+    """It would get none."""
+    import m2_amd
+    lin = m2_amd.Int4Linear.from_weight(torch.randn(70, 96, device=gpu), torch.randn(70, device=gpu), 32)
+    x = torch.randn(3, 96, device=gpu)
+    want = lin(x)
+    lin.bias.requires_grad_()
+    with pytest.raises(RuntimeError, match="bias: this operator has no gradient"):
+        lin(x)
+    with torch.no_grad():
+        assert torch.equal(lin(x), want)
+    bias = torch.nn.Parameter(lin.bias.detach().clone())
+    del lin.bias
+    lin.bias = bias
+    with pytest.raises(RuntimeError, match="bias: this operator has no gradient"):
+        lin(x)
+    lin.bias.requires_grad_(False)
+    assert torch.equal(lin(x), want)
