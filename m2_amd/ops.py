@@ -8,6 +8,7 @@ there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import warnings
 from typing import Optional, Sequence
 
 import torch
@@ -17,14 +18,22 @@ from ._lib import HyenaFilterParams, SplitJob, M2_DTYPE_BF16, M2_DTYPE_F32, chec
 
 try:
     from . import _answer_calls
+    # what the calls of Int4Linear and token_logprobs need of the library that _lib has loaded
+    _answer_calls.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+        "m2_last_error", "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd")])
 except ImportError as e:
-    raise ImportError(f"m2_amd/_answer_calls.so is missing or does not fit this torch ({e}): build it with `python m2_amd/build.py`") from e
+    # built against torch's internals, unlike the library with its plain C interface: without it all else runs
+    class _answer_calls:
+        _why = f"m2_amd/_answer_calls.so is missing or does not fit this torch ({e}): build it with `python m2_amd/build.py`"
+
+        @classmethod
+        def _absent(cls, *_):
+            raise RuntimeError(cls._why)
+
+        int4_linear = token_logprobs = _absent
+    warnings.warn(f"{_answer_calls._why}; until then Int4Linear and token_logprobs raise", RuntimeWarning)
 
 Tensor = torch.Tensor
-
-# what the calls of Int4Linear and token_logprobs need of the library that _lib has loaded
-_answer_calls.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
-    "m2_last_error", "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd")])
 
 
 # handle of the current stream of a device: 0.3 us, where torch.cuda.current_stream() makes an object in 3 us
