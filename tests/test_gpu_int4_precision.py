@@ -6,7 +6,6 @@ import math
 import pytest
 import torch
 
-pytestmark = pytest.mark.gpu
 U = 2.0 ** -24                                  # half a step of fp32
 SUMMED = [(1, 700, 768), (1, 8000, 1536), (3, 30522, 768), (4, 6200, 1000), (20, 4000, 768), (7, 30522, 520), (40, 2000, 768), (16, 960, 960), (16, 30522, 768), (48, 30522, 400), (64, 12000, 768), (64, 1100, 300)]
 
@@ -36,6 +35,25 @@ def many(M, N, K, dtype):
     return lib.m2_int4_workspace_bytes(M, N, K, 0 if dtype == torch.float32 else 1) > 0
 
 
+def of_sums(K, group, many):
+    """n products added one after the other, partial sums growing as a walk, are off by U sqrt(n / 6) of their result in the root mean square (roundings of
+    U / sqrt(3) of partial sums sqrt(j)); the groups' sums are added in the same way, and the result is rounded once.  A quarter is left for seeds.  In half
+    precision n is K, and a row's values, cut to two halves, are off by 2 U at most, in the root mean square below U."""
+    n = K if many else min(group, K)
+    return 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + many)
+
+
+def test_the_bound_notices_lost_bits():
+    """Rows cut to 18 bits are outside of it, also where it is widest."""
+    codes, scales = weights(None, 400, 1024, 64)
+    w = (codes - 8).double() * scales.double().repeat_interleave(64, 1)
+    x = torch.randn(20, 1024, generator=torch.Generator().manual_seed(3))
+    cut = x.view(torch.int32).bitwise_and(-64).view(torch.float32)
+    y = x.double() @ w.t()
+    assert (cut.double() @ w.t() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt() > of_sums(1024, 64, True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 128])
 @pytest.mark.parametrize("M,N,K", SUMMED)
@@ -56,23 +74,21 @@ def test_large_values_on_codes_of_zero(gpu, dtype, group, M, N, K):
         assert torch.equal(lin(x), want), power
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M,N,K", SUMMED + [(40, 30522, 768), (200, 30522, 768), (20, 40000, 512), (64, 1792, 5000), (128, 1792, 1792), (512, 3000, 1000)])
 @pytest.mark.parametrize("kind", ["normal", "one sign", "mean"])
 def test_errors_are_those_of_sums(gpu, group, M, N, K, kind):
-    """n products added one after the other, partial sums growing as a walk, are off by U sqrt(n / 6) of their result in the root mean square (roundings of
-    U / sqrt(3) of partial sums sqrt(j)); the groups' sums are added in the same way, and the result is rounded once.  A quarter is left for seeds.  In half
-    precision n is K, and a row's values, cut to two halves, are off by 2 U at most, in the root mean square below U."""
     codes, scales = weights(gpu, N, K, group)
     lin, w = make(gpu, codes, scales, group)
     x = rows(gpu, M, K)
     x = x.abs() if kind == "one sign" else x + 8 if kind == "mean" else x
     y = x.double() @ w.t()
     err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
-    n = K if many(M, N, K, torch.float32) else min(group, K)
-    assert err <= 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)), err
+    assert err <= of_sums(K, group, many(M, N, K, torch.float32)), err
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M,N,K", [(3, 2000, 512), (20, 40000, 512), (200, 40000, 512), (64, 16000, 1500), (512, 3000, 1000)])
@@ -91,12 +107,12 @@ def test_scales_far_below_their_rows_largest(gpu, dtype, group, M, N, K):
         x[:, :group] = 0
         y = x.double() @ w.t()
         err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
-        n = K if many(M, N, K, dtype) else min(group, K)
-        tol = 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)) + (torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0)
+        tol = of_sums(K, group, many(M, N, K, dtype)) + (torch.finfo(dtype).eps / 2 if dtype == torch.bfloat16 else 0)
         tol += 2.0 ** -146 * (math.ceil(K / group) + 8) / y.pow(2).mean().sqrt()
         assert err <= tol, (power, offset, err)
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("M,N,K", [(3, 2000, 512), (20, 40000, 512), (200, 40000, 512), (64, 16000, 1500), (512, 3000, 1000), (130, 30522, 640), (256, 8192, 1024), (512, 8192, 700), (512, 30522, 400)])
 def test_fp32_values_far_below_their_rows_largest(gpu, group, M, N, K):
@@ -110,5 +126,4 @@ def test_fp32_values_far_below_their_rows_largest(gpu, group, M, N, K):
         x[:, [0, K // 2, K - 1]] = 2.0 ** power
         y = x.double() @ w.t()
         err = (lin(x).double() - y).pow(2).mean().sqrt() / y.pow(2).mean().sqrt()
-        n = K if many(M, N, K, torch.float32) else min(group, K)
-        assert err <= 1.25 * U * (math.sqrt(n / 6) + math.sqrt(math.ceil(K / group) / 6) + 1 + (n == K)), (power, err)
+        assert err <= of_sums(K, group, many(M, N, K, torch.float32)), (power, err)
