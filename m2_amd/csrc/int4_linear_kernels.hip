@@ -666,23 +666,22 @@ extern "C" size_t m2_int4_weight_bytes(int N, int K, int group) {
 // Which kernel a product runs on, with how many times 16 places of rows (MT) and tiles of 16 rows of W (NT) a wave, and how many parts of K.
 //
 // What a wave takes for a tile of 128 columns is mostly waiting, so the smallest workgroups of one round over the chip win, and K is split as far as registers and
-// shared memory go.  us, as it was before (32 rows of bf16 or 16 of fp32 a workgroup, K whole) / the few rows' kernel over MT = 1, NT = 1 / 2 / 4 / rows 2 1 4 / many 4 1 4 / many
-// 4 2 2, bf16, K -> N:
-//   1792 -> 1792 M = 32 10.0 / 4.0 / 5.1 / 7.0 / 7.0; M = 128 10.2 / 9.6 / 7.0 / 7.1 / 7.3 / 12.9; M = 256 11.5 / 15.4 / 12.2 / 10.4 / 8.1 / 13.4
-//   4096 -> 2000 M = 64 20.4 / 11.3 / 8.3 / 8.8 / 12.1 / 17.9; M = 256 22.7 / 35 / 23 / 16.9 / 13.9 / 21.0; M = 512 28.7 / 68 / 43 / 32 / 26.9 / 24.3
-//   7168 -> 1792 M = 128 34.6 / 30.5 / 18.6 / 13.4 / 19.1 / 27.6; M = 512 41.7 / 101 / 57 / 46 / 37.6 / 33.6 / 45
-//   4096 -> 8192 M = 64 23 / 36 / 22 / 16.9 / 14.0 / 19.2; M = 128 27 / 67 / 40 / 31 / 26 / 21.8 / 27.6; M = 256 41 / - / - / 58 / 49 / 38 / 31.5
+// shared memory go.  us, rows 2 1 1 (32 rows of bf16 or 16 of fp32 a workgroup, K whole) / the few rows' kernel over MT = 1, NT = 1 / 2 / 4 / rows 2 1 4 / many 4 1 4 / many 4 2 2, bf16, K -> N:
+//   1792 -> 1792 M = 32 10.5 / 5.2 / 5.6 / 6.8 / 7.5; M = 128 10.6 / 10.2 / 7.5 / 6.9 / 7.7 / 13.4; M = 256 11.1 / 15.9 / 11.9 / 9.6 / 8.4 / 14.1
+//   4096 -> 2000 M = 64 19.8 / 11.7 / 8.7 / 9.9 / 12.5 / 18.8; M = 256 22.9 / 35 / 23 / 16.3 / 13.6 / 21.1; M = 512 24.3 / - / - / - / 25.2 / 24.3
+//   7168 -> 1792 M = 128 34.3 / 30.4 / 19.0 / 15.5 / 19.3 / 28.1; M = 512 38.3 / - / - / - / 39.2 / 32.7 / 43
+//   4096 -> 8192 M = 64 23 / 34 / 21.5 / 16.4 / 13.9 / 19.6; M = 128 23.8 / 69 / 38 / 28 / 25 / 21.7 / 27.3; M = 256 38.5 / - / - / 49 / 47 / 36 / 30.0
 // fp32 (rows 4 1 2 / many 1 1 4 / 2 1 4 / 2 2 2):
-//   5672 -> 1200 M = 8 32 / 8.2 / 9.4 / 12.4 / 26.6; M = 64 36 / 28 / 21 / 25 / 27.8 / 22.4 / 27.1; M = 256 40 / - / - / 64 / 59 / 39 / 32.1 / 41
-//   4096 -> 8192 M = 32 26.6 / 56 / 37 / 34 / 23.2 / 18.3 / 20.9; M = 64 29 / - / - / - / 46 / 29.3 / 23.6 / 29.7; M = 128 38 / - / - / - / 88 / 50 / 39.5 / 33.9
-// many 2 2 1 / 2 2 2 / 3 2 2 / 4 2 2, groups of 32: 768 -> 30522 M = 32 12.9 / 12.9 / 14.0 / 15.0, M = 48 16.4 / 19.1 / 14.8 / 15.7, M = 64 17.0 / 19.6 / 22.2 / 16.5, 1536 -> 16000 M = 96
-// 26.0 / 26.5 / 20.1 / 22.6, M = 128 25.5 / 28.2 / 31.6 / 23.5.
-// Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 10.8 /
-// 12.9, 128 17.0 / 16.8, 256 29.7 / 24.1, 512 49 / 37; 1792 -> 4096 M = 256 12.9 / 14.6; fp32 1792 -> 1792 M = 64 10.5 / 11.4, 4096 -> 2000 M = 64 21.4 / 17.5, 768 -> 30522 M = 16
-// 9.1 / 10.9, 40 22.2 / 15.9, 128 50 / 24, 512 164 / 56.  Its workgroups have 4 NT tiles, and 8 NT where as much of the chip is used: 768 -> 30528 M = 256 19.7 / 19.1, 1792 -> 16000 M = 512 36.4 /
-// 35.4, 7168 -> 30528 M = 150 93 / 109 (717 and 360 workgroups), 4096 -> 8192 fp32 M = 256 43.6 / 58, 512 75 / 67.
-// fp32 of 64 rows by 8 NT takes 144 registers with its two sums, so that one workgroup has a compute unit; 48 rows 120, which two share: 512 rows, 64 / 48: 768 -> 30528 64.8 / 59.5 (960 and 1320
-// workgroups), 7168 -> 16384 220 / 228 (512, 704), 4096 -> 8192 70.9 / 84.8 (256, 352).
+//   5672 -> 1200 M = 8 31 / 8.2 / 9.8 / 13.5 / 26.1; M = 64 32 / 27 / 21.4 / 28 / 26.2 / 23.3 / 26.8; M = 256 40 / - / - / 66 / 39 / 39 / 30.8 / 40
+//   4096 -> 8192 M = 32 23.9 / 52 / 35 / 36 / 20.2 / 18.7 / 20.8; M = 64 31 / - / - / - / 31 / 28.6 / 23.0 / 28.9; M = 128 54 / - / - / - / 58 / 48 / 37.0 / 32.5
+// many 2 2 1 / 2 2 2 / 3 2 2 / 4 2 2, groups of 32: 768 -> 30522 M = 40 16.0 / 18.8 / 14.3 / 15.6, M = 48 16.1 / 19.0 / 14.5 / 15.9, M = 64 16.8 / 19.6 / 22.1 / 16.9, 1536 -> 16000 M = 96
+// 23.3 / 26.7 / 20.2 / 22.7, M = 128 25.1 / 27.9 / 31.0 / 23.6.
+// Where x is written as half-precision operands first (kMany), that takes 4 us and more, which only a large product wins back.  us, rows / many: 768 -> 30528 bf16 M = 64 11.1 /
+// 12.2, 128 17.9 / 16.1, 256 29.5 / 23.5; fp32 1792 -> 1792 M = 64 10.4 / 11.7, 768 -> 30522 M = 16 9.6 / 11.9, 40 19.9 / 14.3, 128 43 / 24.7.
+// Its workgroups have 4 NT tiles, and 8 NT where as much of the chip is used: 768 -> 30528 M = 256 24.0 / 23.5, 1792 -> 16000 M = 512 41.5 / 40.8, 7168 -> 30528 M = 150 100 / 112 (717 and 360
+// workgroups); fp32, 32 rows by 4 NT / 64 by 8 NT: 4096 -> 8192 M = 256 50.6 / 61.7, 512 85.7 / 73.4, 7168 -> 16384 M = 512 258 / 224.
+// fp32 of 64 rows by 8 NT takes 144 registers with its two sums, so that one workgroup has a compute unit; 48 rows 120, which two share: 512 rows, 64 / 48: 768 -> 30528 68.0 / 61.9 (960 and 1320
+// workgroups), 7168 -> 16384 224 / 235 (512, 704), 4096 -> 8192 73.4 / 87.4 (256, 352).
 struct Plan {
   enum Kernel { kFew, kRows, kMany } kernel;
   int mt, nt, split, waves = 4;      // waves: of kMany, times split
@@ -694,13 +693,16 @@ static Plan plan_of(int M, int N, int K, int dtype) {
   const auto blocks = [&](int rows, int columns) { return (M + rows - 1L) / rows * ((tiles + columns - 1) / columns); };      // of `rows` rows and `columns` tiles
   if (places == 1) {
     // Few tiles: all of a workgroup's waves share one.  More: tiles share what a wave reads (and splits) of x, four where that is as much as a tile, and
-    // long rows are shared by eight waves, short ones by four where there are many tiles.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 2.7 / 3.3 / 3.2 / 4.2 / 3.8; 4096 -> 4096 M = 16
-    // 7.2 / 8.7 / 7.5 / 11.7 / 9.4; 1792 -> 7168 M = 16 7.2 / 6.6 / 5.6 / 7.0 / 7.0; 768 -> 30528 M = 1 6.6 / 6.1 / 6.7 / 6.8 / 6.5, M = 16 9.3 / 7.0 / 7.4 / 6.9 / 6.9;
-    // 4096 -> 16384 M = 1 10.0 / 10.3 / 9.4 / 12.4 / 9.9, M = 16 19.5 / 13.0 / 13.0 / 13.4 / 11.2; 7168 -> 16384 fp32 M = 1 24.6 / 18.6 / 17.4 / 17.5 / 14.7;
-    // groups of 32, 1792 -> 15000 M = 1 7.3 / 6.9 / 6.4 / 8.0 / 6.9, 768 -> 17000 fp32 M = 1 7.6 / 5.7 / 5.4 / 6.9 / 7.2, 1536 -> 30522 fp32 M = 4 15.2 / 11.5 / 10.9 / 10.0 / 11.1.
+    // long rows are shared by eight waves, short ones by four where there are many tiles and a wave has little more to do.  us, NT and SPLIT 1, 8 / 2, 4 / 2, 8 / 4, 4 / 4, 8: 768 -> 768 M = 1 3.5 / 3.9 / 3.7 / 4.6 / 4.3;
+    // 4096 -> 4096 M = 16 7.6 / 9.3 / 8.1 / 12.1 / 10.4; 1792 -> 7168 M = 16 6.9 / 6.3 / 5.8 / 7.6 / 6.9; 768 -> 30528 M = 1 5.9 / 5.7 / 6.3 / 6.6 / 5.9, M = 16 9.4 / 7.4 / 8.0 / 7.7 / 6.8; 1536 ->
+    // 30522 M = 16 15.6 / 11.1 / 11.5 / 10.0 / 9.3, M = 9 11.4 / 9.6 / 9.7 / 9.5 / 8.8; 4096 -> 16384 M = 1 10.2 / 11.2 / 10.3 / 12.8 / 11.1, M = 16 19.6 / 13.1 / 13.3 / 13.7 / 11.9; 1792 -> 15000
+    // M = 1 6.7 / 7.5 / 6.7 / 8.8 / 7.2; fp32 768 -> 17000 M = 1 6.4 / 5.6 / 5.6 / 6.8 / 7.0, 768 -> 30522 M = 4 9.3 / 6.6 / 7.4 / 7.3 / 7.8, 1536 -> 30522 M = 4 13.1 / 10.5 / 10.2 / 9.8 / 11.1, 7168 ->
+    // 16384 M = 1 25.3 / 22.0 / 19.0 / 22.7 / 18.2.
     if (K < 8 || tiles < 384) return {Plan::kFew, 1, 1, 8};
     const bool many = tiles >= 1536 || (kt >= 16 && tiles >= 1024);
-    return {Plan::kFew, 1, many && (f32 || M > 8) ? 4 : 2, kt < 16 && many ? 4 : 8};
+    if (!many) return {Plan::kFew, 1, 2, 8};
+    if (f32) return {Plan::kFew, 1, kt < 8 ? 2 : 4, kt < 16 ? 4 : 8};
+    return M > 8 ? Plan{Plan::kFew, 1, 4, 8} : Plan{Plan::kFew, 1, 2, kt < 16 ? 4 : 8};
   }
   if (K >= 8)
     for (int nt = 1; nt <= 4; nt *= 2)
@@ -794,7 +796,9 @@ extern "C" int m2_int4_linear_fwd(const void* x, long x_row, const void* weight,
       if (K < 8) return go(int4_few_rows_kernel<T, G, true, 1, 8>, t, 1, 8);
       if (p.nt == 1) return go(int4_few_rows_kernel<T, G, false, 1, 8>, t, 1, 8);
       if (p.nt == 2) return p.split == 4 ? go(int4_few_rows_kernel<T, G, false, 2, 4>, t, 2, 4) : go(int4_few_rows_kernel<T, G, false, 2, 8>, t, 2, 8);
-      return p.split == 4 ? go(int4_few_rows_kernel<T, G, false, 4, 4>, t, 4, 4) : go(int4_few_rows_kernel<T, G, false, 4, 8>, t, 4, 8);
+      if constexpr (kF32)
+        if (p.split == 4) return go(int4_few_rows_kernel<T, G, false, 4, 4>, t, 4, 4);
+      return go(int4_few_rows_kernel<T, G, false, 4, 8>, t, 4, 8);
     }
     if (p.kernel == Plan::kRows) {
       constexpr int kMt = kF32 ? 4 : 2;
