@@ -2,8 +2,8 @@
 //
 // Their calls are a few microseconds of GPU time for a row or a handful of them, and checks, output tensors and the call through ctypes took
 // 10 to 17 us in Python (torch's own linear: 19), a gradient 100: here the same checks raise the same errors.  us a call, one stream, back to back, Python / here:
-// Int4Linear 768 x 768 11.8 / 6.4 (the launch itself 3.0, the output tensor 0.7); token_logprobs 1 x 30522 17.0 / 7.9, 1 x 30522 fp32 with its gradient 118 / 66
-// (most of it torch's own backward pass).
+// Int4Linear 768 x 768 11.8 / 6.3 (the launch itself 3.0, the output tensor 0.7); token_logprobs 1 x 30522 17.0 / 8.5, 128 x 30522 fp32 with its gradient 118 / 35 .. 58
+// (most of it torch's own backward pass, which takes one or the other from process to process, on one machine).
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>

@@ -1,19 +1,21 @@
 // y = act(x W^T + b) for few rows x, W (N, K) in 4 bits with a bf16 scale for each group of a row: W[n, k] = (q - 8) s, q in 0 .. 15.
 //
 // Few rows are bound by the weight, N K / 2 bytes and 2 N K / group of scales: 12.5 MB and 2.4 us for the word embeddings at K = 768, beside 3 us that any launch of
-// a few dependent loads takes.  Many rows are bound by several things alike, which hardly overlap: of 33 us at M = 512 making W out of the codes takes 7, fetching x and W 7,
-// the products 12 (as copies of the kernel without one or two of these say; the matrix unit is busy 27 % of the cycles, the vector unit 42 %), and workgroups twice as wide or high, 64 x 64
-// instead of 64 x 32 to a wave, or another order of the instructions change nothing.  Kernel times, MI355X (floor: bytes at 5.3 TB/s, products at 1.27 PFLOP/s):
+// a few dependent loads takes; a wave's loads, the 14 vector instructions for eight codes and the products stand behind one another (vector unit 38 % busy at 1 x 7168 -> 16384).  Many rows are
+// bound by several things alike, which hardly overlap: of 34 us at M = 512 making W out of the codes takes 7, fetching x and W 7,
+// the products 12 (as copies of the kernel without one or two of these say; the matrix unit is busy 27 % of the cycles, the vector unit 43 %), and workgroups twice as wide or high, 64 x 64
+// instead of 64 x 32 to a wave, or another order of the instructions change nothing.  Kernel times, MI355X; beside them bytes at 5.3 TB/s or products at the 1.27 PFLOP/s that a large
+// library product reaches (matrix instructions alone: 1.9):
 //
 //   M x K -> N              us (floor)             M x K -> N                  us (floor)
-//   1 x 768 -> 30528        5.1 (2.4)              64 x 768 -> 30528           11.2 (3.1)
-//   16 x 768 -> 30528       7.2 (2.6)              128 x 768 -> 30528          11.9 + 4.2 (4.7)
-//   16 x 1001 -> 30522      9.2 (3.3)              512 x 768 -> 30528          33.4 + 4.5 (18.9)
-//   13 x 1536 -> 30522      8.0 (4.7)              4096 x 1792 -> 1792         34.9 + 9.5 (20.7)
-//   1 x 7168 -> 16384       11.8 (11.4)            40 x 768 -> 30522, fp32     10.0 + 4.2 (3.5)
-//   16 x 7168 -> 16384      13.7 (11.6)            512 x 768 -> 30528, fp32    51.4 + 4.9 (37.8: two products of half-precision parts)
-//   3 x 960 -> 960, fp32    3.6 (0.1)              8 x 5672 -> 1200, fp32      7.9 (0.7)
-//   64 x 4096 -> 2000       8.3 (1.0)              512 x 7168 -> 1792          23.5 + 8.3 (10.4)
+//   1 x 768 -> 30528        5.7 (2.4)              64 x 768 -> 30528           11.2 (3.1)
+//   16 x 768 -> 30528       6.1 (2.6)              128 x 768 -> 30528          12.3 + 4.3 (4.7)
+//   16 x 1001 -> 30522      8.6 (3.3)              512 x 768 -> 30528          34.6 + 4.4 (18.9)
+//   13 x 1536 -> 30522      8.5 (4.7)              4096 x 1792 -> 1792         36.1 + 9.4 (20.7)
+//   1 x 7168 -> 16384       12.7 (11.4)            40 x 768 -> 30522, fp32     10.6 + 4.2 (3.5)
+//   16 x 7168 -> 16384      14.5 (11.6)            512 x 768 -> 30528, fp32    60 + 5.0 (37.8: two products of half-precision parts)
+//   3 x 960 -> 960, fp32    3.5 (0.1)              8 x 5672 -> 1200, fp32      7.9 (0.7)
+//   64 x 4096 -> 2000       8.6 (1.0)              512 x 7168 -> 1792          25.2 + 8.3 (10.4)
 //
 // A product runs on one of three kernels (plan_of): up to 16 rows of bf16 or 4 of fp32 straight from memory, and more of them so where W is small; more rows with x in shared
 // memory; large products with x as half-precision operands, which a launch of its own writes (behind the +).
