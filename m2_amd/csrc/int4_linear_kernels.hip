@@ -46,7 +46,8 @@ typedef uint32_t __attribute__((ext_vector_type(2), aligned(2))) u32x2_any;
 // Eight codes as bf16 (q - 8) / 16, exactly; results are multiplied by 16 at the end.  The instruction takes the low four bits of a byte as a signed number to fp32, and q with its top bit turned
 // is q - 8; the upper halves of two are put together.  Nothing has to be taken off a sum again, so that a value on a code of zero leaves it as it was.  16 + q, whose bits are quicker to make (8
 // instructions instead of 14), less 24 times the sum of x kept 24 times a row's largest value in the sum: rows of one value 2^16 times the others, on a code of zero, were off by 2^-9.5 of the
-// result, and rows of one sign, at groups of 128, by 5e-7 of it (rms; 5e-8 this way).  That costs 16 x 768 -> 30528 6.3 -> 6.7 us, 1 x 7168 -> 16384 11.9 -> 12.5, fp32 13.6 -> 15.1.
+// result, and rows of one sign, at groups of 128, by 5e-7 of it (rms; 5e-8 this way).  That costs 13 x 1536 -> 30522 7.0 -> 7.4 us, 1 x 7168 -> 16384 11.9 -> 12.5, fp32
+// 13.6 -> 14.9.  fp32 parts below 2^-133, bf16's last place, are lost: rows below 2^-109 are off by up to 2^-131.
 __device__ __forceinline__ bf16x8 codes_of(uint32_t q) {
   // (asm: what the compiler makes of the bytes otherwise are shifts of their own)
   uint32_t low = q ^ 0x88888888u, high;

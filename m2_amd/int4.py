@@ -39,7 +39,7 @@ class Int4Linear(nn.Module):
     x fp32 or bf16 (..., in_features) on the GPU, rows any distance apart; y of the same type (bf16 for fp32 input under CUDA autocast); products are exact,
     sums fp32, rounded once.  Large products of many rows take x as half-precision parts of its row's size: fp32
     values are rounded to 23 bits, and what is far below its row's largest loses more (fp32 values from 2^-27 of it on, by 2^-50 of it; bf16 from 2^-31 on, by 2^-39; scales from 2^-27 of theirs
-    on, by 2^-36).  Rows of magnitudes above 2^115 may overflow inside a sum; a row
+    on, by 2^-36).  Rows of magnitudes above 2^115 may overflow inside a sum, fp32 values may be off by 2^-131 and results by 2^-144; a row
     that holds an infinity or NaN has no finite result.  Weights are constants: an input or bias that asks for gradients is refused.  `weight` holds codes and scales in the kernel's order
     (include/m2_amd.h); make it with `from_linear`, `from_weight` or `from_packed`.
 
