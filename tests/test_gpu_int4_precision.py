@@ -54,13 +54,11 @@ def test_the_bound_notices_lost_bits():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("group", [32, 128])
-@pytest.mark.parametrize("M,N,K", SUMMED)
+@pytest.mark.parametrize("dtype,M,N,K", [(t, *size) for t in (torch.float32, torch.bfloat16) for size in SUMMED if t == torch.bfloat16 or size not in ((48, 30522, 400), (64, 12000, 768))])
 def test_large_values_on_codes_of_zero(gpu, dtype, group, M, N, K):
-    """Such a product is exactly 0 and a sum with it what it was: not a bit of the result changes."""
-    if many(M, N, K, dtype):
-        pytest.skip("sizes of the other kernels")
+    """Such a product is exactly 0 and a sum with it what it was: not a bit of the result changes (where rows are not taken in half precision)."""
+    assert not many(M, N, K, dtype)
     codes, scales = weights(gpu, N, K, group)
     places = [0, 37, K // 2, K - 1]
     codes[:, places] = 8
