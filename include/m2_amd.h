@@ -411,6 +411,63 @@ int m2_token_scores_bwd(const void* logits, int inner, long outer_stride, long r
                         const float* g_logprobs, long g_logprobs_stride, const float* g_entropy, long g_entropy_stride, const float* g_top,
                         void* grad, long grad_row, long rows, int V, int top_k, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The parts of a causal mixer: the short convolution, the selective state space scan and group norm, on hidden states whose channels lie last, with their
+ * gradients, and the first two for one token (the reference's mixer is bidirectional: its short convolution and gates,
+ * bert/src/mm/monarch_mixer_sequence_mixer.py:100-154, and its normalisation, bert/src/bert_layers.py:478-479, are their counterparts).  dtype: of all
+ * tensors given as void*.  Tensors are dense unless a batch and row distance (in values) is given; a row's values always lie one behind the other.  `lengths`
+ * (B) on the GPU, or NULL: sequence b ends at lengths[b] (taken as 0 .. L); positions behind it are not read, outputs and gradients there are 0.
+ *
+ * m2_causal_conv_*: x, y (B, L, C); w (C, K) fp32, the last tap meets the position itself, K 1 .. 8; bias (C) fp32 or NULL; silu 0 or 1; state (B, K - 1, C), the
+ * inputs ahead of the first, oldest first, or NULL (zeros); state_out (B, K - 1, C) or NULL: the last K - 1 inputs.  The gradient takes gy and gstate_out (or
+ * NULL) and writes gx, gw (C, K) fp32, gb (C) fp32 and gstate, each unless NULL; `workspace`: m2_causal_conv_bwd_workspace_bytes.  The step: x (B, C), y (B, C);
+ * state_out may be state. */
+int m2_causal_conv_fwd(const void* x, long x_batch, long x_row, const float* w, const float* bias, const void* state, const long long* lengths, void* y,
+                       void* state_out, int B, int L, int C, int K, int silu, int dtype, void* stream);
+size_t m2_causal_conv_bwd_workspace_bytes(int B, int L, int C, int K, int dtype);
+int m2_causal_conv_bwd(const void* x, long x_batch, long x_row, const float* w, const float* bias, const void* state, const long long* lengths,
+                       const void* gy, long gy_batch, long gy_row, const void* gstate_out, void* gx, float* gw, float* gb, void* gstate, void* workspace,
+                       int B, int L, int C, int K, int silu, int dtype, void* stream);
+int m2_causal_conv_step(const void* x, long x_batch, const void* state, const float* w, const float* bias, void* y, void* state_out, int B, int C, int K,
+                        int silu, int dtype, void* stream);
+
+/* The scan:  d = dt + dt_bias, softplus of it if asked for;  h[t] = exp(d A) h[t - 1] + d B[t] x[t];  y[t] = (sum_n C[t, n] h[t, n] + D x[t]) silu(z[t]).
+ * x, dt, z (or NULL), y (batch, length, channels); B, C (batch, length, groups, states), a group serving channels / groups neighbouring channels; A
+ * (channels, states), D, dt_bias (channels) or NULL and state (batch, channels, states) or NULL (zeros) fp32; states 1 .. 256.
+ * state_out (batch, channels, states) or NULL: the states behind the last position.  `saved`, for the gradient, or NULL: fp32
+ * (batch, ceil(length / m2_selective_scan_span), channels, states).  The gradient takes gy and gstate_out (or NULL) and writes all of m2_scan_gradients that
+ * are not NULL, B and C's dense (batch, length, groups, states), of dtype, the others of their inputs' types; `workspace`: m2_selective_scan_bwd_workspace_bytes.
+ * The step takes length 1; state_out may be state. */
+typedef struct m2_scan_inputs {
+  const void *x, *dt, *z, *Bm, *Cm;
+  long x_batch, x_row, dt_batch, dt_row, z_batch, z_row, b_batch, b_row, b_group, c_batch, c_row, c_group;
+  const float *A, *D, *dt_bias, *state;
+  const long long* lengths;
+  int batch, length, channels, groups, states, softplus;
+} m2_scan_inputs;
+typedef struct m2_scan_gradients {
+  const void* gy;
+  long gy_batch, gy_row;
+  const float* gstate_out;
+  void *gx, *gdt, *gz, *gB, *gC;
+  float *gA, *gD, *gdt_bias, *gstate;
+} m2_scan_gradients;
+int m2_selective_scan_span(int states);
+int m2_selective_scan_fwd(const m2_scan_inputs* in, void* y, float* state_out, float* saved, int dtype, void* stream);
+size_t m2_selective_scan_bwd_workspace_bytes(int batch, int length, int channels, int groups, int states);
+int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gradients* out, const float* saved, void* workspace, int dtype, void* stream);
+int m2_selective_scan_step(const m2_scan_inputs* in, void* y, float* state_out, int dtype, void* stream);
+
+/* Group norm: x (N, S, C), mean and biased variance over the S positions and each of G groups of neighbouring channels, y = act((x - mean) rstd w + b); w, b
+ * (C) fp32 or NULL; act 0 none, 1 SiLU, 2 erf-GELU.  stats (N, G, 2) fp32 (mean, rstd) is written and the gradient's input.  x and gy: rows of C one behind
+ * the other, a sample N and a position S apart as given.  The gradient writes gx (dense), gw and gb (C) fp32, each unless NULL.  Workspaces:
+ * m2_group_norm_workspace_bytes (0: NULL does). */
+size_t m2_group_norm_workspace_bytes(long N, int S, int C, int G, int backward, int dtype);
+int m2_group_norm_fwd(const void* x, long x_sample, long x_row, const float* w, const float* b, float eps, void* y, float* stats, void* workspace, long N, int S,
+                      int C, int G, int act, int dtype, void* stream);
+int m2_group_norm_bwd(const void* x, long x_sample, long x_row, const float* w, const float* b, const float* stats, const void* gy, long gy_sample, long gy_row,
+                      void* gx, float* gw, float* gb, void* workspace, long N, int S, int C, int G, int act, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

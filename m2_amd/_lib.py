@@ -36,6 +36,19 @@ class SplitJob(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("x", "out", "channel_major")] + [(n, c_int) for n in ("rows", "nblocks", "p")]
 
 
+class ScanInputs(ctypes.Structure):
+    """Mirror of `m2_scan_inputs`."""
+    _fields_ = ([(n, c_void_p) for n in ("x", "dt", "z", "Bm", "Cm")]
+                + [(n, c_long) for n in ("x_batch", "x_row", "dt_batch", "dt_row", "z_batch", "z_row", "b_batch", "b_row", "b_group", "c_batch", "c_row", "c_group")]
+                + [(n, c_void_p) for n in ("A", "D", "dt_bias", "state", "lengths")] + [(n, c_int) for n in ("batch", "length", "channels", "groups", "states", "softplus")])
+
+
+class ScanGradients(ctypes.Structure):
+    """Mirror of `m2_scan_gradients`."""
+    _fields_ = ([("gy", c_void_p), ("gy_batch", c_long), ("gy_row", c_long)]
+                + [(n, c_void_p) for n in ("gstate_out", "gx", "gdt", "gz", "gB", "gC", "gA", "gD", "gdt_bias", "gstate")])
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -168,6 +181,30 @@ def _load() -> ctypes.CDLL:
     lib.m2_token_scores_bwd.restype = c_int
     lib.m2_token_scores_bwd.argtypes = ([c_void_p, c_int, c_long, c_long, c_void_p, c_longlong, c_void_p, c_long] + [c_void_p] * 4
                                         + [c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_long] + [c_int] * 3 + [c_void_p])
+    lib.m2_causal_conv_fwd.restype = c_int
+    lib.m2_causal_conv_fwd.argtypes = [c_void_p, c_long, c_long] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p]
+    lib.m2_causal_conv_bwd_workspace_bytes.restype = c_size_t
+    lib.m2_causal_conv_bwd_workspace_bytes.argtypes = [c_int] * 5
+    lib.m2_causal_conv_bwd.restype = c_int
+    lib.m2_causal_conv_bwd.argtypes = ([c_void_p, c_long, c_long] + [c_void_p] * 5 + [c_long, c_long] + [c_void_p] * 6 + [c_int] * 6 + [c_void_p])
+    lib.m2_causal_conv_step.restype = c_int
+    lib.m2_causal_conv_step.argtypes = [c_void_p, c_long] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p]
+    lib.m2_selective_scan_span.restype = c_int
+    lib.m2_selective_scan_span.argtypes = [c_int]
+    lib.m2_selective_scan_fwd.restype = c_int
+    lib.m2_selective_scan_fwd.argtypes = [POINTER(ScanInputs)] + [c_void_p] * 3 + [c_int, c_void_p]
+    lib.m2_selective_scan_bwd_workspace_bytes.restype = c_size_t
+    lib.m2_selective_scan_bwd_workspace_bytes.argtypes = [c_int] * 5
+    lib.m2_selective_scan_bwd.restype = c_int
+    lib.m2_selective_scan_bwd.argtypes = [POINTER(ScanInputs), POINTER(ScanGradients), c_void_p, c_void_p, c_int, c_void_p]
+    lib.m2_selective_scan_step.restype = c_int
+    lib.m2_selective_scan_step.argtypes = [POINTER(ScanInputs), c_void_p, c_void_p, c_int, c_void_p]
+    lib.m2_group_norm_workspace_bytes.restype = c_size_t
+    lib.m2_group_norm_workspace_bytes.argtypes = [c_long] + [c_int] * 5
+    lib.m2_group_norm_fwd.restype = c_int
+    lib.m2_group_norm_fwd.argtypes = [c_void_p, c_long, c_long, c_void_p, c_void_p, c_float] + [c_void_p] * 3 + [c_long] + [c_int] * 5 + [c_void_p]
+    lib.m2_group_norm_bwd.restype = c_int
+    lib.m2_group_norm_bwd.argtypes = ([c_void_p, c_long, c_long] + [c_void_p] * 4 + [c_long, c_long] + [c_void_p] * 4 + [c_long] + [c_int] * 5 + [c_void_p])
     return lib
 
 
@@ -178,7 +215,9 @@ EXPORTS = ["m2_version", "m2_last_error", "m2_hyena_filter_workspace_bytes", "m2
            "m2_fftconv_fwd", "m2_dense_supported", "m2_dense_to_channels_fwd", "m2_dense_to_channels_rows_fwd", "m2_dense_channels_row", "m2_dense_from_channels_fwd", "m2_layernorm_to_channels_supported", "m2_layernorm_to_channels_fwd", "m2_blockdiag_glu_fwd", "m2_blockdiag_glu_few_rows", "m2_blockdiag_linear_fwd", "m2_blockdiag_linear_f32_fwd", "m2_mlp_fused_supported", "m2_mlp_fused_packed_bytes", "m2_mlp_fused_pack", "m2_mlp_fused_fwd", "m2_glu_stream_supported", "m2_glu_stream_packed_bytes", "m2_glu_stream_pack", "m2_glu_stream_fwd", "m2_layernorm_fwd", "m2_layernorm_bf16_fwd", "m2_input_forms_fwd", "m2_pooler_fwd",
            "m2_embed_layernorm_fwd", "m2_blockdiag_linear_layernorm_supported", "m2_blockdiag_linear_layernorm_fwd", "m2_encoder_layers_workspace_bytes", "m2_encoder_layers_fwd", "m2_encoder_layers_taps_fwd",
            "m2_split_bytes", "m2_split_rows_fwd", "m2_split_jobs_fwd", "m2_split_channels_fwd", "m2_split_to_channels_fwd", "m2_split_linear_fwd", "m2_split_glu_fwd",
-           "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd"]
+           "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd",
+           "m2_causal_conv_fwd", "m2_causal_conv_bwd_workspace_bytes", "m2_causal_conv_bwd", "m2_causal_conv_step", "m2_selective_scan_span", "m2_selective_scan_fwd",
+           "m2_selective_scan_bwd_workspace_bytes", "m2_selective_scan_bwd", "m2_selective_scan_step", "m2_group_norm_workspace_bytes", "m2_group_norm_fwd", "m2_group_norm_bwd"]
 
 
 def check(rc: int) -> None:

@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libm2_amd.so")
 SOURCES = ["common.hip", "fftconv_kernels.hip", "fftconv_real_kernels.hip", "fftconv_long_kernels.hip", "mixer_taps_kernels.hip", "hyena_filter_kernels.hip", "filter_fused_kernels.hip", "blockdiag_kernels.hip", "wo_layernorm_kernels.hip",
            "mlp_fused_kernels.hip", "glu_stream_kernels.hip", "dense_kernels.hip", "dense_ws_kernels.hip", "split_gemm_kernels.hip", "layernorm_kernels.hip", "pooler_kernels.hip", "encoder_schedule.hip",
-           "int4_linear_kernels.hip", "token_scores_kernels.hip"]
+           "int4_linear_kernels.hip", "token_scores_kernels.hip", "causal_conv_kernels.hip", "selective_scan_kernels.hip", "selective_scan_bwd_kernels.hip", "group_norm_kernels.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # packed fp32 VALU instructions are switched off on purpose (device flag, the host pass warns about it)
 FLAGS = ["-std=c++17", "-O3", "--offload-arch=gfx950", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
@@ -53,8 +53,8 @@ def _build_extension(name: str, incremental: bool = False) -> str:
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     src, out = os.path.join(CSRC, name + ".cpp"), os.path.join(HERE, f"_{name}.so")
-    header = os.path.join(HERE, "..", "include", "m2_amd.h")
-    if incremental and os.path.exists(out) and max(os.path.getmtime(src), os.path.getmtime(header)) < os.path.getmtime(out):
+    headers = [os.path.join(HERE, "..", "include", "m2_amd.h"), os.path.join(CSRC, "torch_calls.h")]
+    if incremental and os.path.exists(out) and max(os.path.getmtime(f) for f in (src, *headers)) < os.path.getmtime(out):
         return out
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            *[f"-I{p}" for p in include_paths()], "-I/opt/rocm/include", f"-I{sysconfig.get_paths()['include']}", src, "-o", out,
@@ -68,7 +68,7 @@ def _build_extension(name: str, incremental: bool = False) -> str:
 def build(verbose: bool = True, incremental: bool = False) -> str:
     """Compiles every source (or, with incremental=True, only those older than their .hip / headers) and links."""
     with ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        checks = [ex.submit(_build_extension, name, incremental) for name in ("answer_calls", "param_check")]
+        checks = [ex.submit(_build_extension, name, incremental) for name in ("answer_calls", "causal_calls", "param_check")]
         objs = list(ex.map(lambda src: _compile(src, incremental), SOURCES))
         for check in checks:
             check.result()

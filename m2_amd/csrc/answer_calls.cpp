@@ -4,36 +4,17 @@
 // 10 to 17 us in Python (torch's own linear: 19), a gradient 100: here the same checks raise the same errors.  us a call, one stream, back to back, Python / here:
 // Int4Linear 768 x 768 11.8 / 6.3 (the launch itself 3.0, the output tensor 0.7); token_logprobs 1 x 30522 17.0 / 8.5, 128 x 30522 fp32 with its gradient 118 / 35 .. 58
 // (most of it torch's own backward pass, which takes one or the other from process to process, on one machine).
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/csrc/utils/pybind.h>
-
-#include <ATen/ATen.h>
-
-#include "../../include/m2_amd.h"
+#include "torch_calls.h"
 
 namespace {
 
-using at::Tensor;
-using std::optional;
-
 // The entry points of libm2_amd.so, which m2_amd/_lib.py has loaded.
-decltype(&m2_last_error) last_error;
 decltype(&m2_int4_weight_bytes) int4_weight_bytes;
 decltype(&m2_int4_workspace_bytes) int4_workspace_bytes;
 decltype(&m2_int4_linear_fwd) int4_linear_fwd;
 decltype(&m2_token_scores_workspace_bytes) token_scores_workspace_bytes;
 decltype(&m2_token_scores_fwd) token_scores_fwd;
 decltype(&m2_token_scores_bwd) token_scores_bwd;
-
-template <typename F>
-void set(F& f, uintptr_t address) { f = reinterpret_cast<F>(address); }
 
 void bind(const std::vector<uintptr_t>& a) {
   TORCH_CHECK(a.size() == 7, "seven addresses");
@@ -45,22 +26,6 @@ void bind(const std::vector<uintptr_t>& a) {
   set(token_scores_fwd, a[5]);
   set(token_scores_bwd, a[6]);
 }
-
-void check(int rc) { TORCH_CHECK(rc == M2_OK, "libm2_amd error ", rc, ": ", last_error()); }
-
-void* current_stream() { return c10::hip::getCurrentHIPStream().stream(); }
-
-void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-int type_of(const char* name, const Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), name, ": must live on the GPU (m2_amd has no CPU path); got device ", t.device());
-  TORCH_CHECK_TYPE(t.layout() == at::kStrided, name, ": must be strided, got ", t.layout());
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, ": must be float32 or bfloat16, got ", t.scalar_type());
-  return t.scalar_type() == at::kFloat ? M2_DTYPE_F32 : M2_DTYPE_BF16;
-}
-
-// The values one behind the other.
-Tensor dense(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
 
 // t (..., n): row r of its leading dimensions lies (r / inner) * outer + (r % inner) * row values behind the first, in t or a copy of it: one is made where
 // a row's values lie apart, or the rows at more than `distances` (1 or 2) distances.
@@ -190,9 +155,6 @@ Found scores(const Tensor& logits, const Scores& s) {
 // A gradient of one value a row: it may be one value for all of them.
 Tensor per_row(const Tensor& g) { return g.defined() ? (g.is_neg() ? g.resolve_neg() : g).reshape({-1}) : g; }
 
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
 // The graph's node.  Its inputs are the gradients of entropy, log probabilities and alternatives' log probabilities, undefined where there is none.
 struct TokenLogprobsBackward : torch::autograd::Node {
   SavedVariable logits_, tokens_, allowed_, entropy_, stats_, ids_;
@@ -276,35 +238,6 @@ std::array<Tensor, 4> token_logprobs(const Tensor& logits, const optional<Tensor
   const Scores s = arguments(logits, tokens, top_k, allowed, ignore_index);
   Found f = logits.requires_grad() && at::GradMode::is_enabled() ? scores_with_graph(logits, s) : scores(logits, s);
   return {std::move(f.logprobs), std::move(f.entropy), std::move(f.ids), std::move(f.top)};
-}
-
-// Arguments come by position, without pybind's conversions (1.1 us a call).
-const Tensor& tensor(const char* name, PyObject* o) {
-  TORCH_CHECK_TYPE(THPVariable_Check(o), name, ": expected a tensor, got ", Py_TYPE(o)->tp_name);
-  return THPVariable_Unpack(o);
-}
-optional<Tensor> tensor_or_none(const char* name, PyObject* o) { return o == Py_None ? std::nullopt : optional<Tensor>(tensor(name, o)); }
-int64_t integer(PyObject* o) {
-  const long long v = PyLong_AsLongLong(o);
-  if (v == -1 && PyErr_Occurred()) throw python_error();
-  return v;
-}
-
-// Refuses what a kernel that is given a tensor's memory would answer wrongly: tensors that are no plain ones, transforms of functions (vmap, jvp, ...), traces,
-// forward-mode gradients, and (unless grad_ok) gradients.
-const Tensor& values(const char* name, PyObject* o, bool grad_ok) {
-  TORCH_CHECK_TYPE(THPVariable_CheckExact(o), name, ": expected a plain tensor, got ", Py_TYPE(o)->tp_name);
-  const Tensor& t = THPVariable_Unpack(o);
-  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !torch::jit::tracer::isTracing() && !t._fw_grad(0).defined(), name,
-              ": function transforms, traces and forward-mode gradients are not supported");
-  TORCH_CHECK(grad_ok || !t.requires_grad() || !at::GradMode::is_enabled(), name,
-              ": this operator has no gradient; call it under torch.no_grad() or on a detached tensor");
-  return t;
-}
-
-PyObject* object_of(Tensor t) {
-  if (!t.defined()) Py_RETURN_NONE;
-  return THPVariable_Wrap(std::move(t));
 }
 
 // (x, weight, N, group, bias or None, gelu) -> y

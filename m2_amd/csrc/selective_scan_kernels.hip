@@ -1,0 +1,422 @@
+// The selective state space scan of a mixer, and its form for one token.
+//
+//   d = softplus(dt + bias)     h[t, n] = exp(d[t] A[n]) h[t - 1, n] + d[t] x[t] B[t, n]     y[t] = (sum_n C[t, n] h[t, n] + D x[t]) z sigmoid(z)
+//
+// for every channel with states n = 0 .. N - 1 of its own, B and C shared by a group of channels.
+//
+// A wave holds 16 positions of 64 / NS channels: for each of its states a lane forms the 16 decays and inputs, runs over them from zero, and keeps them.  The waves
+// of a workgroup lie along the positions; what each of them does to a state (a product of decays and a sum) goes through shared memory, so that every wave knows the
+// state it starts with and runs over its kept decays once more, now with the right state, for the outputs.  Positions are thus worked on side by side, at two more
+// operations a state than one position after another takes, and the decays' exponentials, four times as costly as the others, are formed once.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "selective_scan.h"
+
+namespace m2 {
+
+template <typename T, int NS, int NL>
+__global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
+  using S = ScanShape<NS, NL>;
+  constexpr int CW = S::CW, NP = S::NP, TT = S::TT, NT = S::NT, PITCH = S::PITCH;
+  constexpr int kWave = 2 * S::TILE + (NS > 1 ? 2 * CW * PITCH : 0);      // floats
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane % CW, q = lane / CW;
+  const int id = xcd_order(blockIdx.x, gridDim.x), block = id % p.blocks, g = id / p.blocks % p.G, b = id / p.blocks / p.G;
+  const int count = min(CW, p.per_group - block * CW);
+  const bool on = c < count;
+  const int ch = g * p.per_group + block * CW + min(c, count - 1);
+  const int n = scan_length(p, b), span = W * TT;
+  float* Bs = lds + w * kWave;
+  float* Cs = Bs + S::TILE;
+  float* ds = Cs + S::TILE;
+  float* xs = ds + CW * PITCH;
+  float* ex = lds + W * kWave;      // (2, W, 2, 64, NL)
+
+  float A2[NL], H[NL];      // decays in powers of two; the state ahead of the step's first position
+#pragma unroll
+  for (int j = 0; j < NL; ++j) {
+    const int at = q * NL + j;
+    const bool real = on && at < p.N;
+    A2[j] = real ? p.A[(long)ch * p.N + at] * kLog2E : 0.f;
+    H[j] = real && p.state ? p.state[((long)b * p.channels + ch) * p.N + at] : 0.f;
+  }
+  const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.D ? p.D[ch] : 0.f;
+  const T* x = static_cast<const T*>(p.x) + b * p.x_batch + ch;
+  const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch + ch;
+  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_batch + ch : nullptr;
+  const T* Bm = static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group;
+  const T* Cm = static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group;
+  T* y = static_cast<T*>(p.y) + (long)b * p.L * p.channels + ch;
+  // a lane moves positions q, q + NS, ... of its channel (lanes beyond the 16th of a channel none)
+  const bool moves = NS <= TT || q < TT;
+  const int q0 = NS <= TT ? q : min(q, TT - 1);
+
+  T rx[NT], rdt[NT], rz[NT];
+  TileIn<T, NS, NL, S::AHEAD ? S::NB : 1> rb, rc;      // where they fit into registers, a step's tiles are asked for ahead
+  const auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int t = min(t0 + q0 + i * NS, n - 1);
+      rx[i] = x[t * p.x_row], rdt[i] = dt[t * p.dt_row];
+      if (z) rz[i] = z[t * p.z_row];
+    }
+    if constexpr (S::AHEAD) {
+      rb.load(Bm, p.b_row, t0, n, p.N, lane);
+      rc.load(Cm, p.c_row, t0, n, p.N, lane);
+    }
+  };
+  const int steps = (n + span - 1) / span;
+  if (steps > 0) load(w * TT);
+  for (int s = 0; s < steps; ++s) {
+    const int t0 = s * span + w * TT;
+    float xv[NT], gate[NT], own_d[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const bool inside = t0 + q0 + i * NS < n;
+      xv[i] = value_of<T>(rx[i]);
+      float d = value_of<T>(rdt[i]) + bias;
+      if (p.softplus) d = softplus(d);
+      own_d[i] = inside ? d : 0.f;
+      xv[i] = inside ? xv[i] : 0.f;
+      gate[i] = z ? silu(value_of<T>(rz[i])) : 1.f;
+    }
+    wave_sync();      // the tiles have been read
+    if constexpr (S::AHEAD) {
+      rb.put(Bs, lane);
+      rc.put(Cs, lane);
+    } else {
+      tile_in<T, NS, NL>(Bs, Bm, p.b_row, t0, n, p.N, lane);
+      tile_in<T, NS, NL>(Cs, Cm, p.c_row, t0, n, p.N, lane);
+    }
+    if constexpr (NS > 1) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (moves) ds[c * PITCH + q0 + i * NS] = own_d[i], xs[c * PITCH + q0 + i * NS] = own_d[i] * xv[i];
+    }
+    wave_sync();
+    if (s + 1 < steps) load(t0 + span);
+    float a[TT][NL], u[TT][NL], h[NL], total = 0.f;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) h[j] = 0.f;
+#pragma unroll
+    for (int t4 = 0; t4 < TT; t4 += 4) {
+      float d4[4], x4[4];
+      if constexpr (NS > 1) {
+        load_values<float, 4>(ds + c * PITCH + t4, d4);
+        load_values<float, 4>(xs + c * PITCH + t4, x4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d4[i] = own_d[(t4 + i) % NT], x4[i] = d4[i] * xv[(t4 + i) % NT];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t4 + i;
+        float bn[NL];
+        load_values<float, NL>(Bs + t * NP + q * NL, bn);
+        total += d4[i];
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+          a[t][j] = __builtin_amdgcn_exp2f(d4[i] * A2[j]);
+          u[t][j] = x4[i] * bn[j];
+          h[j] = fmaf(a[t][j], h[j], u[t][j]);
+        }
+      }
+    }
+    float P[NL], start[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * A2[j]);
+    if (p.saved && w == 0 && on) {
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+        if (q * NL + j < p.N) p.saved[(((long)b * p.parts + s) * p.channels + ch) * p.N + q * NL + j] = H[j];
+    }
+    if (W == 1) {
+#pragma unroll
+      for (int j = 0; j < NL; ++j) start[j] = H[j], H[j] = fmaf(P[j], H[j], h[j]);
+    } else {
+      float* turn = ex + (s & 1) * W * 2 * 64 * NL;
+      store_values<float, NL>(turn + (w * 2 * 64 + lane) * NL, P);
+      store_values<float, NL>(turn + ((w * 2 + 1) * 64 + lane) * NL, h);
+      __syncthreads();      // (two turns: what is written next is read behind the next barrier)
+      for (int o = 0; o < W; ++o) {
+        if (o == w) {
+#pragma unroll
+          for (int j = 0; j < NL; ++j) start[j] = H[j];
+        }
+        float po[NL], ho[NL];
+        load_values<float, NL>(turn + (o * 2 * 64 + lane) * NL, po);
+        load_values<float, NL>(turn + ((o * 2 + 1) * 64 + lane) * NL, ho);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) H[j] = fmaf(po[j], H[j], ho[j]);
+      }
+    }
+    float out[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      float cn[NL];
+      load_values<float, NL>(Cs + t * NP + q * NL, cn);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        start[j] = fmaf(a[t][j], start[j], u[t][j]);
+        sum = j == 0 ? cn[0] * start[0] : fmaf(cn[j], start[j], sum);
+      }
+      out[t] = sum;
+    }
+    share_positions<NS, log2_of(CW)>(out, lane);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int t = t0 + q0 + i * NS;
+      const float v = fmaf(skip, xv[i], out[i]) * gate[i];
+      if (on && moves && t < p.L) y[(long)t * p.channels] = value_to<T>(t < n ? v : 0.f);
+    }
+  }
+  for (int t0 = steps * span + w * TT; t0 < p.L; t0 += span)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int t = t0 + q0 + i * NS;
+      if (on && moves && t < p.L) y[(long)t * p.channels] = value_to<T>(0.f);
+    }
+  if (p.state_out && w == 0 && on) {
+#pragma unroll
+    for (int j = 0; j < NL; ++j)
+      if (q * NL + j < p.N) p.state_out[((long)b * p.channels + ch) * p.N + q * NL + j] = H[j];
+  }
+}
+
+// One token: P lanes a channel, V states a lane at a time.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void selective_scan_step_kernel(ScanArgs p, int P) {
+  const long i = blockIdx.x * 256L + threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const uint32_t item = (uint32_t)(i / P), q = threadIdx.x & (P - 1);
+  const uint32_t last = (uint32_t)p.batch * (uint32_t)p.channels - 1;
+  const bool on = item <= last;
+  const uint32_t at = on ? item : last, b = at / (uint32_t)p.channels, ch = at - b * (uint32_t)p.channels, g = ch / (uint32_t)p.per_group;
+  const T* Bm = static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group;
+  const T* Cm = static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group;
+  const long first = (long)at * p.N;
+  const float xv = value_of<T>(static_cast<const T*>(p.x)[b * p.x_batch + ch]);
+  float d = value_of<T>(static_cast<const T*>(p.dt)[b * p.dt_batch + ch]) + (p.dt_bias ? p.dt_bias[ch] : 0.f);
+  if (p.softplus) d = softplus(d);
+  const float dx = d * xv;
+  float sum = 0.f;
+  for (int n = q * V; n < p.N; n += P * V) {
+    float av[V], hv[V];
+    load_values<float, V>(p.A + (long)ch * p.N + n, av);
+    load_values<float, V>(p.state + first + n, hv);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      hv[j] = fmaf(__builtin_amdgcn_exp2f(d * (av[j] * kLog2E)), hv[j], dx * value_of<T>(Bm[n + j]));
+      sum = fmaf(value_of<T>(Cm[n + j]), hv[j], sum);
+    }
+    if (on) store_values<float, V>(p.state_out + first + n, hv);
+  }
+  if (P > 1) sum = sum_over_bit<0>(sum, lane);
+  if (P > 2) sum = sum_over_bit<1>(sum, lane);
+  if (P > 4) sum = sum_over_bit<2>(sum, lane);
+  if (P > 8) sum = sum_over_bit<3>(sum, lane);
+  if (P > 16) sum = sum_over_bit<4>(sum, lane);
+  if (P > 32) sum = sum_over_bit<5>(sum, lane);
+  if (on && q == 0) {
+    float v = fmaf(p.D ? p.D[ch] : 0.f, xv, sum);
+    if (p.z) v *= silu(value_of<T>(static_cast<const T*>(p.z)[b * p.z_batch + ch]));
+    static_cast<T*>(p.y)[(long)b * p.channels + ch] = value_to<T>(v);
+  }
+}
+
+namespace {
+
+constexpr int kMaxStates = 256;
+
+int check_scan(const char* name, const ScanArgs& p, int dtype) {
+  if (p.batch < 1 || p.L < 1 || p.channels < 1 || p.G < 1 || p.channels % p.G) return set_error(M2_ERR_ARG, "%s: B=%d, L=%d, D=%d, G=%d", name, p.batch, p.L, p.channels, p.G);
+  if (p.N < 1 || p.N > kMaxStates) return set_error(M2_ERR_UNSUPPORTED, "%s: N=%d states, 1 .. %d are supported", name, p.N, kMaxStates);
+  if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype %d", name, dtype);
+  if ((long)p.batch * p.L > (1L << 36) / ((long)p.G * p.N)) return set_error(M2_ERR_ARG, "%s: at most 2^36 values of B", name);
+  if (p.channels > 1 << 20 || p.L > 1 << 30 || (long)p.batch * p.channels > 1L << 24)
+    return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^24 channels of all sequences", name);
+  return M2_OK;
+}
+
+int check_grid(const char* name, const ScanArgs& p, const ScanPlan& plan) {
+  if ((long)plan.blocks * p.G * p.batch * plan.W >= 1L << 26) return set_error(M2_ERR_ARG, "%s: B=%d, D=%d, N=%d are more than a launch holds", name, p.batch, p.channels, p.N);
+  return M2_OK;
+}
+
+int pow2_from(int n) {
+  int r = 1;
+  while (r < n) r *= 2;
+  return r;
+}
+
+size_t fwd_lds(const ScanPlan& s) {
+  const int CW = 64 / s.NS;
+  return sizeof(float) * s.W * (2 * 16 * s.NS * s.NL + (s.NS > 1 ? 2 * CW * 20 : 0) + (s.W > 1 ? 2 * 2 * 64 * s.NL : 0));
+}
+
+// The first of the numbers of states a lane that is built, one where the workgroups would leave compute units without.
+template <typename SHAPES>
+void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
+  const int per_group = D / G;
+  for (int NL : {4, 2, 1}) {
+    const int NS = std::max(pow2_from((N + NL - 1) / NL), SHAPES::built(1, 1) ? 1 : 2);
+    if (NS > 64) break;
+    if (!SHAPES::built(NS, NL)) continue;
+    const int CW = 64 / NS;
+    r.NS = NS, r.NL = NL, r.blocks = (per_group + CW - 1) / CW;
+    if ((long)r.blocks * G * B >= num_cus()) break;
+  }
+}
+// Waves as many as there are positions for, up to eight; as the gradient's where the states ahead of each step are kept for it.
+ScanPlan fwd_plan(int B, int L, int D, int G, int N, bool saved) {
+  ScanPlan r{};
+  choose_shape<ForwardShapes>(r, B, D, G, N);
+  r.W = saved ? m2_selective_scan_span(N) / 16 : 8;
+  while (!saved && r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
+  while (!saved && fwd_lds(r) > (80 << 10)) r.W /= 2;
+  return r;
+}
+ScanPlan bwd_plan(int B, int D, int G, int N) {
+  ScanPlan r{};
+  choose_shape<GradientShapes>(r, B, D, G, N);
+  r.W = m2_selective_scan_span(N) / 16;
+  return r;
+}
+
+// The gradient's workspace: partial gradients of B and C, then of A, D and dt_bias.
+struct Partials {
+  size_t bc, a, d;      // floats of one of each
+  Partials(const ScanArgs& p, int blocks) : bc((size_t)blocks * p.batch * p.L * p.G * p.N), a((size_t)p.batch * p.channels * p.N), d((size_t)p.batch * p.channels) {}
+  size_t bytes() const { return sizeof(float) * (2 * bc + a + 2 * d); }
+};
+
+// A group's partial gradients of B (blockIdx.y 0) or C, one from each of its workgroups, added up; 0 behind the end of a sequence.
+template <typename T>
+__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, T* gB, T* gC) {
+  T* out = blockIdx.y ? gC : gB;
+  if (!out) return;
+  const long row = (long)p.G * p.N, count = (long)p.batch * p.L * row, i = blockIdx.x * 256L + threadIdx.x;
+  if (i >= count) return;
+  const long bt = i / row;
+  const int b = bt / p.L, t = bt - (long)b * p.L;
+  const float* part = (blockIdx.y ? p.c_part : p.b_part) + i;
+  float sum = 0.f;
+  if (t < scan_length(p, b))
+    for (int k = 0; k < p.blocks; ++k) sum += part[k * count];
+  out[i] = value_to<T>(sum);
+}
+
+}  // namespace
+}  // namespace m2
+
+using namespace m2;
+
+// Positions between the states that are kept for the gradient.
+extern "C" int m2_selective_scan_span(int N) {
+  if (N < 1 || N > kMaxStates) return 0;
+  return N <= 64 ? 128 : N <= 128 ? 64 : 32;
+}
+
+namespace {
+
+void fill(ScanArgs& p, const m2_scan_inputs* in) {
+  p.x = in->x, p.dt = in->dt, p.z = in->z, p.Bm = in->Bm, p.Cm = in->Cm;
+  p.x_batch = in->x_batch, p.x_row = in->x_row, p.dt_batch = in->dt_batch, p.dt_row = in->dt_row, p.z_batch = in->z_batch, p.z_row = in->z_row;
+  p.b_batch = in->b_batch, p.b_row = in->b_row, p.b_group = in->b_group, p.c_batch = in->c_batch, p.c_row = in->c_row, p.c_group = in->c_group;
+  p.A = in->A, p.D = in->D, p.dt_bias = in->dt_bias, p.state = in->state, p.lengths = in->lengths;
+  p.batch = in->batch, p.L = in->length, p.channels = in->channels, p.G = in->groups, p.N = in->states, p.softplus = in->softplus;
+  p.per_group = p.G > 0 ? p.channels / p.G : 0;
+}
+bool given(const ScanArgs& p) { return p.x && p.dt && p.Bm && p.Cm && p.A; }
+
+}  // namespace
+
+extern "C" int m2_selective_scan_fwd(const m2_scan_inputs* in, void* y, float* state_out, float* saved, int dtype, void* stream) {
+  ScanArgs p{};
+  if (in) fill(p, in);
+  if (!in || !y || !given(p)) return set_error(M2_ERR_ARG, "selective_scan_fwd: null pointer");
+  if (int rc = check_scan("selective_scan_fwd", p, dtype)) return rc;
+  const ScanPlan plan = fwd_plan(p.batch, p.L, p.channels, p.G, p.N, saved != nullptr);
+  p.y = y, p.state_out = state_out, p.saved = saved, p.blocks = plan.blocks;
+  p.parts = (p.L + plan.positions() - 1) / plan.positions();
+  if (int rc = check_grid("selective_scan_fwd", p, plan)) return rc;
+  const unsigned grid = (unsigned)((long)plan.blocks * p.G * p.batch);
+  const size_t lds = fwd_lds(plan);
+  int rc = M2_OK;
+  with_scan_shape<ForwardShapes>(plan.NS, plan.NL, [&](auto ns, auto nl) {
+    const auto launch = [&](auto t) {
+      const auto kernel = selective_scan_kernel<decltype(t), decltype(ns)::value, decltype(nl)::value>;
+      const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) {
+        rc = set_error(M2_ERR_LAUNCH, "selective_scan_fwd: %zu bytes of shared memory: %s", lds, hipGetErrorString(e));
+        return;
+      }
+      hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * plan.W), lds, (hipStream_t)stream, p);
+    };
+    if (dtype == M2_DTYPE_F32) launch(float{});
+    else launch(uint16_t{});
+  });
+  return rc != M2_OK ? rc : check_launch("selective_scan_kernel");
+}
+
+extern "C" size_t m2_selective_scan_bwd_workspace_bytes(int batch, int length, int channels, int groups, int states) {
+  ScanArgs p{};
+  p.batch = batch, p.L = length, p.channels = channels, p.G = groups, p.N = states;
+  if (check_scan("selective_scan_bwd", p, M2_DTYPE_F32)) return 0;
+  return Partials(p, bwd_plan(batch, channels, groups, states).blocks).bytes();
+}
+
+extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gradients* out, const float* saved, void* workspace, int dtype, void* stream) {
+  ScanArgs p{};
+  if (in) fill(p, in);
+  if (!in || !out || !given(p) || !out->gy || !saved || !workspace) return set_error(M2_ERR_ARG, "selective_scan_bwd: null pointer");
+  if (int rc = check_scan("selective_scan_bwd", p, dtype)) return rc;
+  const ScanPlan plan = bwd_plan(p.batch, p.channels, p.G, p.N);
+  if (int rc = check_grid("selective_scan_bwd", p, plan)) return rc;
+  const hipStream_t s = (hipStream_t)stream;
+  p.blocks = plan.blocks, p.parts = (p.L + plan.positions() - 1) / plan.positions();
+  p.gy = out->gy, p.gy_batch = out->gy_batch, p.gy_row = out->gy_row, p.gstate_out = out->gstate_out;
+  p.gx = out->gx, p.gdt = out->gdt, p.gz = out->gz, p.gstate = out->gstate;
+  p.saved = const_cast<float*>(saved);
+  const Partials room(p, plan.blocks);
+  p.b_part = static_cast<float*>(workspace), p.c_part = p.b_part + room.bc;
+  p.a_part = p.c_part + room.bc, p.d_part = p.a_part + room.a, p.bias_part = p.d_part + room.d;
+  if (int rc = scan_bwd(p, plan, dtype, s)) return rc;
+  if (out->gB || out->gC) {
+    const long count = (long)p.batch * p.L * p.G * p.N;
+    const dim3 grid((unsigned)((count + 255) / 256), 2);
+    if (dtype == M2_DTYPE_F32) hipLaunchKernelGGL(scan_join_kernel<float>, grid, dim3(256), 0, s, p, (float*)out->gB, (float*)out->gC);
+    else hipLaunchKernelGGL(scan_join_kernel<uint16_t>, grid, dim3(256), 0, s, p, (uint16_t*)out->gB, (uint16_t*)out->gC);
+    if (int rc = check_launch("scan_join_kernel")) return rc;
+  }
+  if (out->gA)
+    if (int rc = sum_partials(p.a_part, p.batch, 0, (long)p.channels * p.N, nullptr, out->gA, s)) return rc;
+  if (out->gD)
+    if (int rc = sum_partials(p.d_part, p.batch, 0, p.channels, nullptr, out->gD, s)) return rc;
+  if (out->gdt_bias) return sum_partials(p.bias_part, p.batch, 0, p.channels, nullptr, out->gdt_bias, s);
+  return M2_OK;
+}
+
+extern "C" int m2_selective_scan_step(const m2_scan_inputs* in, void* y, float* state_out, int dtype, void* stream) {
+  ScanArgs p{};
+  if (in) fill(p, in);
+  if (!in || !y || !state_out || !given(p) || !p.state) return set_error(M2_ERR_ARG, "selective_scan_step: null pointer");
+  if (int rc = check_scan("selective_scan_step", p, dtype)) return rc;
+  p.y = y, p.state_out = state_out;
+  const bool wide = p.N % 4 == 0 && m2::aligned16(p.A, p.state, p.state_out);
+  const int P = std::min(64, pow2_from(wide ? p.N / 4 : p.N));
+  const unsigned grid = (unsigned)(((long)p.batch * p.channels * P + 255) / 256);
+  const auto launch = [&](auto t) {
+    using T = decltype(t);
+    if (wide) hipLaunchKernelGGL((selective_scan_step_kernel<T, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p, P);
+    else hipLaunchKernelGGL((selective_scan_step_kernel<T, 1>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p, P);
+    return check_launch("selective_scan_step_kernel");
+  };
+  return dtype == M2_DTYPE_F32 ? launch(float{}) : launch(uint16_t{});
+}

@@ -33,6 +33,22 @@ except ImportError as e:
         int4_linear = token_logprobs = _absent
     warnings.warn(f"{_answer_calls._why}; until then Int4Linear and token_logprobs raise", RuntimeWarning)
 
+try:
+    from . import _causal_calls
+    _causal_calls.bind([ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+        "m2_last_error", "m2_causal_conv_fwd", "m2_causal_conv_bwd_workspace_bytes", "m2_causal_conv_bwd", "m2_causal_conv_step", "m2_selective_scan_span", "m2_selective_scan_fwd",
+        "m2_selective_scan_bwd_workspace_bytes", "m2_selective_scan_bwd", "m2_selective_scan_step", "m2_group_norm_workspace_bytes", "m2_group_norm_fwd", "m2_group_norm_bwd")])
+except ImportError as e:
+    class _causal_calls:
+        _why = f"m2_amd/_causal_calls.so is missing or does not fit this torch ({e}): build it with `python m2_amd/build.py`"
+
+        @classmethod
+        def _absent(cls, *_):
+            raise RuntimeError(cls._why)
+
+        causal_conv = causal_conv_step = selective_scan = selective_scan_step = group_norm = _absent
+    warnings.warn(f"{_causal_calls._why}; until then causal_conv, selective_scan, their steps and group_norm raise", RuntimeWarning)
+
 Tensor = torch.Tensor
 
 
@@ -772,3 +788,36 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor], top_k: int, allowed
     """-> (log probabilities of `tokens` | None, entropies, alternatives' ids | None, their log probabilities | None), with a gradient where the logits ask for one;
     see scores.token_logprobs."""
     return _answer_calls.token_logprobs(logits, tokens, top_k, allowed, ignore_index)
+
+
+def _activation(activation: Optional[str], known: Sequence[str]) -> int:
+    if activation is None:
+        return 0
+    if activation not in known:
+        raise ValueError(f"activation must be None or one of {tuple(known)}, got {activation!r}")
+    return 1 + known.index(activation)
+
+
+def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], state: Optional[Tensor], lengths: Optional[Tensor], return_state: bool):
+    """-> (y, state | None), with a gradient where an input asks for one; see causal.causal_conv."""
+    return _causal_calls.causal_conv(x, weight, bias, _activation(activation, ("silu",)) == 1, state, lengths, bool(return_state))
+
+
+def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str], out_state: Optional[Tensor]) -> Tensor:
+    return _causal_calls.causal_conv_step(x, state, weight, bias, _activation(activation, ("silu",)) == 1, out_state)
+
+
+def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor], dt_softplus: bool,
+                   state: Optional[Tensor], lengths: Optional[Tensor], return_state: bool):
+    """-> (y, state | None), with a gradient where an input asks for one; see causal.selective_scan."""
+    return _causal_calls.selective_scan(x, dt, A, B, C, D, z, dt_bias, state, lengths, bool(dt_softplus), bool(return_state))
+
+
+def selective_scan_step(x: Tensor, dt: Tensor, state: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Optional[Tensor], z: Optional[Tensor], dt_bias: Optional[Tensor],
+                        dt_softplus: bool, out_state: Optional[Tensor]) -> Tensor:
+    return _causal_calls.selective_scan_step(x, dt, A, B, C, D, z, dt_bias, state, bool(dt_softplus), out_state)
+
+
+def group_norm(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, activation: Optional[str]) -> Tensor:
+    """act(group norm of x (N, ..., C)), with a gradient where an input asks for one; see causal.group_norm."""
+    return _causal_calls.group_norm(x, groups, weight, bias, float(eps), _activation(activation, ("silu", "gelu")))
