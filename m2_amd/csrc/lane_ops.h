@@ -117,41 +117,38 @@ __device__ __forceinline__ float lane_sum(float v, int lane) {
 
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// exp(x) to about 2^-23 of itself: the product with log2 e in two parts, of which the second is a factor near 1.
+// exp(x), x <= 88, to about 2^-23 of itself: the product with log2 e in two parts, of which the second is a factor near 1.  Below -100: as at -100 (NaN too).
 __device__ __forceinline__ float exp_of(float x) {
+  x = fmaxf(x, -100.f);
   const float hi = x * kLog2E;
-  const float lo = fmaf(x, kLog2E, -hi) + x * 1.925963033500e-8f;      // what hi has lost, and log2 e beyond its 24 bits
+  const float lo = fmaf(x, 1.925963033500e-8f, fmaf(x, kLog2E, -hi));      // what hi has lost, and log2 e beyond its 24 bits
   const float e = __builtin_amdgcn_exp2f(hi);
-  const float r = fmaf(e, lo * kLn2, e);
-  return fabsf(hi) < 150.f ? r : e;      // (0, infinity and NaN as they are)
+  return fmaf(e, lo * kLn2, e);
 }
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x)); }
+// 1 / (1 + exp(-x)); of NaN some number.
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(fminf(-x, 88.f))); }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
-// d/dx of x sigmoid(x) = s (1 + x (1 - s)); 1 - s = sigmoid(-x) is formed without cancellation where it is small.
-__device__ __forceinline__ float silu_slope(float x) {
-  const float e = exp_of(-fabsf(x));
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
-  const float s = x < 0.f ? e * r : r, t = x < 0.f ? r : e * r;      // sigmoid(x), sigmoid(-x)
-  return fmaf(s * x, t, s);
+// u = exp(-|x|) and r = 1 / (1 + u): what sigmoid(x), sigmoid(-x), softplus(x) and their products are made of, without cancellation.
+struct Logistic {
+  float u, r;
+  bool below;
+  __device__ __forceinline__ explicit Logistic(float x) : u(exp_of(-fabsf(x))), r(__builtin_amdgcn_rcpf(1.f + u)), below(x < 0.f) {}
+  __device__ __forceinline__ float value() const { return below ? u * r : r; }
+  __device__ __forceinline__ float other() const { return below ? r : u * r; }      // of -x
+};
+// log(1 + exp(x)) = max(x, 0) + log(1 + u), u = exp(-|x|) <= 1: log(w) of the rounded w = 1 + u, and what the rounding has lost over w (1 / w by a parabola: 6 % are enough).
+__device__ __forceinline__ float softplus_of(float x, float u) {
+  const float w = 1.f + u, lost = u - (w - 1.f);
+  const float l = fmaf(__builtin_amdgcn_logf(w), kLn2, lost * fmaf(u, fmaf(u, 0.5f, -1.f), 1.f));
+  return (x < 0.f ? 0.f : x) + l;
 }
-// log(1 + exp(x)) = max(x, 0) + log1p(u), u = exp(-|x|) <= 1: log1p(u) = 2 artanh(u / (2 + u)), whose argument is at most 1/3, by its series.
-__device__ __forceinline__ float softplus(float x) {
-  const float u = exp_of(-fabsf(x));
-  const float den = 2.f + u;
-  float r = __builtin_amdgcn_rcpf(den);
-  r = fmaf(fmaf(-den, r, 1.f), r, r);
-  const float s = u * r, q = s * s;
-  float p = 1.f / 17.f;
-  p = fmaf(p, q, 1.f / 15.f);
-  p = fmaf(p, q, 1.f / 13.f);
-  p = fmaf(p, q, 1.f / 11.f);
-  p = fmaf(p, q, 1.f / 9.f);
-  p = fmaf(p, q, 1.f / 7.f);
-  p = fmaf(p, q, 1.f / 5.f);
-  p = fmaf(p, q, 1.f / 3.f);
-  const float l = 2.f * fmaf(s * q, p, s);
-  return x != x ? x : fmaxf(x, 0.f) + l;
+__device__ __forceinline__ float softplus(float x) { return softplus_of(x, exp_of(-fabsf(x))); }
+// d/dx of x sigmoid(x) = s + x s (1 - s)
+__device__ __forceinline__ float silu_slope_of(float x, const Logistic& l) {
+  const float s = l.value();
+  return fmaf(s * x, l.other(), s);
 }
+__device__ __forceinline__ float silu_slope(float x) { return silu_slope_of(x, Logistic(x)); }
 
 // Sums of `rows` partial results: column j of plane k (planes (K + 1 or 1) x n values) goes to wide[j * K + k] for k < K and to last[j] for k = K; either may be null.
 int sum_partials(const float* partials, long rows, int K, long n, float* wide, float* last, hipStream_t stream);

@@ -17,6 +17,9 @@ struct ScanArgs {
   float* saved;                              // (B, parts, D, N): the state ahead of each part of a sequence, for the gradient, or null
   int batch, L, channels, G, N, softplus;
   int per_group, blocks, parts;              // channels of a group, workgroups for them, parts of a sequence
+  int apart;                                 // positions between the states that are kept
+  int kept_parts;                            // the gradient: how many of those a workgroup's step has
+  int sets;                                  // the gradient: sets of 64 / NS channels that a workgroup takes one after the other
   // gradients
   const float* gstate_out;                   // or null
   void *gx, *gdt, *gz;                       // (B, L, D)
@@ -24,6 +27,14 @@ struct ScanArgs {
   float *b_part, *c_part;                    // (blocks, B, L, G, N)
   float *a_part, *d_part, *bias_part;        // (B, D, N), (B, D), (B, D)
 };
+
+// The kernel's arguments anew: values that are read where they are needed, and not kept in (too few) scalar registers from the kernel's start.
+typedef const __attribute__((address_space(4))) ScanArgs ArgsInMemory;
+__device__ __forceinline__ ArgsInMemory* arguments_anew() {
+  ArgsInMemory* p = (ArgsInMemory*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // A wave takes 64 / NS channels times NS lanes with NL states each, for TT positions.  QLOW: a channel's lanes are neighbours; else they lie 64 / NS apart.
 template <int NS, int NL>
@@ -70,41 +81,76 @@ __device__ __forceinline__ T value_to(float v) {
   else return f32_to_bf16(v);
 }
 
-// B or C of a wave's positions on their way from memory (positions t0 .. of a sequence of n > 0; beyond it, the last one's are read) to fp32 in shared memory,
+// The value is made here: one made of a loaded register only later would hold that register over the next load into it, which a loop then waits for.
+__device__ __forceinline__ void made_here(float& v) { asm volatile("" : "+v"(v)); }
+
+// A value at a byte offset from what is the same for all lanes: a scalar address and a 32-bit offset.
+template <typename V, typename T>
+__device__ __forceinline__ V& at_offset(T* base, uint32_t bytes) {
+  if constexpr (std::is_const<T>::value) return *reinterpret_cast<V*>(reinterpret_cast<const char*>(base) + bytes);
+  else return *reinterpret_cast<V*>(reinterpret_cast<char*>(base) + bytes);
+}
+
+// Where a lane's values of a tensor (rows `row` values apart, below 2^24) lie from row t0 of it, in bytes: those of row t0 + t, but of no row behind `last`.  Rows
+// grow with offsets, so the smaller offset is the nearer row; one load serves both, and nothing waits for a choice.
+struct Near {
+  uint32_t first, end;
+  template <typename T>
+  __device__ __forceinline__ static Near of(const T*, int t, long row, int at, int last) {
+    return {(uint32_t)(t * (int)row + at) * (uint32_t)sizeof(T), (uint32_t)(last * (int)row + at) * (uint32_t)sizeof(T)};
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t further) const { return min(first + further, end); }
+};
+
+// B or C of a wave's positions on their way from memory (positions t0 .. of a sequence of n > t0; beyond it, the last one's are read) to fp32 in shared memory,
 // (TT, NP), zero behind N.
 template <typename T, int NS, int NL, int COUNT>
 struct TileIn {
   using S = ScanShape<NS, NL>;
+  static constexpr int PER = S::NP >= 4 ? S::NP / 4 : 1, APART = 64 / PER > 1 ? 64 / PER : 1;      // vectors of a row; rows between a lane's vectors
   typename Raw4<T>::type raw[COUNT];
   __device__ __forceinline__ void load(const T* rows, long row, int t0, int n, int N, int lane, int first = 0) {
+    const T* base = rows + (long)t0 * row;
+    const int last = min(n - 1 - t0, S::TT - 1);
     if constexpr (S::NP >= 4) {
+      if (N >= 4) {      // a vector that would pass N ends with it
+        const Near off = Near::of(rows, min(lane / PER, S::TT - 1), row, min(lane % PER * 4, N - 4), last);
 #pragma unroll
-      for (int i = 0; i < COUNT; ++i) {
-        const int v = lane + 64 * (first + i), t = min(v / (S::NP / 4), S::TT - 1), at = v % (S::NP / 4) * 4;
-        const T* r = rows + min(t0 + t, n - 1) * row;
-        if (at + 4 <= N) {
-          raw[i] = *reinterpret_cast<const typename Raw4<T>::type*>(r + at);
-        } else {
+        for (int i = 0; i < COUNT; ++i) raw[i] = at_offset<const typename Raw4<T>::type>(base, off((uint32_t)((first + i) * APART * (int)row) * (uint32_t)sizeof(T)));
+      } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) raw[i][j] = at + j < N ? r[at + j] : T(0);
+        for (int i = 0; i < COUNT; ++i) {
+          const T* r = base + (long)min(min(lane / PER, S::TT - 1) + (first + i) * APART, last) * row;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raw[i][j] = j < N ? r[j] : T(0);
         }
       }
     } else {
-      const int t = min(lane / S::NP, S::TT - 1), at = lane % S::NP;
-      raw[0][0] = at < N ? rows[min(t0 + t, n - 1) * row + at] : T(0);
+      const int at = lane % S::NP;
+      raw[0][0] = at < N ? base[(long)min(lane / S::NP, last) * row + at] : T(0);
     }
   }
-  __device__ __forceinline__ void put(float* tile, int lane, int first = 0) const {
+  __device__ __forceinline__ void put(float* tile, int N, int lane, int first = 0) const {
     if constexpr (S::NP >= 4) {
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) {
-        const int v = lane + 64 * (first + i);
-        if (v < S::TILE / 4) {
-          float f[4];
+        const int v = lane + 64 * (first + i), at = lane % PER * 4;
+        float f[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[j] = Raw4<T>::get(raw[i], j);
-          store_values<float, 4>(tile + v * 4, f);
+        for (int j = 0; j < 4; ++j) f[j] = Raw4<T>::get(raw[i], j);
+        if (N >= 4 && N < S::NP) {      // (the same for all lanes)
+          float g[4];
+          const int moved = at - min(at, N - 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            g[j] = 0.f;
+#pragma unroll
+            for (int k = j; k < 4; ++k) g[j] = k - j == moved ? f[k] : g[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[j] = g[j];
         }
+        if (v < S::TILE / 4) store_values<float, 4>(tile + v * 4, f);
       }
     } else if (lane < S::TILE) {
       tile[lane] = Raw4<T>::get(raw[0], 0);
@@ -117,7 +163,7 @@ __device__ __forceinline__ void tile_in(float* tile, const T* rows, long row, in
   for (int first = 0; first < NB; first += AT_ONCE) {
     TileIn<T, NS, NL, AT_ONCE> in;
     in.load(rows, row, t0, n, N, lane, first);
-    in.put(tile, lane, first);
+    in.put(tile, N, lane, first);
   }
 }
 
@@ -160,7 +206,7 @@ void with_scan_shape(int NS, int NL, F&& f) {
 }
 // Four states of a lane hold 128 registers of decays and inputs in the forward; the gradient has room for two, and for four only where no channels' sums are formed.
 struct ForwardShapes {
-  static constexpr bool built(int NS, int NL) { return NL == 1 || (NL == 4 && NS >= 2); }
+  static constexpr bool built(int NS, int NL) { return NL <= 2 || NS >= 2; }
 };
 struct GradientShapes {
   static constexpr bool built(int NS, int NL) { return NS >= 2 && (NL <= 2 || NS == 64); }
@@ -168,10 +214,11 @@ struct GradientShapes {
 
 // How a call is spread: lanes a channel, states a lane, waves of a workgroup.
 struct ScanPlan {
-  int NS, NL, W, blocks;
+  int NS, NL, W, blocks, sets;
   int positions() const { return W * 16; }      // of a workgroup's step
 };
 
+size_t scan_bwd_lds(const ScanPlan& plan);
 int scan_bwd(const ScanArgs& p, const ScanPlan& plan, int dtype, hipStream_t stream);
 
 }  // namespace m2

@@ -4,10 +4,11 @@
 //   gB[t, n] = sum over channels dh d x     gC[t, n] = sum over channels u h     gx = d sum_n dh B + D u
 //   gd = sum_n dh a h[t - 1] A + x sum_n dh B     gA = sum_t dh a h[t - 1] d     gD = sum_t u x     gz = gy (sum_n C h + D x) silu'(z)
 //
-// Workgroups lie as in the forward and go through a sequence from its end, a step of `span` positions at a time, each from the state that the forward has kept ahead
-// of it.  A wave forms decays and inputs of its positions, runs over them from zero in both directions, and meets the others once, in shared memory, for the state it
-// starts with and the gradient it ends with.  Forward again for the states, then backward: what the channels of a wave add to B's and C's gradients is summed
-// across lanes as it arises, in a tree over positions that leaves each lane with positions of its own, and goes to memory for scan_join_kernel, in a fixed order.
+// A workgroup goes through a sequence from its end, a step of 16 positions a wave at a time, each from the state that the forward has kept ahead of it, and in a step
+// through several sets of 64 / NS channels.  A wave forms decays and inputs of its positions, runs over them from zero in both directions, and meets the others once,
+// in shared memory, for the state it starts with and the gradient it ends with.  Forward again for the states, then backward: what the channels of a wave add to
+// B's and C's gradients is summed across lanes as it arises, in a tree over positions that leaves each lane with positions of its own, and over the sets in shared
+// memory; the sums of a workgroup go to memory for scan_join_kernel.  All in a fixed order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -15,29 +16,28 @@
 
 namespace m2 {
 
-// Values of the positions of a group of 2^LV, highest first, summed across the lanes of the wave's channels: position bit k goes with lane bit 5 - k.
-template <int LV, int NL>
+// Values of the positions of a group of 2^LV, highest first, summed across 2^LV lanes: position bit k goes with lane bit FIRST + k * STEP, and each lane is left with the
+// sum of its own position.
+template <int LV, int NL, int FIRST, int STEP>
 struct Tree {
   float at[LV > 0 ? LV : 1][NL];      // per level, what waits for its neighbour
-  // position t of the group; the result is complete in v when t is 0
-  template <int T>
+  // position T of the group; v is complete when T is 0
+  template <int T, int K = 0>
   __device__ __forceinline__ void add(float (&v)[NL], int lane) {
-    step<T, 0>(v, lane);
-  }
-  template <int T, int K>
-  __device__ __forceinline__ void step(float (&v)[NL], int lane) {
     if constexpr (K < LV) {
       if constexpr ((T >> K) & 1) {
 #pragma unroll
         for (int j = 0; j < NL; ++j) at[K][j] = v[j];
       } else {
 #pragma unroll
-        for (int j = 0; j < NL; ++j) v[j] = split_over_bit<5 - K>(v[j], at[K][j], lane);
-        step<T, K + 1>(v, lane);
+        for (int j = 0; j < NL; ++j) v[j] = split_over_bit<FIRST + K * STEP>(v[j], at[K][j], lane);
+        add<T, K + 1>(v, lane);
       }
     }
   }
 };
+// Keeps the loads of a group of positions behind those before it: all of them ahead of their use would not fit into registers.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 
 template <int FIRST, int LAST, typename F>
 __device__ __forceinline__ void count_down(F&& f) {      // f(FIRST), ..., f(LAST) as constants
@@ -45,276 +45,394 @@ __device__ __forceinline__ void count_down(F&& f) {      // f(FIRST), ..., f(LAS
   if constexpr (FIRST > LAST) count_down<FIRST - 1, LAST>(f);
 }
 
+// Floats of shared memory: of a wave, of a wave and set, of a set.
+template <int NS, int NL>
+struct GradientRoom {
+  using S = ScanShape<NS, NL>;
+  static constexpr int kChannels = S::CW * S::PITCH;
+  static constexpr int kWave = 4 * S::TILE + 3 * kChannels + 2 * 3 * 64 * NL;      // B, C and their gradients, d, d x, u, and the turns of what passes between waves
+  static constexpr int kWaveSet = 64 * (NL + 2);                                   // gradients of A, D, dt_bias
+  static constexpr int kSet = 2 * 64 * NL;                                         // what reaches the step behind, in two turns
+};
+
+// (read, added and written: an atomic addition in shared memory takes 200 cycles a wave)
+template <int NL>
+__device__ __forceinline__ void add_shared(float* p, const float (&v)[NL]) {
+  float sum[NL];
+  load_values<float, NL>(p, sum);
+#pragma unroll
+  for (int j = 0; j < NL; ++j) sum[j] += v[j];
+  store_values<float, NL>(p, sum);
+}
+
 template <typename T, int NS, int NL>
-__global__ __launch_bounds__(512) void selective_scan_bwd_kernel(ScanArgs p) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && NS > 4 ? 3 : 2))) void selective_scan_bwd_kernel(ScanArgs p) {
   static_assert(NS >= 2, "the sums over channels take up to five lane bits");
   using S = ScanShape<NS, NL>;
+  using Room = GradientRoom<NS, NL>;
   constexpr int CW = S::CW, NP = S::NP, TT = S::TT, NT = S::NT, PITCH = S::PITCH;
   constexpr int CBITS = log2_of(CW), LV = CBITS < 4 ? CBITS : 4;      // lane bits of channels; those that go with positions
-  constexpr int kWave = 2 * S::TILE + 3 * CW * PITCH;
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, W = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane / NS, q = lane % NS;
   const int id = xcd_order(blockIdx.x, gridDim.x), block = id % p.blocks, g = id / p.blocks % p.G, b = id / p.blocks / p.G;
-  const int count = min(CW, p.per_group - block * CW);
-  const bool on = c < count;
-  const int ch = g * p.per_group + block * CW + min(c, count - 1);
   const int n = scan_length(p, b), span = W * TT;
-  float* Bs = lds + w * kWave;
+  const int sets = min(p.sets, (p.per_group - block * p.sets * CW + CW - 1) / CW);
+  float* Bs = lds + w * Room::kWave;
   float* Cs = Bs + S::TILE;
-  float* ds = Cs + S::TILE;
-  float* xs = ds + CW * PITCH;
-  float* us = xs + CW * PITCH;
-  float* ex = lds + W * kWave;      // (2, W, 3, 64, NL)
-
-  float A[NL], R[NL], gA[NL];      // R: the gradient of the state behind the step, times the decay there
-#pragma unroll
-  for (int j = 0; j < NL; ++j) {
-    const int at = q * NL + j;
-    const bool real = on && at < p.N;
-    A[j] = real ? p.A[(long)ch * p.N + at] : 0.f;
-    R[j] = real && p.gstate_out ? p.gstate_out[((long)b * p.channels + ch) * p.N + at] : 0.f;
-    gA[j] = 0.f;
+  float* gBs = Cs + S::TILE;
+  float* gCs = gBs + S::TILE;
+  float* ds = gCs + S::TILE;
+  float* xs = ds + Room::kChannels;
+  float* us = xs + Room::kChannels;
+  float* ex = lds + W * (Room::kWave - 2 * 3 * 64 * NL);      // (2, W, 3, 64, NL), behind the waves' own
+  float* mine = lds + W * Room::kWave + w * p.sets * Room::kWaveSet;
+  float* carried = lds + W * (Room::kWave + p.sets * Room::kWaveSet);
+  // (the waves' own tiles lie one behind the other without the turns)
+  {
+    const int shift = w * 2 * 3 * 64 * NL;
+    Bs -= shift, Cs -= shift, gBs -= shift, gCs -= shift, ds -= shift, xs -= shift, us -= shift;
   }
-  const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.D ? p.D[ch] : 0.f;
-  const T* x = static_cast<const T*>(p.x) + b * p.x_batch + ch;
-  const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch + ch;
-  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_batch + ch : nullptr;
-  const T* gy = static_cast<const T*>(p.gy) + b * p.gy_batch + ch;
-  const T* Bm = static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group;
-  const T* Cm = static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group;
-  const long out_at = (long)b * p.L * p.channels + ch;
   const bool moves = NS <= TT || q < TT;
   const int q0 = NS <= TT ? q : min(q, TT - 1);
-  const long bc_at = (((long)block * p.batch + b) * p.L * p.G + g) * p.N, bc_row = (long)p.G * p.N;      // of partial gradients of B and C
+  const auto channel = [&](int set, bool& on) {
+    const int first = (block * p.sets + set) * CW, count = min(CW, p.per_group - first);
+    on = c < count;
+    return g * p.per_group + first + min(c, count - 1);
+  };
+
+  for (int i = lane; i < 2 * S::TILE; i += 64) gBs[i] = 0.f;
+  for (int i = lane; i < sets * Room::kWaveSet; i += 64) mine[i] = 0.f;
+  if (w == 0)
+    for (int set = 0; set < sets; ++set) {
+      bool on;
+      const int ch = channel(set, on);
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn)
+          carried[((set * 2 + turn) * 64 + lane) * NL + j] = on && q * NL + j < p.N && p.gstate_out ? p.gstate_out[((long)b * p.channels + ch) * p.N + q * NL + j] : 0.f;
+    }
+
+  const long out_at = (long)b * p.L * p.channels;
+  const int steps = (n + span - 1) / span;
+  const bool gated = p.z, soft = p.softplus, biased = p.dt_bias, skips = p.D;
+  const int N = p.N;
 
   T rx[NT], rdt[NT], rz[NT], rg[NT];
-  const auto load = [&](int t0) {
+  float rA[NL], rH[NL], rbias, rskip;
+  TileIn<T, NS, NL, S::AHEAD ? S::NB : 1> rb, rc;
+  const auto load = [&](int s, int set) {
+    ArgsInMemory& p = *arguments_anew();
+    bool on;
+    const int ch = channel(set, on), t0 = min(s * span + w * TT, n - 1), last = min(n - 1 - t0, TT - 1);
+    const auto rows = [&](T (&r)[NT], const void* tensor, long batch, long row) {
+      const T* base = static_cast<const T*>(tensor) + b * batch + t0 * row;
+      const Near off = Near::of(base, q0, row, ch, last);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int t = min(t0 + q0 + i * NS, n - 1);
-      rx[i] = x[t * p.x_row], rdt[i] = dt[t * p.dt_row], rg[i] = gy[t * p.gy_row];
-      if (z) rz[i] = z[t * p.z_row];
-    }
-  };
-  const int steps = (n + span - 1) / span;
-  if (steps > 0) load((steps - 1) * span + w * TT);
-  float gD = 0.f, gbias = 0.f;
-  for (int s = steps - 1; s >= 0; --s) {
-    const int t0 = s * span + w * TT;
-    float H[NL];
+      for (int i = 0; i < NT; ++i) r[i] = at_offset<const T>(base, off((uint32_t)(i * NS * sizeof(T)) * (uint32_t)row));
+    };
+    rows(rx, p.x, p.x_batch, p.x_row);
+    rows(rdt, p.dt, p.dt_batch, p.dt_row);
+    rows(rg, p.gy, p.gy_batch, p.gy_row);
+    rows(rz, p.z ? p.z : p.x, p.z ? p.z_batch : p.x_batch, p.z ? p.z_row : p.x_row);      // (no gate: loads that nothing comes of, rather than waits around a branch)
+    const float* kept = p.saved + ((long)b * p.parts + s * p.kept_parts) * p.channels * p.N;
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const int at = q * NL + j;
-      H[j] = on && at < p.N ? p.saved[(((long)b * p.parts + s) * p.channels + ch) * p.N + at] : 0.f;
+      const uint32_t at = (uint32_t)(ch * p.N + min(q * NL + j, p.N - 1)) * 4u;
+      rA[j] = at_offset<const float>(p.A, at), rH[j] = at_offset<const float>(kept, at);
     }
-    float xv[NT], raw[NT], own_d[NT], zv[NT], gv[NT], u[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const bool inside = on && t0 + q0 + i * NS < n;
-      raw[i] = value_of<T>(rdt[i]) + bias;
-      own_d[i] = inside ? (p.softplus ? softplus(raw[i]) : raw[i]) : 0.f;
-      xv[i] = inside ? value_of<T>(rx[i]) : 0.f;
-      gv[i] = inside ? value_of<T>(rg[i]) : 0.f;
-      zv[i] = z && inside ? value_of<T>(rz[i]) : 0.f;
-      u[i] = z ? gv[i] * silu(zv[i]) : gv[i];
-    }
+    // (without a bias or D: a value that is not used)
+    rbias = at_offset<const float>(p.dt_bias ? p.dt_bias : p.A, (uint32_t)ch * 4u);
+    rskip = at_offset<const float>(p.D ? p.D : p.A, (uint32_t)ch * 4u);
+  };
+  const auto load_tiles = [&](int s) {
+    ArgsInMemory& p = *arguments_anew();
+    const int t0 = min(s * span + w * TT, n - 1);
+    rb.load(static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group, p.b_row, t0, n, p.N, lane);
+    rc.load(static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group, p.c_row, t0, n, p.N, lane);
+  };
+  if (steps > 0) {
+    load(steps - 1, 0);
+    if constexpr (S::AHEAD) load_tiles(steps - 1);
+  }
+  __syncthreads();
+  int turn = 0;
+  for (int s = steps - 1; s >= 0; --s) {
+    const int t0 = s * span + w * TT;
     wave_sync();      // the tiles have been read
-    tile_in<T, NS, NL>(Bs, Bm, p.b_row, t0, n, p.N, lane);
-    tile_in<T, NS, NL>(Cs, Cm, p.c_row, t0, n, p.N, lane);
+    if constexpr (S::AHEAD) {
+      rb.put(Bs, N, lane);
+      rc.put(Cs, N, lane);
+      load_tiles(max(s - 1, 0));
+    } else {
+      ArgsInMemory& p = *arguments_anew();
+      tile_in<T, NS, NL>(Bs, static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group, p.b_row, min(t0, n - 1), n, p.N, lane);
+      tile_in<T, NS, NL>(Cs, static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group, p.c_row, min(t0, n - 1), n, p.N, lane);
+    }
+    for (int set = 0; set < sets; ++set, turn ^= 1) {
+      bool on;
+      const int ch = channel(set, on);
+      float A[NL], start[NL], xv[NT], d[NT], d_slope[NT], gv[NT], u[NT], gz[NT], own_total = 0.f;
+      float skip = skips ? rskip : 0.f;
+      const float bias = biased ? rbias : 0.f;
+      made_here(skip);
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      if (moves) ds[c * PITCH + q0 + i * NS] = own_d[i], xs[c * PITCH + q0 + i * NS] = own_d[i] * xv[i], us[c * PITCH + q0 + i * NS] = u[i];
-    wave_sync();
-    if (s > 0) load(t0 - span);
-    float a[TT][NL], h[TT][NL], last[NL], left[NL], total = 0.f;
+      for (int j = 0; j < NL; ++j) {
+        const bool real = on && q * NL + j < N;
+        A[j] = real ? rA[j] : 0.f, start[j] = real ? rH[j] : 0.f;
+        made_here(A[j]), made_here(start[j]);
+      }
 #pragma unroll
-    for (int j = 0; j < NL; ++j) last[j] = left[j] = 0.f;
+      for (int i = 0; i < NT; ++i) {
+        const bool inside = on && t0 + q0 + i * NS < n;
+        const float raw = value_of<T>(rdt[i]) + bias;
+        d[i] = raw, d_slope[i] = inside ? 1.f : 0.f;
+        if (soft) {
+          const Logistic l(raw);
+          d[i] = softplus_of(raw, l.u);
+          d_slope[i] = inside ? l.value() : 0.f;
+        }
+        d[i] = inside ? d[i] : 0.f;
+        xv[i] = inside ? value_of<T>(rx[i]) : 0.f;
+        gv[i] = inside ? value_of<T>(rg[i]) : 0.f;
+        u[i] = gv[i], gz[i] = 0.f;
+        if (gated) {
+          const float zv = inside ? value_of<T>(rz[i]) : 0.f;
+          const Logistic l(zv);
+          u[i] = gv[i] * (zv * l.value());
+          gz[i] = gv[i] * silu_slope_of(zv, l);
+        }
+        made_here(xv[i]), made_here(d[i]), made_here(d_slope[i]), made_here(u[i]), made_here(gz[i]);
+        own_total += moves ? d[i] : 0.f;
+        if (moves) ds[c * PITCH + q0 + i * NS] = d[i], xs[c * PITCH + q0 + i * NS] = d[i] * xv[i], us[c * PITCH + q0 + i * NS] = u[i];
+      }
+      wave_sync();
+      load(set + 1 < sets ? s : max(s - 1, 0), set + 1 < sets ? set + 1 : 0);      // (the very last for nothing)
+      const float total = lane_sum<NS>(own_total, lane);
+      float a[TT][NL], h[TT][NL], last[NL], left[NL], A2[NL];
 #pragma unroll
-    for (int t4 = 0; t4 < TT; t4 += 4) {
-      float d4[4], x4[4];
-      load_values<float, 4>(ds + c * PITCH + t4, d4);
-      load_values<float, 4>(xs + c * PITCH + t4, x4);
+      for (int j = 0; j < NL; ++j) last[j] = left[j] = 0.f, A2[j] = A[j] * kLog2E;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t4 + i;
-        float bn[NL];
-        load_values<float, NL>(Bs + t * NP + q * NL, bn);
-        total += d4[i];
+      for (int t4 = 0; t4 < TT; t4 += 4) {
+        keep_order();
+        float d4[4], x4[4];
+        load_values<float, 4>(ds + c * PITCH + t4, d4);
+        load_values<float, 4>(xs + c * PITCH + t4, x4);
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          a[t][j] = __builtin_amdgcn_exp2f(d4[i] * (A[j] * kLog2E));
-          h[t][j] = x4[i] * bn[j];      // (for now what the position puts in)
-          last[j] = fmaf(a[t][j], last[j], h[t][j]);
+        for (int i = 0; i < 4; ++i) {
+          const int t = t4 + i;
+          float bn[NL];
+          load_values<float, NL>(Bs + t * NP + q * NL, bn);
+#pragma unroll
+          for (int j = 0; j < NL; ++j) {
+            a[t][j] = __builtin_amdgcn_exp2f(d4[i] * A2[j]);
+            h[t][j] = x4[i] * bn[j];      // (for now what the position puts in)
+            last[j] = fmaf(a[t][j], last[j], h[t][j]);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int t4 = TT - 4; t4 >= 0; t4 -= 4) {
-      float u4[4];
-      load_values<float, 4>(us + c * PITCH + t4, u4);
+      for (int t4 = TT - 4; t4 >= 0; t4 -= 4) {
+        keep_order();
+        float u4[4];
+        load_values<float, 4>(us + c * PITCH + t4, u4);
 #pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        float cn[NL];
-        load_values<float, NL>(Cs + (t4 + i) * NP + q * NL, cn);
+        for (int i = 3; i >= 0; --i) {
+          float cn[NL];
+          load_values<float, NL>(Cs + (t4 + i) * NP + q * NL, cn);
 #pragma unroll
-        for (int j = 0; j < NL; ++j) left[j] = fmaf(cn[j], u4[i], left[j]) * a[t4 + i][j];
+          for (int j = 0; j < NL; ++j) left[j] = fmaf(cn[j], u4[i], left[j]) * a[t4 + i][j];
+        }
       }
-    }
-    // what the waves before and behind do to a state and to its gradient
-    float P[NL], start[NL], right[NL];
+      // what the waves before and behind do to a state and to its gradient
+      float P[NL], right[NL], R[NL];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * (A[j] * kLog2E)), start[j] = H[j], right[j] = R[j];
-    float* turn = ex + (s & 1) * W * 3 * 64 * NL;
-    store_values<float, NL>(turn + (w * 3 * 64 + lane) * NL, P);
-    store_values<float, NL>(turn + ((w * 3 + 1) * 64 + lane) * NL, last);
-    store_values<float, NL>(turn + ((w * 3 + 2) * 64 + lane) * NL, left);
-    __syncthreads();      // (two turns: what is written next is read behind the next barrier)
-    for (int o = 0; o < w; ++o) {
-      float po[NL], ho[NL];
-      load_values<float, NL>(turn + (o * 3 * 64 + lane) * NL, po);
-      load_values<float, NL>(turn + ((o * 3 + 1) * 64 + lane) * NL, ho);
+      for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * A2[j]);
+      float* now = ex + turn * W * 3 * 64 * NL;
+      store_values<float, NL>(now + (w * 3 * 64 + lane) * NL, P);
+      store_values<float, NL>(now + ((w * 3 + 1) * 64 + lane) * NL, last);
+      store_values<float, NL>(now + ((w * 3 + 2) * 64 + lane) * NL, left);
+      __syncthreads();      // (two turns: what is written next is read behind the next barrier)
+      load_values<float, NL>(carried + ((set * 2 + (s & 1)) * 64 + lane) * NL, R);
+      for (int o = 0; o < w; ++o) {
+        float po[NL], ho[NL];
+        load_values<float, NL>(now + (o * 3 * 64 + lane) * NL, po);
+        load_values<float, NL>(now + ((o * 3 + 1) * 64 + lane) * NL, ho);
 #pragma unroll
-      for (int j = 0; j < NL; ++j) start[j] = fmaf(po[j], start[j], ho[j]);
-    }
-    for (int o = W - 1; o >= 0; --o) {
-      if (o == w) {
-#pragma unroll
-        for (int j = 0; j < NL; ++j) right[j] = R[j];
+        for (int j = 0; j < NL; ++j) start[j] = fmaf(po[j], start[j], ho[j]);
       }
-      float po[NL], lo[NL];
-      load_values<float, NL>(turn + (o * 3 * 64 + lane) * NL, po);
-      load_values<float, NL>(turn + ((o * 3 + 2) * 64 + lane) * NL, lo);
+      const auto meet = [&](int o) {
+        float po[NL], lo[NL];
+        load_values<float, NL>(now + (o * 3 * 64 + lane) * NL, po);
+        load_values<float, NL>(now + ((o * 3 + 2) * 64 + lane) * NL, lo);
 #pragma unroll
-      for (int j = 0; j < NL; ++j) R[j] = fmaf(po[j], R[j], lo[j]);
-    }
-    // the states, and the outputs where a gate asks for them
-    float out[TT];
-    {
-      float run[NL];
+        for (int j = 0; j < NL; ++j) R[j] = fmaf(po[j], R[j], lo[j]);
+      };
+      for (int o = W - 1; o > w; --o) meet(o);
 #pragma unroll
-      for (int j = 0; j < NL; ++j) run[j] = start[j];
+      for (int j = 0; j < NL; ++j) right[j] = R[j];
+      if (w == 0) {      // the first wave has met all others
+        meet(0);
+        store_values<float, NL>(carried + ((set * 2 + (~s & 1)) * 64 + lane) * NL, R);
+      }
+      // the states
+      {
+        float run[NL];
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
+        for (int j = 0; j < NL; ++j) run[j] = start[j];
 #pragma unroll
-        for (int j = 0; j < NL; ++j) h[t][j] = run[j] = fmaf(a[t][j], run[j], h[t][j]);
-    }
-    if (z) {
+        for (int t = 0; t < TT; ++t)
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        float cn[NL];
+          for (int j = 0; j < NL; ++j) h[t][j] = run[j] = fmaf(a[t][j], run[j], h[t][j]);
+      }
+      // sum_n dh B, sum_n dh a h A, sum_n C h of the lane's positions
+      constexpr int QV = log2_of(NS) < 4 ? log2_of(NS) : 4;
+      float into[NT], kept[NT], out[NT], gA[NL];
+#pragma unroll
+      for (int j = 0; j < NL; ++j) gA[j] = 0.f;
+      Tree<LV, NL, 5, -1> tb, tc;
+      Tree<QV, 3, 0, 1> tq;
+      float d4[4], x4[4], u4[4];
+      count_down<TT - 1, 0>([&](auto tt) {
+        constexpr int t = decltype(tt)::value;
+        if constexpr (t % 4 == 3) {
+          keep_order();
+          load_values<float, 4>(ds + c * PITCH + t - 3, d4);
+          load_values<float, 4>(xs + c * PITCH + t - 3, x4);
+          load_values<float, 4>(us + c * PITCH + t - 3, u4);
+        }
+        float bn[NL], cn[NL], vb[NL], vc[NL], vq[3];
+        load_values<float, NL>(Bs + t * NP + q * NL, bn);
         load_values<float, NL>(Cs + t * NP + q * NL, cn);
-        out[t] = cn[0] * h[t][0];
 #pragma unroll
-        for (int j = 1; j < NL; ++j) out[t] = fmaf(cn[j], h[t][j], out[t]);
+        for (int j = 0; j < NL; ++j) {
+          const float dh = fmaf(cn[j], u4[t % 4], right[j]);
+          vb[j] = dh * x4[t % 4];
+          vc[j] = u4[t % 4] * h[t][j];
+          right[j] = dh * a[t][j];
+          const float k = right[j] * (t > 0 ? h[t > 0 ? t - 1 : 0][j] : start[j]);
+          vq[0] = j == 0 ? dh * bn[j] : fmaf(dh, bn[j], vq[0]);
+          vq[1] = j == 0 ? k * A[j] : fmaf(k, A[j], vq[1]);
+          vq[2] = j == 0 ? cn[j] * h[t][j] : fmaf(cn[j], h[t][j], vq[2]);
+          gA[j] = fmaf(d4[t % 4], k, gA[j]);
+        }
+        tq.template add<t % (1 << QV)>(vq, lane);
+        if constexpr (t % (1 << QV) == 0) {
+          if constexpr (NS > 16) {      // (lanes beyond the positions)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              vq[k] = sum_over_bit<4>(vq[k], lane);
+              if constexpr (NS > 32) vq[k] = sum_over_bit<5>(vq[k], lane);
+            }
+          }
+          into[t >> QV] = vq[0], kept[t >> QV] = vq[1], out[t >> QV] = vq[2];
+        }
+        tb.template add<t % (1 << LV)>(vb, lane);
+        tc.template add<t % (1 << LV)>(vc, lane);
+        if constexpr (t % (1 << LV) == 0) {
+          // (two lanes a channel: the fifth bit of the channels)
+          if constexpr (CBITS > 4) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) vb[j] = sum_over_bit<1>(vb[j], lane), vc[j] = sum_over_bit<1>(vc[j], lane);
+          }
+          int at = t;
+#pragma unroll
+          for (int k = 0; k < LV; ++k) at += ((lane >> (5 - k)) & 1) << k;
+          if (CBITS <= 4 || (lane & 3) < NS) add_shared<NL>(gBs + at * NP + q * NL, vb), add_shared<NL>(gCs + at * NP + q * NL, vc);
+        }
+      });
+      float gD = 0.f, gbias = 0.f;
+      ArgsInMemory& p = *arguments_anew();
+      T* gx = static_cast<T*>(p.gx) + out_at + (long)t0 * p.channels;
+      T* gdt = static_cast<T*>(p.gdt) + out_at + (long)t0 * p.channels;
+      T* gzs = static_cast<T*>(p.gz) + out_at + (long)t0 * p.channels;
+      const uint32_t off = (uint32_t)(q0 * p.channels + ch) * sizeof(T);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int t = t0 + i * NS;
+        const float gxv = fmaf(d[i], into[i], skip * u[i]), gd = fmaf(xv[i], into[i], kept[i]) * d_slope[i];
+        gD = fmaf(u[i], xv[i], gD);
+        gbias += gd;
+        const bool inside = t + q0 < n;
+        if (on && moves && t + q0 < p.L) {
+          const uint32_t at = off + (uint32_t)(i * NS * sizeof(T)) * (uint32_t)p.channels;
+          if (p.gx) at_offset<T>(gx, at) = value_to<T>(inside ? gxv : 0.f);
+          if (p.gdt) at_offset<T>(gdt, at) = value_to<T>(inside ? gd : 0.f);
+          if (p.gz) at_offset<T>(gzs, at) = value_to<T>(inside ? gz[i] * fmaf(skip, xv[i], out[i]) : 0.f);
+        }
       }
-      share_positions<NS, 0>(out, lane);
+      float* sums = mine + set * Room::kWaveSet + lane;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) sums[j * 64] += gA[j];
+      sums[NL * 64] += moves ? gD : 0.f;
+      sums[(NL + 1) * 64] += moves ? gbias : 0.f;
+      wave_sync();      // positions' values have been read
+    }
+    // the workgroup's part of B's and C's gradients
+    ArgsInMemory& p = *arguments_anew();
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float* sums = which ? gCs : gBs;
+      float* out = (which ? p.c_part : p.b_part) + ((((long)block * p.batch + b) * p.L + t0) * p.G + g) * p.N;
+      for (int i = lane; i < S::TILE; i += 64) {
+        const int t = i / NP, at = i % NP;
+        if (t0 + t < n && at < p.N) out[(long)t * p.G * p.N + at] = sums[i];
+        sums[i] = 0.f;
+      }
+    }
+  }
+  for (int set = 0; set < sets; ++set) {
+    bool on;
+    const int ch = channel(set, on);
+    for (int t0 = steps * span + w * TT; t0 < p.L; t0 += span)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int t = t0 + q0 + i * NS;
-        if (p.gz && on && moves && t < p.L) static_cast<T*>(p.gz)[out_at + (long)t * p.channels] = value_to<T>(gv[i] * fmaf(skip, xv[i], out[i]) * silu_slope(zv[i]));
-      }
-    }
-    float into[TT];      // sum_n dh B; out: sum_n dh a h A
-    Tree<LV, NL> tb, tc;
-    count_down<TT - 1, 0>([&](auto tt) {
-      constexpr int t = decltype(tt)::value;
-      const float d = ds[c * PITCH + t], dx = xs[c * PITCH + t], ut = us[c * PITCH + t];
-      float bn[NL], cn[NL], vb[NL], vc[NL];
-      load_values<float, NL>(Bs + t * NP + q * NL, bn);
-      load_values<float, NL>(Cs + t * NP + q * NL, cn);
-      into[t] = out[t] = 0.f;
-#pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const float dh = fmaf(cn[j], ut, right[j]);
-        vb[j] = dh * dx;
-        vc[j] = ut * h[t][j];
-        into[t] = fmaf(dh, bn[j], into[t]);
-        right[j] = dh * a[t][j];
-        const float k = right[j] * (t > 0 ? h[t > 0 ? t - 1 : 0][j] : start[j]);
-        out[t] = fmaf(k, A[j], out[t]);
-        gA[j] = fmaf(d, k, gA[j]);
-      }
-      tb.template add<t % (1 << LV)>(vb, lane);
-      tc.template add<t % (1 << LV)>(vc, lane);
-      if constexpr (t % (1 << LV) == 0) {
-        // (two lanes a channel: the fifth bit of the channels)
-        if constexpr (CBITS > 4) {
-#pragma unroll
-          for (int j = 0; j < NL; ++j) vb[j] = sum_over_bit<1>(vb[j], lane), vc[j] = sum_over_bit<1>(vc[j], lane);
-        }
-        int mine = t0 + t;
-#pragma unroll
-        for (int k = 0; k < LV; ++k) mine += ((lane >> (5 - k)) & 1) << k;
-        if (mine < n && (CBITS <= 4 || (lane & 3) < NS)) {
-          const long at = bc_at + mine * bc_row + q * NL;
-#pragma unroll
-          for (int j = 0; j < NL; ++j)
-            if (q * NL + j < p.N) p.b_part[at + j] = vb[j], p.c_part[at + j] = vc[j];
+        const long at = out_at + (long)t * p.channels + ch;
+        if (on && moves && t < p.L) {
+          if (p.gx) static_cast<T*>(p.gx)[at] = value_to<T>(0.f);
+          if (p.gdt) static_cast<T*>(p.gdt)[at] = value_to<T>(0.f);
+          if (p.gz) static_cast<T*>(p.gz)[at] = value_to<T>(0.f);
         }
       }
-    });
-    share_positions<NS, 0>(into, lane);
-    share_positions<NS, 0>(out, lane);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int t = t0 + q0 + i * NS;
-      const bool inside = t < n;
-      const float gx = fmaf(own_d[i], into[i], skip * u[i]);
-      float gd = fmaf(xv[i], into[i], out[i]);
-      if (p.softplus) gd *= sigmoid(raw[i]);
-      if (!inside) gd = 0.f;
-      if (on && moves) {
-        gD = fmaf(u[i], xv[i], gD);
-        gbias += gd;
-        if (t < p.L) {
-          if (p.gx) static_cast<T*>(p.gx)[out_at + (long)t * p.channels] = value_to<T>(inside ? gx : 0.f);
-          if (p.gdt) static_cast<T*>(p.gdt)[out_at + (long)t * p.channels] = value_to<T>(gd);
-        }
-      }
-    }
   }
-  for (int t0 = steps * span + w * TT; t0 < p.L; t0 += span)
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int t = t0 + q0 + i * NS;
-      if (on && moves && t < p.L) {
-        if (p.gx) static_cast<T*>(p.gx)[out_at + (long)t * p.channels] = value_to<T>(0.f);
-        if (p.gdt) static_cast<T*>(p.gdt)[out_at + (long)t * p.channels] = value_to<T>(0.f);
-        if (p.gz) static_cast<T*>(p.gz)[out_at + (long)t * p.channels] = value_to<T>(0.f);
-      }
-    }
-  // over a channel's lanes, then over the waves
-  gD = lane_sum<NS>(gD, lane);
-  gbias = lane_sum<NS>(gbias, lane);
+  // over the waves, and over a channel's lanes
   __syncthreads();
-  store_values<float, NL>(lds + (w * 64 + lane) * NL, gA);
-  float* more = lds + W * 64 * NL;
-  if (q == 0) more[w * 64 + c] = gD, more[(W + w) * 64 + c] = gbias;
-  __syncthreads();
-  if (w > 0 || !on) return;
-  for (int o = 1; o < W; ++o) {
-    float v[NL];
-    load_values<float, NL>(lds + (o * 64 + lane) * NL, v);
+  for (int set = w; set < sets; set += W) {
+    bool on;
+    const int ch = channel(set, on);
+    float sums[NL + 2];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) gA[j] += v[j];
-    gD += more[o * 64 + c], gbias += more[(W + o) * 64 + c];
-  }
-#pragma unroll
-  for (int j = 0; j < NL; ++j) {
-    const long at = ((long)b * p.channels + ch) * p.N + q * NL + j;
-    if (q * NL + j < p.N) {
-      p.a_part[at] = gA[j];
-      if (p.gstate) p.gstate[at] = R[j];
+    for (int j = 0; j < NL + 2; ++j) {
+      sums[j] = 0.f;
+      for (int o = 0; o < W; ++o) sums[j] += lds[W * Room::kWave + (o * p.sets + set) * Room::kWaveSet + j * 64 + lane];
     }
+    const float gD = lane_sum<NS>(sums[NL], lane), gbias = lane_sum<NS>(sums[NL + 1], lane);
+    if (!on) continue;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const long at = ((long)b * p.channels + ch) * p.N + q * NL + j;
+      if (q * NL + j >= p.N) continue;
+      p.a_part[at] = sums[j];
+      if (p.gstate) p.gstate[at] = carried[((set * 2 + 1) * 64 + lane) * NL + j];      // (behind step 0)
+    }
+    if (q == 0) p.d_part[(long)b * p.channels + ch] = gD, p.bias_part[(long)b * p.channels + ch] = gbias;
   }
-  if (q == 0) p.d_part[(long)b * p.channels + ch] = gD, p.bias_part[(long)b * p.channels + ch] = gbias;
+}
+
+size_t scan_bwd_lds(const ScanPlan& plan) {
+  size_t bytes = 0;
+  with_scan_shape<GradientShapes>(plan.NS, plan.NL, [&](auto ns, auto nl) {
+    using Room = GradientRoom<decltype(ns)::value, decltype(nl)::value>;
+    bytes = sizeof(float) * (plan.W * (Room::kWave + plan.sets * Room::kWaveSet) + plan.sets * Room::kSet);
+  });
+  return bytes;
 }
 
 int scan_bwd(const ScanArgs& p, const ScanPlan& plan, int dtype, hipStream_t stream) {
   const unsigned grid = (unsigned)((long)plan.blocks * p.G * p.batch);
-  const int CW = 64 / plan.NS, floats = plan.W * (2 * 16 * plan.NS * plan.NL + 3 * CW * 20 + 2 * 3 * 64 * plan.NL);
-  const size_t lds = sizeof(float) * (size_t)floats;
+  const size_t lds = scan_bwd_lds(plan);
   int rc = M2_OK;
   with_scan_shape<GradientShapes>(plan.NS, plan.NL, [&](auto ns, auto nl) {
     const auto launch = [&](auto t) {

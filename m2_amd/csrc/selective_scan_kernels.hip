@@ -19,7 +19,7 @@
 namespace m2 {
 
 template <typename T, int NS, int NL>
-__global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && NS > 1 ? 3 : 2))) void selective_scan_kernel(ScanArgs p) {
   using S = ScanShape<NS, NL>;
   constexpr int CW = S::CW, NP = S::NP, TT = S::TT, NT = S::NT, PITCH = S::PITCH;
   constexpr int kWave = 2 * S::TILE + (NS > 1 ? 2 * CW * PITCH : 0);      // floats
@@ -46,24 +46,29 @@ __global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
     H[j] = real && p.state ? p.state[((long)b * p.channels + ch) * p.N + at] : 0.f;
   }
   const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.D ? p.D[ch] : 0.f;
-  const T* x = static_cast<const T*>(p.x) + b * p.x_batch + ch;
-  const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch + ch;
-  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_batch + ch : nullptr;
+  const T* x = static_cast<const T*>(p.x) + b * p.x_batch;
+  const T* dt = static_cast<const T*>(p.dt) + b * p.dt_batch;
+  const T* z = p.z ? static_cast<const T*>(p.z) + b * p.z_batch : x;      // (no gate: loads that nothing comes of, rather than waits around a branch)
+  const long z_row = p.z ? p.z_row : p.x_row;
   const T* Bm = static_cast<const T*>(p.Bm) + b * p.b_batch + g * p.b_group;
   const T* Cm = static_cast<const T*>(p.Cm) + b * p.c_batch + g * p.c_group;
-  T* y = static_cast<T*>(p.y) + (long)b * p.L * p.channels + ch;
+  T* y = static_cast<T*>(p.y) + (long)b * p.L * p.channels;
   // a lane moves positions q, q + NS, ... of its channel (lanes beyond the 16th of a channel none)
   const bool moves = NS <= TT || q < TT;
   const int q0 = NS <= TT ? q : min(q, TT - 1);
 
+  const uint32_t y_off = (uint32_t)(q0 * p.channels + ch) * sizeof(T);
   T rx[NT], rdt[NT], rz[NT];
   TileIn<T, NS, NL, S::AHEAD ? S::NB : 1> rb, rc;      // where they fit into registers, a step's tiles are asked for ahead
   const auto load = [&](int t0) {
+    t0 = min(t0, n - 1);      // (a wave whose positions all lie behind the end)
+    const int last = min(n - 1 - t0, TT - 1);
+    const Near x_off = Near::of(x, q0, p.x_row, ch, last), dt_off = Near::of(dt, q0, p.dt_row, ch, last), z_off = Near::of(z, q0, z_row, ch, last);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int t = min(t0 + q0 + i * NS, n - 1);
-      rx[i] = x[t * p.x_row], rdt[i] = dt[t * p.dt_row];
-      if (z) rz[i] = z[t * p.z_row];
+      const uint32_t t = i * NS * sizeof(T);
+      rx[i] = at_offset<const T>(x + t0 * p.x_row, x_off(t * (uint32_t)p.x_row)), rdt[i] = at_offset<const T>(dt + t0 * p.dt_row, dt_off(t * (uint32_t)p.dt_row));
+      rz[i] = at_offset<const T>(z + t0 * z_row, z_off(t * (uint32_t)z_row));
     }
     if constexpr (S::AHEAD) {
       rb.load(Bm, p.b_row, t0, n, p.N, lane);
@@ -83,15 +88,15 @@ __global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
       if (p.softplus) d = softplus(d);
       own_d[i] = inside ? d : 0.f;
       xv[i] = inside ? xv[i] : 0.f;
-      gate[i] = z ? silu(value_of<T>(rz[i])) : 1.f;
+      gate[i] = p.z ? silu(value_of<T>(rz[i])) : 1.f;
     }
     wave_sync();      // the tiles have been read
     if constexpr (S::AHEAD) {
-      rb.put(Bs, lane);
-      rc.put(Cs, lane);
+      rb.put(Bs, p.N, lane);
+      rc.put(Cs, p.N, lane);
     } else {
-      tile_in<T, NS, NL>(Bs, Bm, p.b_row, t0, n, p.N, lane);
-      tile_in<T, NS, NL>(Cs, Cm, p.c_row, t0, n, p.N, lane);
+      tile_in<T, NS, NL>(Bs, Bm, p.b_row, min(t0, n - 1), n, p.N, lane);
+      tile_in<T, NS, NL>(Cs, Cm, p.c_row, min(t0, n - 1), n, p.N, lane);
     }
     if constexpr (NS > 1) {
 #pragma unroll
@@ -130,11 +135,7 @@ __global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
     float P[NL], start[NL];
 #pragma unroll
     for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * A2[j]);
-    if (p.saved && w == 0 && on) {
-#pragma unroll
-      for (int j = 0; j < NL; ++j)
-        if (q * NL + j < p.N) p.saved[(((long)b * p.parts + s) * p.channels + ch) * p.N + q * NL + j] = H[j];
-    }
+
     if (W == 1) {
 #pragma unroll
       for (int j = 0; j < NL; ++j) start[j] = H[j], H[j] = fmaf(P[j], H[j], h[j]);
@@ -143,17 +144,23 @@ __global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
       store_values<float, NL>(turn + (w * 2 * 64 + lane) * NL, P);
       store_values<float, NL>(turn + ((w * 2 + 1) * 64 + lane) * NL, h);
       __syncthreads();      // (two turns: what is written next is read behind the next barrier)
-      for (int o = 0; o < W; ++o) {
-        if (o == w) {
-#pragma unroll
-          for (int j = 0; j < NL; ++j) start[j] = H[j];
-        }
+      const auto meet = [&](int o) {
         float po[NL], ho[NL];
         load_values<float, NL>(turn + (o * 2 * 64 + lane) * NL, po);
         load_values<float, NL>(turn + ((o * 2 + 1) * 64 + lane) * NL, ho);
 #pragma unroll
         for (int j = 0; j < NL; ++j) H[j] = fmaf(po[j], H[j], ho[j]);
-      }
+      };
+      for (int o = 0; o < w; ++o) meet(o);
+#pragma unroll
+      for (int j = 0; j < NL; ++j) start[j] = H[j];
+      for (int o = w; o < W; ++o) meet(o);
+    }
+    if (p.saved && t0 % p.apart == 0 && t0 < n && on) {
+      float* kept = p.saved + (((long)b * p.parts + t0 / p.apart) * p.channels + ch) * p.N + q * NL;
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+        if (q * NL + j < p.N) kept[j] = start[j];
     }
     float out[TT];
 #pragma unroll
@@ -169,18 +176,25 @@ __global__ __launch_bounds__(512) void selective_scan_kernel(ScanArgs p) {
       out[t] = sum;
     }
     share_positions<NS, log2_of(CW)>(out, lane);
+    if (t0 + TT <= n) {
+      if (on && moves) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int t = t0 + q0 + i * NS;
-      const float v = fmaf(skip, xv[i], out[i]) * gate[i];
-      if (on && moves && t < p.L) y[(long)t * p.channels] = value_to<T>(t < n ? v : 0.f);
+        for (int i = 0; i < NT; ++i) at_offset<T>(y + (long)(t0 + i * NS) * p.channels, y_off) = value_to<T>(fmaf(skip, xv[i], out[i]) * gate[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int t = t0 + q0 + i * NS;
+        const float v = fmaf(skip, xv[i], out[i]) * gate[i];
+        if (on && moves && t < p.L) y[(long)t * p.channels + ch] = value_to<T>(t < n ? v : 0.f);
+      }
     }
   }
   for (int t0 = steps * span + w * TT; t0 < p.L; t0 += span)
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int t = t0 + q0 + i * NS;
-      if (on && moves && t < p.L) y[(long)t * p.channels] = value_to<T>(0.f);
+      if (on && moves && t < p.L) y[(long)t * p.channels + ch] = value_to<T>(0.f);
     }
   if (p.state_out && w == 0 && on) {
 #pragma unroll
@@ -238,6 +252,8 @@ int check_scan(const char* name, const ScanArgs& p, int dtype) {
   if (p.batch < 1 || p.L < 1 || p.channels < 1 || p.G < 1 || p.channels % p.G) return set_error(M2_ERR_ARG, "%s: B=%d, L=%d, D=%d, G=%d", name, p.batch, p.L, p.channels, p.G);
   if (p.N < 1 || p.N > kMaxStates) return set_error(M2_ERR_UNSUPPORTED, "%s: N=%d states, 1 .. %d are supported", name, p.N, kMaxStates);
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype %d", name, dtype);
+  for (long row : {p.x_row, p.dt_row, p.z_row, p.b_row, p.c_row, p.gy_row})
+    if (row < 0 || row >= 1L << 24) return set_error(M2_ERR_UNSUPPORTED, "%s: rows %ld values apart, below 2^24 are supported", name, row);
   if ((long)p.batch * p.L > (1L << 36) / ((long)p.G * p.N)) return set_error(M2_ERR_ARG, "%s: at most 2^36 values of B", name);
   if (p.channels > 1 << 20 || p.L > 1 << 30 || (long)p.batch * p.channels > 1L << 24)
     return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^24 channels of all sequences", name);
@@ -260,32 +276,51 @@ size_t fwd_lds(const ScanPlan& s) {
   return sizeof(float) * s.W * (2 * 16 * s.NS * s.NL + (s.NS > 1 ? 2 * CW * 20 : 0) + (s.W > 1 ? 2 * 2 * 64 * s.NL : 0));
 }
 
-// The first of the numbers of states a lane that is built, one where the workgroups would leave compute units without.
+// Lanes a channel and states a lane.  A wave's sixteen positions cost some 150 instructions for each state of a lane (a product, an exponential at four times the cost of others, a product,
+// three sums), 45 for each position whose x, dt, z and y it moves, a sum across lanes, and 60 for what all waves do; four states a lane leave room for two waves a SIMD instead of
+// three (8 % more).  What counts is the share of the compute unit with most workgroups.  16 states, us, with four / two / one a lane: 1 x 8192 x 1536 225 / 154 / 162 (96, 192,
+// 384 workgroups), 4 x 8192 x 1536 424 / 374 / 532 (384, 768, 1536); 61 states, 5 x 1013 x 1002 143 / 171 / 240.
 template <typename SHAPES>
 void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
-  const int per_group = D / G;
+  const int per_group = D / G, cus = num_cus();
+  double least = 0;
   for (int NL : {4, 2, 1}) {
     const int NS = std::max(pow2_from((N + NL - 1) / NL), SHAPES::built(1, 1) ? 1 : 2);
-    if (NS > 64) break;
-    if (!SHAPES::built(NS, NL)) continue;
-    const int CW = 64 / NS;
-    r.NS = NS, r.NL = NL, r.blocks = (per_group + CW - 1) / CW;
-    if ((long)r.blocks * G * B >= num_cus()) break;
+    if (NS > 64 || !SHAPES::built(NS, NL)) continue;
+    const int CW = 64 / NS, blocks = (per_group + CW - 1) / CW;
+    const long share = ((long)blocks * G * B + cus - 1) / cus;
+    const double cost = (150 * NL + 45 * std::max(16 / NS, 1) + 2.5 * (16 - 16 / std::min(NS, 16)) + 60) * (NL == 4 ? 1.08 : 1.0) * share;
+    if (least == 0 || cost < least) least = cost, r.NS = NS, r.NL = NL, r.blocks = blocks;
   }
 }
-// Waves as many as there are positions for, up to eight; as the gradient's where the states ahead of each step are kept for it.
-ScanPlan fwd_plan(int B, int L, int D, int G, int N, bool saved) {
+// Waves of a workgroup: eight, where a compute unit has one workgroup; fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there are positions for.
+// us with two / four / eight waves: 1 x 8192 x 1536 (one workgroup a compute unit, two states a lane) 415 / 222 / 154, 4 x 8192 x 1536 (three) 499 / 376 / 473, 8 x 2048 x 1536 (six) with its
+// gradient 717 / 732 / 799.
+ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<ForwardShapes>(r, B, D, G, N);
-  r.W = saved ? m2_selective_scan_span(N) / 16 : 8;
-  while (!saved && r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
-  while (!saved && fwd_lds(r) > (80 << 10)) r.W /= 2;
+  const long share = ((long)r.blocks * G * B + num_cus() - 1) / num_cus();
+  const int room = r.NL == 4 ? 8 : r.NL == 2 ? 12 : 16;
+  r.W = 8;
+  while (r.W > (r.NL == 4 ? 4 : 2) && r.W * share > room) r.W /= 2;
+  while (r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
+  while (fwd_lds(r) > (80 << 10)) r.W /= 2;
   return r;
 }
+// The gradient: sets of channels that a workgroup takes one after the other, so that it writes one partial gradient of B and C for all of them: as many as leave the share of
+// the compute unit with most of them as it is, and three workgroups for each.  8 x 2048 x 1536 of 16 states, us with the forward: one set 815, two 724, three 759.
 ScanPlan bwd_plan(int B, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<GradientShapes>(r, B, D, G, N);
   r.W = m2_selective_scan_span(N) / 16;
+  const int sets = r.blocks, cus = num_cus();
+  long least = 0;
+  for (int each = 1; each <= 8; ++each) {
+    const ScanPlan t{r.NS, r.NL, r.W, (sets + each - 1) / each, each};
+    const long groups = (long)t.blocks * G * B, share = (groups + cus - 1) / cus * each;
+    if (each > 1 && (groups < 3L * cus || scan_bwd_lds(t) > (53 << 10))) break;
+    if (least == 0 || share <= least) least = share, r.blocks = t.blocks, r.sets = each;
+  }
   return r;
 }
 
@@ -320,7 +355,7 @@ using namespace m2;
 // Positions between the states that are kept for the gradient.
 extern "C" int m2_selective_scan_span(int N) {
   if (N < 1 || N > kMaxStates) return 0;
-  return N <= 64 ? 128 : N <= 128 ? 64 : 32;
+  return N <= 128 ? 64 : 32;
 }
 
 namespace {
@@ -342,9 +377,9 @@ extern "C" int m2_selective_scan_fwd(const m2_scan_inputs* in, void* y, float* s
   if (in) fill(p, in);
   if (!in || !y || !given(p)) return set_error(M2_ERR_ARG, "selective_scan_fwd: null pointer");
   if (int rc = check_scan("selective_scan_fwd", p, dtype)) return rc;
-  const ScanPlan plan = fwd_plan(p.batch, p.L, p.channels, p.G, p.N, saved != nullptr);
+  const ScanPlan plan = fwd_plan(p.batch, p.L, p.channels, p.G, p.N);
   p.y = y, p.state_out = state_out, p.saved = saved, p.blocks = plan.blocks;
-  p.parts = (p.L + plan.positions() - 1) / plan.positions();
+  p.apart = m2_selective_scan_span(p.N), p.parts = (p.L + p.apart - 1) / p.apart;
   if (int rc = check_grid("selective_scan_fwd", p, plan)) return rc;
   const unsigned grid = (unsigned)((long)plan.blocks * p.G * p.batch);
   const size_t lds = fwd_lds(plan);
@@ -380,7 +415,7 @@ extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gra
   const ScanPlan plan = bwd_plan(p.batch, p.channels, p.G, p.N);
   if (int rc = check_grid("selective_scan_bwd", p, plan)) return rc;
   const hipStream_t s = (hipStream_t)stream;
-  p.blocks = plan.blocks, p.parts = (p.L + plan.positions() - 1) / plan.positions();
+  p.blocks = plan.blocks, p.sets = plan.sets, p.apart = m2_selective_scan_span(p.N), p.parts = (p.L + p.apart - 1) / p.apart, p.kept_parts = plan.positions() / p.apart;
   p.gy = out->gy, p.gy_batch = out->gy_batch, p.gy_row = out->gy_row, p.gstate_out = out->gstate_out;
   p.gx = out->gx, p.gdt = out->gdt, p.gz = out->gz, p.gstate = out->gstate;
   p.saved = const_cast<float*>(saved);
