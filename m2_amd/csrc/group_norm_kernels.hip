@@ -31,13 +31,15 @@ struct NormArgs {
 
 constexpr int kSilu = 1, kGelu = 2;
 
+template <typename T>
 __device__ __forceinline__ float activate(float v, int act) {
-  if (act == kSilu) return silu(v);
+  if (act == kSilu) return silu<T>(v);
   if (act == kGelu) return 0.5f * v * (1.f + erff(v * 0.70710678118654752440f));
   return v;
 }
+template <typename T>
 __device__ __forceinline__ float slope(float v, int act) {
-  if (act == kSilu) return silu_slope(v);
+  if (act == kSilu) return silu_slope<T>(v);
   if (act == kGelu) return fmaf(v * 0.39894228040143267794f, exp_of(-0.5f * v * v), 0.5f * (1.f + erff(v * 0.70710678118654752440f)));
   return 1.f;
 }
@@ -74,37 +76,49 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs p) {
   const float each = 1.f / (float)p.Cg;
   float w[NV][V], b[NV][V];
   my.weights(p, w, b);
-  for (long r = blockIdx.x * 4L + (threadIdx.x >> 6); r < p.N; r += gridDim.x * 4L) {
-    const T* x = static_cast<const T*>(p.x) + r * p.x_sample + my.g * p.Cg;
-    float f[NV][V], sum = 0.f, sq = 0.f;
+  constexpr int U = NV == 1 ? 2 : 1;      // rows asked for together
+  for (long r0 = blockIdx.x * 4L + (threadIdx.x >> 6); r0 < p.N; r0 += gridDim.x * 4L * U) {
+    float f[U][NV][V];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int u = 0; u < U; ++u) {
+      const long r = min(r0 + u * gridDim.x * 4L, p.N - 1);
+      const T* x = static_cast<const T*>(p.x) + r * p.x_sample + my.g * p.Cg;
 #pragma unroll
-      for (int v = 0; v < V; ++v) f[k][v] = 0.f;
-      if (my.at(k) < p.Cg) load_values<T, V>(x + my.at(k), f[k]);
+      for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) sum += f[k][v];
-    }
-    const float mean = lane_sum<P>(sum, lane) * each;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        f[k][v] -= mean;
-        sq = fmaf(f[k][v], my.at(k) < p.Cg ? f[k][v] : 0.f, sq);
+        for (int v = 0; v < V; ++v) f[u][k][v] = 0.f;
+        if (my.at(k) < p.Cg) load_values<T, V>(x + my.at(k), f[u][k]);
       }
-    const float rstd = rsqrtf(fmaf(lane_sum<P>(sq, lane), each, p.eps));
-    if (!my.on) continue;
-    if (my.li == 0 && p.stats) {
-      p.stats[(r * p.G + my.g) * 2] = mean;
-      p.stats[(r * p.G + my.g) * 2 + 1] = rstd;
     }
-    T* y = static_cast<T*>(p.y) + r * p.C + my.g * p.Cg;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
+    for (int u = 0; u < U; ++u) {
+      const long r = r0 + u * gridDim.x * 4L;
+      float sum = 0.f, sq = 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) f[k][v] = activate(fmaf(f[k][v] * rstd, w[k][v], b[k][v]), p.act);
-      if (my.at(k) < p.Cg) store_values<T, V>(y + my.at(k), f[k]);
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum += f[u][k][v];
+      const float mean = lane_sum<P>(sum, lane) * each;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          f[u][k][v] -= mean;
+          sq = fmaf(f[u][k][v], my.at(k) < p.Cg ? f[u][k][v] : 0.f, sq);
+        }
+      const float rstd = rsqrtf(fmaf(lane_sum<P>(sq, lane), each, p.eps));
+      if (!my.on || r >= p.N) continue;
+      if (my.li == 0 && p.stats) {
+        p.stats[(r * p.G + my.g) * 2] = mean;
+        p.stats[(r * p.G + my.g) * 2 + 1] = rstd;
+      }
+      T* y = static_cast<T*>(p.y) + r * p.C + my.g * p.Cg;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[u][k][v] = activate<T>(fmaf(f[u][k][v] * rstd, w[k][v], b[k][v]), p.act);
+        if (my.at(k) < p.Cg) store_values<T, V>(y + my.at(k), f[u][k]);
+      }
     }
   }
 }
@@ -140,7 +154,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(NormArgs p) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         xh[k][v] = (xh[k][v] - mean) * rstd;
-        const float g = p.act ? t[k][v] * slope(fmaf(xh[k][v], w[k][v], b[k][v]), p.act) : t[k][v];
+        const float g = p.act ? t[k][v] * slope<T>(fmaf(xh[k][v], w[k][v], b[k][v]), p.act) : t[k][v];
         gb[k][v] += g;
         gw[k][v] = fmaf(g, xh[k][v], gw[k][v]);
         t[k][v] = g * w[k][v];
@@ -299,7 +313,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs p, int CL) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) f[u][v] = activate(fmaf((f[u][v] - mean) * rstd, w[v], b[v]), p.act);
+      for (int v = 0; v < V; ++v) f[u][v] = activate<T>(fmaf((f[u][v] - mean) * rstd, w[v], b[v]), p.act);
       if (s + u * my.parts < my.s1) store_values<T, V>(y + (long)(s + u * my.parts) * p.C, f[u]);
     }
   }
@@ -335,7 +349,7 @@ __global__ __launch_bounds__(256) void norm_bwd_partials_kernel(NormArgs p, int 
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float xh = (f[u][v] - mean) * rstd;
-          const float d = p.act ? g[u][v] * slope(fmaf(xh, w[v], b[v]), p.act) : g[u][v];
+          const float d = p.act ? g[u][v] * slope<T>(fmaf(xh, w[v], b[v]), p.act) : g[u][v];
           gb[v] += d;
           gw[v] = fmaf(d, xh, gw[v]);
         }
@@ -400,7 +414,7 @@ __global__ __launch_bounds__(256) void norm_bwd_apply_kernel(NormArgs p, int CL)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float xh = (f[u][v] - mean) * rstd;
-        const float d = p.act ? g[u][v] * slope(fmaf(xh, w[v], b[v]), p.act) : g[u][v];
+        const float d = p.act ? g[u][v] * slope<T>(fmaf(xh, w[v], b[v]), p.act) : g[u][v];
         f[u][v] = rstd * (fmaf(d, w[v], -sums.x) - xh * sums.y);
       }
       if (s + u * my.parts < my.s1) store_values<T, V>(gx + (long)(s + u * my.parts) * p.C, f[u]);
@@ -437,7 +451,7 @@ NormPlan norm_plan(long N, int S, int C, int G, int V) {
   const int parts = 256 / r.CL;
   const long across = (columns + r.CL - 1) / r.CL;
   r.chunk = 64 * parts;
-  while (r.chunk > 4 * parts && N * across * ((S + r.chunk - 1) / r.chunk) < 8L * num_cus()) r.chunk /= 2;
+  while (r.chunk > 4 * parts && N * across * ((S + r.chunk - 1) / r.chunk) < 2L * num_cus()) r.chunk /= 2;
   r.chunks = (S + r.chunk - 1) / r.chunk;
   return r;
 }

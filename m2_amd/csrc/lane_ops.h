@@ -125,14 +125,20 @@ __device__ __forceinline__ float exp_of(float x) {
   const float e = __builtin_amdgcn_exp2f(hi);
   return fmaf(e, lo * kLn2, e);
 }
-// 1 / (1 + exp(-x)); of NaN some number.
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(fminf(-x, 88.f))); }
-__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+// x / (1 + exp(-x)), for a result of type T: the exponential of a bf16 result has its argument as it is rounded (off by |x| 2^-23 of itself at most, against bf16's 2^-8), which saves six
+// of eleven instructions.
+template <typename T>
+__device__ __forceinline__ float silu(float x) {
+  const float e = sizeof(T) == 2 ? __builtin_amdgcn_exp2f(x * -kLog2E) : exp_of(fminf(-x, 88.f));
+  return x * __builtin_amdgcn_rcpf(1.f + e);
+}
 // u = exp(-|x|) and r = 1 / (1 + u): what sigmoid(x), sigmoid(-x), softplus(x) and their products are made of, without cancellation.
+// EXACT: the exponential to 2^-23 of itself; else, for what ends in bf16, as in silu.
+template <bool EXACT>
 struct Logistic {
   float u, r;
   bool below;
-  __device__ __forceinline__ explicit Logistic(float x) : u(exp_of(-fabsf(x))), r(__builtin_amdgcn_rcpf(1.f + u)), below(x < 0.f) {}
+  __device__ __forceinline__ explicit Logistic(float x) : u(EXACT ? exp_of(-fabsf(x)) : __builtin_amdgcn_exp2f(-kLog2E * fabsf(x))), r(__builtin_amdgcn_rcpf(1.f + u)), below(x < 0.f) {}
   __device__ __forceinline__ float value() const { return below ? u * r : r; }
   __device__ __forceinline__ float other() const { return below ? r : u * r; }      // of -x
 };
@@ -144,11 +150,19 @@ __device__ __forceinline__ float softplus_of(float x, float u) {
 }
 __device__ __forceinline__ float softplus(float x) { return softplus_of(x, exp_of(-fabsf(x))); }
 // d/dx of x sigmoid(x) = s + x s (1 - s)
-__device__ __forceinline__ float silu_slope_of(float x, const Logistic& l) {
+template <bool EXACT>
+__device__ __forceinline__ float silu_slope_of(float x, const Logistic<EXACT>& l) {
   const float s = l.value();
   return fmaf(s * x, l.other(), s);
 }
-__device__ __forceinline__ float silu_slope(float x) { return silu_slope_of(x, Logistic(x)); }
+template <typename T>
+__device__ __forceinline__ float silu_slope(float x) { return silu_slope_of(x, Logistic<sizeof(T) == 4>(x)); }
+
+// Workgroups go round the eight XCDs: those of neighbouring numbers after this share one and its L2.
+__device__ __forceinline__ int xcd_order(int id, int count) {
+  const int each = count / 8, rest = count % 8, x = id % 8;
+  return id / 8 + x * each + min(x, rest);
+}
 
 // Sums of `rows` partial results: column j of plane k (planes (K + 1 or 1) x n values) goes to wide[j * K + k] for k < K and to last[j] for k = K; either may be null.
 int sum_partials(const float* partials, long rows, int K, long n, float* wide, float* last, hipStream_t stream);

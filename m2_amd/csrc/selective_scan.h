@@ -48,12 +48,6 @@ struct ScanShape {
 };
 constexpr int log2_of(int n) { return n > 1 ? 1 + log2_of(n / 2) : 0; }
 
-// Workgroups go round the eight XCDs: those of neighbouring numbers after this share one and its L2.
-__device__ __forceinline__ int xcd_order(int id, int count) {
-  const int each = count / 8, rest = count % 8, x = id % 8;
-  return id / 8 + x * each + min(x, rest);
-}
-
 __device__ __forceinline__ int scan_length(const ScanArgs& p, int b) {
   if (!p.lengths) return p.L;
   const long long n = p.lengths[b];

@@ -189,7 +189,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
         const float raw = value_of<T>(rdt[i]) + bias;
         d[i] = raw, d_slope[i] = inside ? 1.f : 0.f;
         if (soft) {
-          const Logistic l(raw);
+          const Logistic<true> l(raw);
           d[i] = softplus_of(raw, l.u);
           d_slope[i] = inside ? l.value() : 0.f;
         }
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
         u[i] = gv[i], gz[i] = 0.f;
         if (gated) {
           const float zv = inside ? value_of<T>(rz[i]) : 0.f;
-          const Logistic l(zv);
+          const Logistic<sizeof(T) == 4> l(zv);
           u[i] = gv[i] * (zv * l.value());
           gz[i] = gv[i] * silu_slope_of(zv, l);
         }
