@@ -91,7 +91,8 @@ struct Near {
   uint32_t first, end;
   template <typename T>
   __device__ __forceinline__ static Near of(const T*, int t, long row, int at, int last) {
-    return {(uint32_t)(t * (int)row + at) * (uint32_t)sizeof(T), (uint32_t)(last * (int)row + at) * (uint32_t)sizeof(T)};
+    // (a product of 24-bit factors takes a quarter of the time)
+    return {(__umul24((uint32_t)t, (uint32_t)row) + (uint32_t)at) * (uint32_t)sizeof(T), (uint32_t)(last * (int)row + at) * (uint32_t)sizeof(T)};
   }
   __device__ __forceinline__ uint32_t operator()(uint32_t further) const { return min(first + further, end); }
 };

@@ -96,6 +96,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
   const bool moves = NS <= TT || q < TT;
   const int q0 = NS <= TT ? q : min(q, TT - 1);
   const auto channel = [&](int set, bool& on) {
+    const ArgsInMemory& p = *arguments_anew();
     const int first = (block * p.sets + set) * CW, count = min(CW, p.per_group - first);
     on = c < count;
     return g * p.per_group + first + min(c, count - 1);
@@ -114,7 +115,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
           carried[((set * 2 + turn) * 64 + lane) * NL + j] = on && q * NL + j < p.N && p.gstate_out ? p.gstate_out[((long)b * p.channels + ch) * p.N + q * NL + j] : 0.f;
     }
 
-  const long out_at = (long)b * p.L * p.channels;
   const int steps = (n + span - 1) / span;
   const bool gated = p.z, soft = p.softplus, biased = p.dt_bias, skips = p.D;
   const int N = p.N;
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
     const float* kept = p.saved + ((long)b * p.parts + s * p.kept_parts) * p.channels * p.N;
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const uint32_t at = (uint32_t)(ch * p.N + min(q * NL + j, p.N - 1)) * 4u;
+      const uint32_t at = (__umul24((uint32_t)ch, (uint32_t)p.N) + (uint32_t)min(q * NL + j, p.N - 1)) * 4u;
       rA[j] = at_offset<const float>(p.A, at), rH[j] = at_offset<const float>(kept, at);
     }
     // (without a bias or D: a value that is not used)
@@ -344,10 +344,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
       });
       float gD = 0.f, gbias = 0.f;
       ArgsInMemory& p = *arguments_anew();
-      T* gx = static_cast<T*>(p.gx) + out_at + (long)t0 * p.channels;
-      T* gdt = static_cast<T*>(p.gdt) + out_at + (long)t0 * p.channels;
-      T* gzs = static_cast<T*>(p.gz) + out_at + (long)t0 * p.channels;
-      const uint32_t off = (uint32_t)(q0 * p.channels + ch) * sizeof(T);
+      const long out_at = ((long)b * p.L + t0) * p.channels;
+      T* gx = static_cast<T*>(p.gx) + out_at;
+      T* gdt = static_cast<T*>(p.gdt) + out_at;
+      T* gzs = static_cast<T*>(p.gz) + out_at;
+      const uint32_t off = (__umul24((uint32_t)q0, (uint32_t)p.channels) + (uint32_t)ch) * sizeof(T);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int t = t0 + i * NS;
@@ -382,18 +383,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
       }
     }
   }
+  const ArgsInMemory& end = *arguments_anew();
   for (int set = 0; set < sets; ++set) {
     bool on;
     const int ch = channel(set, on);
-    for (int t0 = steps * span + w * TT; t0 < p.L; t0 += span)
+    for (int t0 = steps * span + w * TT; t0 < end.L; t0 += span)
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int t = t0 + q0 + i * NS;
-        const long at = out_at + (long)t * p.channels + ch;
-        if (on && moves && t < p.L) {
-          if (p.gx) static_cast<T*>(p.gx)[at] = value_to<T>(0.f);
-          if (p.gdt) static_cast<T*>(p.gdt)[at] = value_to<T>(0.f);
-          if (p.gz) static_cast<T*>(p.gz)[at] = value_to<T>(0.f);
+        const long at = ((long)b * end.L + t) * end.channels + ch;
+        if (on && moves && t < end.L) {
+          if (end.gx) static_cast<T*>(end.gx)[at] = value_to<T>(0.f);
+          if (end.gdt) static_cast<T*>(end.gdt)[at] = value_to<T>(0.f);
+          if (end.gz) static_cast<T*>(end.gz)[at] = value_to<T>(0.f);
         }
       }
   }
@@ -406,18 +408,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
 #pragma unroll
     for (int j = 0; j < NL + 2; ++j) {
       sums[j] = 0.f;
-      for (int o = 0; o < W; ++o) sums[j] += lds[W * Room::kWave + (o * p.sets + set) * Room::kWaveSet + j * 64 + lane];
+      for (int o = 0; o < W; ++o) sums[j] += lds[W * Room::kWave + (o * end.sets + set) * Room::kWaveSet + j * 64 + lane];
     }
     const float gD = lane_sum<NS>(sums[NL], lane), gbias = lane_sum<NS>(sums[NL + 1], lane);
     if (!on) continue;
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const long at = ((long)b * p.channels + ch) * p.N + q * NL + j;
-      if (q * NL + j >= p.N) continue;
-      p.a_part[at] = sums[j];
-      if (p.gstate) p.gstate[at] = carried[((set * 2 + 1) * 64 + lane) * NL + j];      // (behind step 0)
+      const long at = ((long)b * end.channels + ch) * end.N + q * NL + j;
+      if (q * NL + j >= end.N) continue;
+      end.a_part[at] = sums[j];
+      if (end.gstate) end.gstate[at] = carried[((set * 2 + 1) * 64 + lane) * NL + j];      // (behind step 0)
     }
-    if (q == 0) p.d_part[(long)b * p.channels + ch] = gD, p.bias_part[(long)b * p.channels + ch] = gbias;
+    if (q == 0) end.d_part[(long)b * end.channels + ch] = gD, end.bias_part[(long)b * end.channels + ch] = gbias;
   }
 }
 

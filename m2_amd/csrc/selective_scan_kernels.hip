@@ -275,7 +275,7 @@ int check_scan(const char* name, const ScanArgs& p, int dtype) {
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype %d", name, dtype);
   for (long row : {p.x_row, p.dt_row, p.z_row, p.b_row, p.c_row, p.gy_row})
     if (row < 0 || row >= 1L << 24) return set_error(M2_ERR_UNSUPPORTED, "%s: rows %ld values apart, below 2^24 are supported", name, row);
-  if ((long)p.batch * p.L > (1L << 36) / ((long)p.G * p.N)) return set_error(M2_ERR_ARG, "%s: at most 2^36 values of B", name);
+  if ((long)p.batch * p.L >= (1L << 32) / ((long)p.G * p.N)) return set_error(M2_ERR_ARG, "%s: below 2^32 values of B are supported", name);
   if (p.channels > 1 << 20 || p.L > 1 << 30 || (long)p.batch * p.channels > 1L << 24)
     return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^24 channels of all sequences", name);
   return M2_OK;
@@ -316,21 +316,23 @@ void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
 }
 // Waves of a workgroup: eight, where a compute unit has one workgroup; fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there are positions for.
 // us with two / four / eight waves: 1 x 8192 x 1536 (one workgroup a compute unit, two states a lane) 415 / 222 / 154, 4 x 8192 x 1536 (three) 499 / 376 / 473, 8 x 2048 x 1536 (six) with its
-// gradient 717 / 732 / 799.
+// gradient 717 / 732 / 799; four states a lane, 4 x 8192 x 1536 (two workgroups) 424 with four waves and 457 with eight, 8 x 2048 x 1536 (three) 192 and 171.
 ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<ForwardShapes>(r, B, D, G, N);
   const long share = ((long)r.blocks * G * B + num_cus() - 1) / num_cus();
   const int room = r.NL == 4 ? 8 : r.NL == 2 ? 12 : 16;
   r.W = 8;
-  while (r.W > (r.NL == 4 ? 4 : 2) && r.W * share > room) r.W /= 2;
+  if (r.NL == 4) r.W = share % 2 ? 8 : 4;      // one workgroup at a time fills a compute unit with eight, two with four
+  else while (r.W > 2 && r.W * share > room) r.W /= 2;
   while (r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
   while (fwd_lds(r) > (80 << 10)) r.W /= 2;
   return r;
 }
 // The gradient: sets of channels that a workgroup takes one after the other, so that it writes one partial gradient of B and C for all of them: as many as leave the share of
-// the compute unit with most of them as it is, and three workgroups for each.  8 x 2048 x 1536 of 16 states, us with the forward: one set 815, two 724, three 759.
-ScanPlan bwd_plan(int B, int D, int G, int N) {
+// the compute unit with most of them as it is, and three workgroups for each.  8 x 2048 x 1536 of 16 states, us with the forward: one set 815, two 724, three 759.  More where the
+// partial gradients would take more than 1 GiB and sixteen bytes for each value of x (many states, whose workgroups have few channels a set).
+ScanPlan bwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<GradientShapes>(r, B, D, G, N);
   r.W = m2_selective_scan_span(N) / 16;
@@ -342,6 +344,12 @@ ScanPlan bwd_plan(int B, int D, int G, int N) {
     if (each > 1 && (groups < 3L * cus || scan_bwd_lds(t) > (53 << 10))) break;
     if (least == 0 || share <= least) least = share, r.blocks = t.blocks, r.sets = each;
   }
+  const double values = (double)B * L, most = std::max(1073741824.0, 16 * values * D);
+  for (int each = r.sets + 1; each <= std::min(64, sets) && 8 * values * r.blocks * G * N > most; ++each) {
+    const ScanPlan t{r.NS, r.NL, r.W, (sets + each - 1) / each, each};
+    if (scan_bwd_lds(t) > (160 << 10)) break;
+    r.blocks = t.blocks, r.sets = each;
+  }
   return r;
 }
 
@@ -352,20 +360,45 @@ struct Partials {
   size_t bytes() const { return sizeof(float) * (2 * bc + a + 2 * d); }
 };
 
-// A group's partial gradients of B (blockIdx.y 0) or C, one from each of its workgroups, added up; 0 behind the end of a sequence.
+// The rest of the gradient, in one launch.  blockIdx.y 0 and 1: a group's partial gradients of B and C, one from each of its workgroups, added up; 0 behind the end of a sequence.  2: those of
+// A, D and dt_bias, one from each sequence.
 template <typename T>
-__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, T* gB, T* gC) {
-  T* out = blockIdx.y ? gC : gB;
-  if (!out) return;
-  const long row = (long)p.G * p.N, count = (long)p.batch * p.L * row, i = blockIdx.x * 256L + threadIdx.x;
-  if (i >= count) return;
-  const long bt = i / row;
-  const int b = bt / p.L, t = bt - (long)b * p.L;
-  const float* part = (blockIdx.y ? p.c_part : p.b_part) + i;
+__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs p, T* gB, T* gC, float* gA, float* gD, float* gbias) {
+  constexpr int U = 8;
+  const long i = blockIdx.x * 256L + threadIdx.x;
+  const float* part;
+  long count, apart;      // terms, and how far they lie from each other
+  if (blockIdx.y == 2) {
+    const long states = (long)p.channels * p.N, at = i - states;
+    apart = at < 0 ? states : p.channels, count = p.batch;
+    part = at < 0 ? p.a_part + i : at < p.channels ? p.d_part + at : p.bias_part + (at - p.channels);
+    float* out = at < 0 ? gA : at < p.channels ? gD : gbias;
+    if (at >= 2L * p.channels || !out) return;
+  } else {
+    const long row = (long)p.G * p.N;
+    apart = (long)p.batch * p.L * row;
+    if (i >= apart || !(blockIdx.y ? gC : gB)) return;
+    const long bt = i / row;
+    const int b = bt / p.L, t = bt - (long)b * p.L;
+    count = t < scan_length(p, b) ? p.blocks : 0;
+    part = (blockIdx.y ? p.c_part : p.b_part) + i;
+  }
   float sum = 0.f;
-  if (t < scan_length(p, b))
-    for (int k = 0; k < p.blocks; ++k) sum += part[k * count];
-  out[i] = value_to<T>(sum);
+  for (long k = 0; k < count; k += U) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = part[min(k + u, count - 1) * apart];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum += k + u < count ? v[u] : 0.f;
+  }
+  if (blockIdx.y == 2) {
+    const long states = (long)p.channels * p.N, at = i - states;
+    if (at < 0) gA[i] = sum;
+    else if (at < p.channels) gD[at] = sum;
+    else gbias[at - p.channels] = sum;
+  } else {
+    (blockIdx.y ? gC : gB)[i] = value_to<T>(sum);
+  }
 }
 
 }  // namespace
@@ -376,7 +409,7 @@ using namespace m2;
 // Positions between the states that are kept for the gradient.
 extern "C" int m2_selective_scan_span(int N) {
   if (N < 1 || N > kMaxStates) return 0;
-  return N <= 128 ? 64 : 32;
+  return N <= 64 ? 64 : 32;
 }
 
 namespace {
@@ -425,7 +458,7 @@ extern "C" size_t m2_selective_scan_bwd_workspace_bytes(int batch, int length, i
   ScanArgs p{};
   p.batch = batch, p.L = length, p.channels = channels, p.G = groups, p.N = states;
   if (check_scan("selective_scan_bwd", p, M2_DTYPE_F32)) return 0;
-  return Partials(p, bwd_plan(batch, channels, groups, states).blocks).bytes();
+  return Partials(p, bwd_plan(batch, length, channels, groups, states).blocks).bytes();
 }
 
 extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gradients* out, const float* saved, void* workspace, int dtype, void* stream) {
@@ -433,7 +466,7 @@ extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gra
   if (in) fill(p, in);
   if (!in || !out || !given(p) || !out->gy || !saved || !workspace) return set_error(M2_ERR_ARG, "selective_scan_bwd: null pointer");
   if (int rc = check_scan("selective_scan_bwd", p, dtype)) return rc;
-  const ScanPlan plan = bwd_plan(p.batch, p.channels, p.G, p.N);
+  const ScanPlan plan = bwd_plan(p.batch, p.L, p.channels, p.G, p.N);
   if (int rc = check_grid("selective_scan_bwd", p, plan)) return rc;
   const hipStream_t s = (hipStream_t)stream;
   p.blocks = plan.blocks, p.sets = plan.sets, p.apart = m2_selective_scan_span(p.N), p.parts = (p.L + p.apart - 1) / p.apart, p.kept_parts = plan.positions() / p.apart;
@@ -444,19 +477,11 @@ extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gra
   p.b_part = static_cast<float*>(workspace), p.c_part = p.b_part + room.bc;
   p.a_part = p.c_part + room.bc, p.d_part = p.a_part + room.a, p.bias_part = p.d_part + room.d;
   if (int rc = scan_bwd(p, plan, dtype, s)) return rc;
-  if (out->gB || out->gC) {
-    const long count = (long)p.batch * p.L * p.G * p.N;
-    const dim3 grid((unsigned)((count + 255) / 256), 2);
-    if (dtype == M2_DTYPE_F32) hipLaunchKernelGGL(scan_join_kernel<float>, grid, dim3(256), 0, s, p, (float*)out->gB, (float*)out->gC);
-    else hipLaunchKernelGGL(scan_join_kernel<uint16_t>, grid, dim3(256), 0, s, p, (uint16_t*)out->gB, (uint16_t*)out->gC);
-    if (int rc = check_launch("scan_join_kernel")) return rc;
-  }
-  if (out->gA)
-    if (int rc = sum_partials(p.a_part, p.batch, 0, (long)p.channels * p.N, nullptr, out->gA, s)) return rc;
-  if (out->gD)
-    if (int rc = sum_partials(p.d_part, p.batch, 0, p.channels, nullptr, out->gD, s)) return rc;
-  if (out->gdt_bias) return sum_partials(p.bias_part, p.batch, 0, p.channels, nullptr, out->gdt_bias, s);
-  return M2_OK;
+  const long count = std::max((long)p.batch * p.L * p.G * p.N, (long)p.channels * (p.N + 2));
+  const dim3 grid((unsigned)((count + 255) / 256), 3);
+  if (dtype == M2_DTYPE_F32) hipLaunchKernelGGL(scan_join_kernel<float>, grid, dim3(256), 0, s, p, (float*)out->gB, (float*)out->gC, out->gA, out->gD, out->gdt_bias);
+  else hipLaunchKernelGGL(scan_join_kernel<uint16_t>, grid, dim3(256), 0, s, p, (uint16_t*)out->gB, (uint16_t*)out->gC, out->gA, out->gD, out->gdt_bias);
+  return check_launch("scan_join_kernel");
 }
 
 extern "C" int m2_selective_scan_step(const m2_scan_inputs* in, void* y, float* state_out, int dtype, void* stream) {

@@ -132,3 +132,11 @@ def test_without_their_extension_only_they_raise():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
+
+
+def test_scan_gradient_workspace_stays_in_proportion():
+    """Partial gradients of B and C: 1 GiB, or sixteen bytes for each value of x; sets of channels share one where there would be more, as far as shared memory holds them (29 channels of 65 to 128 states)."""
+    from m2_amd._lib import lib
+    for batch, length, channels, groups, states in ((8, 2048, 1536, 1, 16), (8, 2048, 1536, 1, 128), (1, 131072, 1536, 1, 16), (4, 4096, 4096, 8, 64), (8, 2048, 3584, 1, 100)):
+        rest = 4 * (batch * channels * (states + 2))
+        assert lib.m2_selective_scan_bwd_workspace_bytes(batch, length, channels, groups, states) <= max(1 << 30, 16 * batch * length * channels, 8 * batch * length * states * -(-channels // 29)) + rest, (batch, length, channels, groups, states)
