@@ -4,7 +4,7 @@ first two, for one token more.
 The reference mixes sequences with both sides in view (`MonarchMixerSequenceMixing`: short convolution of three, gates and long convolutions,
 bert/src/mm/monarch_mixer_sequence_mixer.py:100-154); these are their counterparts where a position may use only what lies before it.  Hidden states are
 (batch, positions, channels), fp32 or bf16 on the GPU; parameters and the scan's states are fp32.  Arithmetic is fp32, results are rounded once.
-Rows may lie any distance apart (one half of a projection's result, say); other layouts are copied.  All of them are differentiable once in every tensor but
+Rows may lie any distance apart (one half of a projection's result, say; the scan copies what lies 2^24 values apart); other layouts are copied.  All of them are differentiable once in every tensor but
 `lengths`; the steps are not.
 
 Inside a stream capture a forward that asks for gradients is refused while a graph made on another stream still holds one of its leaves.
@@ -22,7 +22,7 @@ Tensor = torch.Tensor
 
 def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None, state: Optional[Tensor] = None,
                 lengths: Optional[Tensor] = None, return_state: bool = False):
-    """y[:, t] = act(bias + sum_k weight[:, k] x[:, t - K + 1 + k]) of x (B, L, C), each channel on its own; weight (C, K), K 1 to 8, bias (C); `activation` None or
+    """y[:, t] = act(bias + sum_k weight[:, k] x[:, t - K + 1 + k]) of x (B, L, C), B at most 65535, each channel on its own; weight (C, K), K 1 to 8, bias (C); `activation` None or
     "silu".
 
     `state` (B, K - 1, C) of x's type: the inputs ahead of the first position, oldest first (None: zeros).  `lengths` (B) int64: sequence b ends there

@@ -61,6 +61,9 @@ Tensor rows(const Tensor& t, int64_t last = 1) {
   }
   return t;
 }
+// t (B, L, ...) of what the scan's kernels address in 32 bits from a position on: rows below 2^24 values apart.
+Tensor near_rows(const Tensor& t) { return t.defined() && t.size(1) > 1 && t.stride(1) >= 1 << 24 ? t.contiguous() : t; }
+int64_t row_of(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
 const float* floats(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 float* floats_out(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 const long long* lengths_of(const Tensor& t) { return t.defined() ? reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) : nullptr; }
@@ -316,7 +319,8 @@ struct ScanCall {
     keep.push_back(s.in.size() > LENGTHS ? dense(s.in[LENGTHS]) : Tensor());
     const auto place = [&](int i, const void*& p, long& batch, long& row) {
       if (!keep[i].defined()) return;
-      p = keep[i].data_ptr(), batch = keep[i].stride(0), row = s.step ? 0 : keep[i].stride(1);
+      if (!s.step) keep[i] = near_rows(keep[i]);
+      p = keep[i].data_ptr(), batch = keep[i].stride(0), row = s.step ? 0 : row_of(keep[i]);
     };
     place(X, in.x, in.x_batch, in.x_row);
     place(DT, in.dt, in.dt_batch, in.dt_row);
@@ -361,7 +365,7 @@ struct SelectiveScanBackward : CausalNode {
     {
       const at::AutoDispatchBelowADInplaceOrView below;
       const c10::DeviceGuard guard(in[X].device());
-      const Tensor kept = dense(in[SAVED]), gy = given(g[0], in[X]), glast = dense(g[1]);
+      const Tensor kept = dense(in[SAVED]), gy = near_rows(given(g[0], in[X])), glast = dense(g[1]);
       for (int i = 0; i < INPUTS; ++i)
         if (task_should_compute_output(i)) out[i] = at::empty(in[i].sizes(), in[i].options().requires_grad(false));
       in.pop_back();
@@ -373,7 +377,7 @@ struct SelectiveScanBackward : CausalNode {
         const ScanCall call(s);
         const Tensor room = scratch(scan_bwd_workspace_bytes(s.batch, s.L, s.D, s.G, s.N), s.in[X]);
         m2_scan_gradients into{};
-        into.gy = gy.data_ptr(), into.gy_batch = gy.stride(0), into.gy_row = gy.stride(1), into.gstate_out = floats(glast);
+        into.gy = gy.data_ptr(), into.gy_batch = gy.stride(0), into.gy_row = row_of(gy), into.gstate_out = floats(glast);
         into.gx = pointer(out[X]), into.gdt = pointer(out[DT]), into.gz = pointer(out[Z]), into.gB = pointer(out[B_]), into.gC = pointer(out[C_]);
         into.gA = floats_out(out[A_]), into.gD = floats_out(out[D_]), into.gdt_bias = floats_out(out[DT_BIAS]), into.gstate = floats_out(out[STATE]);
         check(scan_bwd(&call.in, &into, floats(kept), pointer(room), s.type, current_stream()));

@@ -3,7 +3,8 @@
 //   pre[t, c] = bias[c] + sum_k w[c, k] x[t - K + 1 + k, c]      y = pre, or pre sigmoid(pre)      x[t] for t < 0: the state, oldest first, or 0
 //   g = gy act'(pre)     gx[s] = sum_j w[K - 1 - j] g[s + j]     gw[k] = sum g[t] x[t - K + 1 + k]     gb = sum g
 //
-// A thread owns V neighbouring channels and a run of positions; what the taps need of the positions before stays in registers.
+// A thread owns V neighbouring channels and a run of positions; what the taps need of the positions before stays in registers, so that x is read once but for the ends of runs.  Bound by memory: 4 x
+// 8192 x 1536 bf16 47 us (4.3 TB/s, where a copy of as much reaches 5.1), 8 x 2049 x 1920 fp32 with its gradient 118 (4.3 TB/s; the forward 37, the gradient 66, its sums over runs 5).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -5,6 +5,10 @@
 //
 // One position (groups of a token): P neighbouring lanes hold a group in registers, read once.  More: the values are read twice, first for means and squared distances
 // of small blocks, joined with what their means differ by, so that nothing cancels; second for the result.
+//
+// Bound by memory: 32768 x 1536 bf16 in 24 groups with SiLU 51 us (3.9 TB/s).  8 x 2048 x 1536 with its gradient 107 us: x twice, gy and x twice more, 0.4 GB of reads and writes at 3.8 TB/s, part of
+// them from the last cache; 3 x 4001 x 960 fp32 29 us (blocks 9, their join 3.6, the result 17).  Chunks that give two workgroups a compute unit: with eight, partial results and their sums took 175 us
+// instead of 115.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

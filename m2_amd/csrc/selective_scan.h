@@ -199,12 +199,13 @@ void with_scan_shape(int NS, int NL, F&& f) {
   else if (NL == 2) with_lanes(std::integral_constant<int, 2>{});
   else with_lanes(std::integral_constant<int, 4>{});
 }
-// Four states of a lane hold 128 registers of decays and inputs in the forward; the gradient has room for two, and for four only where no channels' sums are formed.
+// Those whose registers do not pass a wave's: four states of a lane hold 128 of decays and inputs, and many channels of a wave need more for each lane's own positions; the gradient has room
+// for two, and for four only where no channels' sums are formed.
 struct ForwardShapes {
-  static constexpr bool built(int NS, int NL) { return NL <= 2 || NS >= 2; }
+  static constexpr bool built(int NS, int NL) { return NL <= 2 || NS >= 4; }
 };
 struct GradientShapes {
-  static constexpr bool built(int NS, int NL) { return NS >= 2 && (NL <= 2 || NS == 64); }
+  static constexpr bool built(int NS, int NL) { return NL == 1 ? NS >= 2 : NL == 2 ? NS >= 4 : NS == 64; }
 };
 
 // How a call is spread: lanes a channel, states a lane, waves of a workgroup.

@@ -81,7 +81,7 @@ def _bounds(d, softplus, lengths, dtype=F32):
 
 SIZES = [(1, 1, 1, 1, None), (1, 1, 64, 16, None), (2, 2, 5, 3, None), (3, 17, 40, 16, 2), (2, 129, 100, 16, None), (1, 300, 33, 8, 1), (2, 150, 24, 61, 3), (4, 65, 130, 4, None), (1, 257, 70, 2, None),
          (2, 40, 12, 128, 2), (1, 70, 9, 200, None), (2, 33, 7, 256, None), (1, 1000, 20, 16, None), (40, 19, 256, 16, 4), (20, 140, 336, 24, None), (3, 128, 64, 64, None), (70, 50, 260, 32, 1),
-         (17, 37, 1024, 1, 1), (65, 21, 130, 100, None), (140, 35, 8, 130, 2)]
+         (17, 37, 1024, 1, 1), (65, 21, 130, 100, None), (140, 35, 8, 130, 2), (2, 50, 12, 16, 12), (1, 33, 6, 70, 6)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -267,3 +267,23 @@ def test_long_offsets(gpu):
     w = torch.randn(40, 4, device=gpu)
     assert torch.equal(m2_amd.causal_conv(x, w), m2_amd.causal_conv(part.unsqueeze(0), w))
     assert torch.equal(m2_amd.group_norm(x, 4), m2_amd.group_norm(part.unsqueeze(0), 4))
+
+
+def test_rows_far_apart(gpu):
+    """Rows 2^24 values apart: further than the kernels' 32-bit offsets go, they are copied."""
+    import m2_amd
+    wide = torch.randn(5, 2 ** 24, generator=torch.Generator(device=gpu).manual_seed(1), device=gpu)
+    ins, _ = _inputs(gpu, 1, 5, 24, 16, None, F32, ("D", "z"))
+    far = dict(ins, x=wide[:, :24].unsqueeze(0), B=wide[:, 100:116].unsqueeze(0), z=wide[:, 200:224].unsqueeze(0))
+    near = {k: None if v is None else v.contiguous() for k, v in far.items()}
+    gy = wide[:, 300:324].unsqueeze(0)
+    results = []
+    for which, g in ((far, gy), (near, gy.contiguous())):
+        mine = {k: None if v is None else v.detach().requires_grad_() for k, v in which.items()}
+        y, last = _call(mine, True)
+        results.append([y.detach(), last.detach(), *torch.autograd.grad(y, [v for v in mine.values() if v is not None], g)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # one position: its distance to a next one says nothing
+    one = wide.as_strided((1, 1, 24), (2 ** 25, 2 ** 26, 1))
+    a = m2_amd.selective_scan(one, ins["dt"][:, :1], ins["A"], ins["B"][:, :1], ins["C"][:, :1])
+    assert torch.equal(a, m2_amd.selective_scan(one.contiguous(), ins["dt"][:, :1], ins["A"], ins["B"][:, :1], ins["C"][:, :1]))
