@@ -10,7 +10,7 @@
 // operation a state than one position after another takes, and the decays' exponentials, four times as costly as the others, are formed once.
 //
 // Bound by vector instructions: nine issue slots of a state and position (product, exponential, product, three sums) and six more for all else, of which the step size's softplus and the gate are
-// half, shared memory being busy 60 % of that time.  bf16, 16 states: 4 x 8192 x 1536 370 us, where bytes would take 79; 1 x 8192 x 1536 155 (192 workgroups for 256 compute units); fp32, 61 states,
+// half, shared memory being busy 60 % of that time.  bf16, 16 states: 4 x 8192 x 1536 365 us, where bytes would take 79; 1 x 8192 x 1536 134 (192 workgroups for 256 compute units); fp32, 61 states,
 // 5 x 1013 x 1002 142.  A loop must not wait for its prefetch: a choice between two loads, or a value that is made of a loaded register only later, made the compiler move registers at once
 // (4 x 8192 x 1536 464 -> 374 us without).  Addresses are a scalar and 32 bits of a lane: in 64 bits they were a tenth of all instructions.
 #include <hip/hip_runtime.h>
@@ -23,8 +23,11 @@
 
 namespace m2 {
 
+// Shapes of two states a lane whose registers leave room for three waves a SIMD.
+constexpr bool three_waves(int NS, int NL) { return NL == 2 && NS > 2 && NS < 32; }
+
 template <typename T, int NS, int NL>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && NS > 2 ? 3 : 2))) void selective_scan_kernel(ScanArgs p) {
+__global__ __launch_bounds__(three_waves(NS, NL) ? 768 : 512) __attribute__((amdgpu_waves_per_eu(three_waves(NS, NL) ? 3 : 2))) void selective_scan_kernel(ScanArgs p) {
   using S = ScanShape<NS, NL>;
   constexpr int CW = S::CW, NP = S::NP, TT = S::TT, NT = S::NT, PITCH = S::PITCH;
   constexpr int kWave = 2 * S::TILE + (NS > 1 ? 2 * CW * PITCH : 0);      // floats
@@ -139,7 +142,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
     }
     float P[NL], start[NL];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * A2[j]);
+    for (int j = 0; j < NL; ++j) P[j] = __builtin_amdgcn_exp2f(total * A2[j]), start[j] = 0.f;
 
     if (W == 1) {
 #pragma unroll
@@ -149,17 +152,40 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
       store_values<float, NL>(turn + (w * 2 * 64 + lane) * NL, P);
       store_values<float, NL>(turn + ((w * 2 + 1) * 64 + lane) * NL, h);
       __syncthreads();      // (two turns: what is written next is read behind the next barrier)
-      const auto meet = [&](int o) {
-        float po[NL], ho[NL];
-        load_values<float, NL>(turn + (o * 2 * 64 + lane) * NL, po);
-        load_values<float, NL>(turn + ((o * 2 + 1) * 64 + lane) * NL, ho);
+      // four at a time, since one after another would wait for shared memory each (1 x 8192 x 1536 150 -> 132 us); with four states a lane that takes too many registers (61 states, 5 x 1013 x
+      // 1002 142 -> 171)
+      if constexpr (NL < 4) {
+        for (int first = 0; first < W; first += 4) {
+          float po[4][NL], ho[4][NL];
 #pragma unroll
-        for (int j = 0; j < NL; ++j) H[j] = fmaf(po[j], H[j], ho[j]);
-      };
-      for (int o = 0; o < w; ++o) meet(o);
+          for (int k = 0; k < 4; ++k) {
+            const int o = min(first + k, W - 1);
+            load_values<float, NL>(turn + (o * 2 * 64 + lane) * NL, po[k]);
+            load_values<float, NL>(turn + ((o * 2 + 1) * 64 + lane) * NL, ho[k]);
+          }
 #pragma unroll
-      for (int j = 0; j < NL; ++j) start[j] = H[j];
-      for (int o = w; o < W; ++o) meet(o);
+          for (int k = 0; k < 4; ++k) {
+            const bool here = first + k == w, met = first + k < W;
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+              start[j] = here ? H[j] : start[j];
+              H[j] = met ? fmaf(po[k][j], H[j], ho[k][j]) : H[j];
+            }
+          }
+        }
+      } else {
+        const auto meet = [&](int o) {
+          float po[NL], ho[NL];
+          load_values<float, NL>(turn + (o * 2 * 64 + lane) * NL, po);
+          load_values<float, NL>(turn + ((o * 2 + 1) * 64 + lane) * NL, ho);
+#pragma unroll
+          for (int j = 0; j < NL; ++j) H[j] = fmaf(po[j], H[j], ho[j]);
+        };
+        for (int o = 0; o < w; ++o) meet(o);
+#pragma unroll
+        for (int j = 0; j < NL; ++j) start[j] = H[j];
+        for (int o = w; o < W; ++o) meet(o);
+      }
     }
     if (p.saved && t0 % p.apart == 0 && t0 < n && on) {
       float* kept = p.saved + (((long)b * p.parts + t0 / p.apart) * p.channels + ch) * p.N + q * NL;
@@ -305,7 +331,7 @@ size_t fwd_lds(const ScanPlan& s) {
 // Lanes a channel and states a lane.  A wave's sixteen positions cost some 150 instructions for each state of a lane (a product, an exponential at four times the cost of others, a product,
 // three sums), 45 for each position whose x, dt, z and y it moves, a sum across lanes, and 60 for what all waves do; four states a lane leave room for two waves a SIMD instead of
 // three (8 % more).  What counts is the share of the compute unit with most workgroups.  16 states, us, with four / two / one a lane: 1 x 8192 x 1536 225 / 154 / 162 (96, 192,
-// 384 workgroups), 4 x 8192 x 1536 424 / 374 / 532 (384, 768, 1536); 61 states, 5 x 1013 x 1002 143 / 171 / 240.
+// 384 workgroups of eight waves), 4 x 8192 x 1536 424 / 374 / 532 (384, 768, 1536); 61 states, 5 x 1013 x 1002 143 / 171 / 240.
 template <typename SHAPES>
 void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
   const int per_group = D / G, cus = num_cus();
@@ -319,15 +345,15 @@ void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
     if (least == 0 || cost < least) least = cost, r.NS = NS, r.NL = NL, r.blocks = blocks;
   }
 }
-// Waves of a workgroup: eight, where a compute unit has one workgroup; fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there are positions for.
+// Waves of a workgroup: eight, or twelve with two states a lane, where a compute unit has one workgroup (1 x 8192 x 1536 148 us with eight, 132 with twelve); fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there are positions for.
 // us with two / four / eight waves: 1 x 8192 x 1536 (one workgroup a compute unit, two states a lane) 415 / 222 / 154, 4 x 8192 x 1536 (three) 499 / 376 / 473, 8 x 2048 x 1536 (six) with its
 // gradient 717 / 732 / 799; four states a lane, 4 x 8192 x 1536 (two workgroups) 424 with four waves and 457 with eight, 8 x 2048 x 1536 (three) 192 and 171.
 ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<ForwardShapes>(r, B, D, G, N);
   const long share = ((long)r.blocks * G * B + num_cus() - 1) / num_cus();
-  const int room = r.NL == 4 ? 8 : r.NL == 2 ? 12 : 16;
-  r.W = 8;
+  const int room = three_waves(r.NS, r.NL) ? 12 : r.NL == 1 ? 16 : 8;
+  r.W = three_waves(r.NS, r.NL) && share == 1 ? 12 : 8;
   if (r.NL == 4) r.W = share % 2 ? 8 : 4;      // one workgroup at a time fills a compute unit with eight, two with four
   else while (r.W > 2 && r.W * share > room) r.W /= 2;
   while (r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
