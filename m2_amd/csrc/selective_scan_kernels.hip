@@ -307,8 +307,8 @@ int check_scan(const char* name, const ScanArgs& p, int dtype) {
   for (long row : {p.x_row, p.dt_row, p.z_row, p.b_row, p.c_row, p.gy_row})
     if (row < 0 || row >= 1L << 24) return set_error(M2_ERR_UNSUPPORTED, "%s: rows %ld values apart, below 2^24 are supported", name, row);
   if ((long)p.batch * p.L >= (1L << 32) / ((long)p.G * p.N)) return set_error(M2_ERR_ARG, "%s: below 2^32 values of B are supported", name);
-  if (p.channels > 1 << 20 || p.L > 1 << 30 || (long)p.batch * p.channels > 1L << 24)
-    return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^24 channels of all sequences", name);
+  if (p.channels > 1 << 20 || p.L > 1 << 30 || (long)p.batch * p.channels > 1L << 26)
+    return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^26 channels of all sequences", name);
   return M2_OK;
 }
 
@@ -357,7 +357,7 @@ ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
   if (r.NL == 4) r.W = share % 2 ? 8 : 4;      // one workgroup at a time fills a compute unit with eight, two with four
   else while (r.W > 2 && r.W * share > room) r.W /= 2;
   while (r.W > 1 && (r.W / 2) * 16 >= L) r.W /= 2;
-  while (fwd_lds(r) > (80 << 10)) r.W /= 2;
+  while (fwd_lds(r) > (share == 1 ? 150 << 10 : 80 << 10)) r.W /= 2;
   return r;
 }
 // The gradient: sets of channels that a workgroup takes one after the other, so that it writes one partial gradient of B and C for all of them: as many as leave the share of
@@ -524,6 +524,7 @@ extern "C" int m2_selective_scan_step(const m2_scan_inputs* in, void* y, float* 
   const bool wide = p.N % 4 == 0 && m2::aligned16(p.A, p.state, p.state_out);
   const int P = std::min(64, pow2_from(wide ? p.N / 4 : p.N));
   const long groups = ((long)p.batch * p.channels * P + 255) / 256;
+  if (groups >= 1L << 24) return set_error(M2_ERR_ARG, "selective_scan_step: B=%d, D=%d, N=%d are more than a launch holds", p.batch, p.channels, p.N);
   // 64 x 3584 x 64: 35.3 us with one channel a thread, 33.1 (3.6 TB/s) with two, 41 with four
   const int I = groups >= 16L * num_cus() ? 2 : 1;
   const auto launch = [&](auto t) {

@@ -52,7 +52,7 @@ def test_scan_entry_points():
         assert fwd(**{f: None}) == -1 and b"null" in lib.m2_last_error()
     assert fwd(batch=0) == -1 and fwd(length=0) == -1 and fwd(channels=0) == -1 and fwd(groups=3) == -1 and fwd(groups=0) == -1 and fwd(dtype=5) == -1
     assert fwd(states=0) == -2 and fwd(states=257) == -2 and b"257 states" in lib.m2_last_error()
-    assert fwd(channels=(1 << 20) + 1) == -1 and fwd(batch=1 << 20, channels=32) == -1 and fwd(length=1 << 30, batch=32) == -1
+    assert fwd(channels=(1 << 20) + 1) == -1 and fwd(batch=1 << 20, channels=128) == -1 and fwd(length=1 << 30, batch=32) == -1
     g = _lib.ScanGradients()
     assert lib.m2_selective_scan_bwd(_scan(_lib), ctypes.byref(g), _p(), _p(), 0, None) == -1      # no gy
     g.gy = 4096
@@ -61,6 +61,10 @@ def test_scan_entry_points():
     assert lib.m2_selective_scan_bwd(_scan(_lib), None, _p(), _p(), 0, None) == -1
     assert lib.m2_selective_scan_step(_scan(_lib, length=1), _p(), _p(), 0, None) == -1      # no state
     assert lib.m2_selective_scan_step(_scan(_lib, length=1, state=4096), _p(), None, 0, None) == -1
+    assert lib.m2_selective_scan_step(_scan(_lib, length=1, state=4096, batch=1 << 20, channels=64, states=256), _p(), _p(), 0, None) == -1 and b"launch" in lib.m2_last_error()
+    assert fwd(batch=1 << 20, channels=64, states=256) == -1 and b"launch" in lib.m2_last_error()
+    for row in ("x_row", "dt_row", "z_row", "b_row", "c_row"):
+        assert fwd(**{row: 1 << 24}) == -2 and fwd(**{row: -1}) == -2 and b"2^24" in lib.m2_last_error()
     assert [lib.m2_selective_scan_span(n) for n in (0, 257)] == [0, 0]
     for n in (1, 16, 64, 100, 256):
         assert lib.m2_selective_scan_span(n) % 16 == 0 and lib.m2_selective_scan_span(n) >= 32
