@@ -270,17 +270,19 @@ __global__ __launch_bounds__(1024) void sum_partials_kernel(const float* __restr
   __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, planes = last ? K + 1 : K;
   const long width = n * (K + 1), at = blockIdx.x * 64L + lane;
-  float sum = 0.f;
+  float sums[U], sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) sums[u] = 0.f;
   if (at < n * planes) {
     for (long r = w; r < rows; r += 16 * U) {
       float v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = partials[min(r + 16 * u, rows - 1) * width + at];
 #pragma unroll
-      for (int u = 0; u < U; ++u) sum += r + 16 * u < rows ? v[u] : 0.f;
+      for (int u = 0; u < U; ++u) sums[u] += r + 16 * u < rows ? v[u] : 0.f;
     }
   }
-  part[w][lane] = sum;
+  part[w][lane] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
   __syncthreads();
   if (w == 0 && at < n * planes) {
     sum = 0.f;
