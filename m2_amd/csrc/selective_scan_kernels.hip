@@ -362,7 +362,9 @@ ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
 }
 // The gradient: sets of channels that a workgroup takes one after the other, so that it writes one partial gradient of B and C for all of them: as many as leave the share of
 // the compute unit with most of them as it is, and three workgroups for each.  8 x 2048 x 1536 of 16 states, us with the forward: one set 815, two 724, three 759.  More where the
-// partial gradients would take more than 1 GiB and sixteen bytes for each value of x (many states, whose workgroups have few channels a set).
+// partial gradients would take more than 1 GiB and sixteen bytes for each value of x (many states, whose workgroups have few channels a set), as long as each compute unit keeps a workgroup.
+// The gradient alone, ms, with sets for the memory alone / as here / three of them: 1 x 16384 x 1536 of 128 states 41.8 (64 workgroups, 1 GiB) / 14.2 (256, 4) / 11.1 (512, 8);
+// 1 x 8192 x 1536 of 128 11.6 (128, 1) / 7.2 (256, 2) / 5.6 (512, 4); 1 x 32768 x 768 of 64 17.4 (64, 1) / 6.6 (256, 4) / 6.6.
 ScanPlan bwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<GradientShapes>(r, B, D, G, N);
@@ -378,7 +380,7 @@ ScanPlan bwd_plan(int B, int L, int D, int G, int N) {
   const double values = (double)B * L, most = std::max(1073741824.0, 16 * values * D);
   for (int each = r.sets + 1; each <= std::min(64, sets) && 8 * values * r.blocks * G * N > most; ++each) {
     const ScanPlan t{r.NS, r.NL, r.W, (sets + each - 1) / each, each};
-    if (scan_bwd_lds(t) > (160 << 10)) break;
+    if ((long)t.blocks * G * B < cus || scan_bwd_lds(t) > (160 << 10)) break;
     r.blocks = t.blocks, r.sets = each;
   }
   return r;
