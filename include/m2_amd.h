@@ -420,8 +420,8 @@ int m2_token_scores_bwd(const void* logits, int inner, long outer_stride, long r
  *
  * m2_causal_conv_*: x, y (B, L, C), B at most 65535; w (C, K) fp32, the last tap meets the position itself, K 1 .. 8; bias (C) fp32 or NULL; silu 0 or 1; state (B, K - 1, C), the
  * inputs ahead of the first, oldest first, or NULL (zeros); state_out (B, K - 1, C) or NULL: the last K - 1 inputs.  The gradient takes gy and gstate_out (or
- * NULL) and writes gx, gw (C, K) fp32, gb (C) fp32 and gstate, each unless NULL; `workspace`: m2_causal_conv_bwd_workspace_bytes.  The step: x (B, C), y (B, C);
- * state_out may be state. */
+ * NULL) and writes gx, gw (C, K) fp32, gb (C) fp32 and gstate, each unless NULL; `workspace`: m2_causal_conv_bwd_workspace_bytes.  The step: x (B, C), y (B, C),
+ * B up to 2^30 and B C up to 2^31; state_out may be state. */
 int m2_causal_conv_fwd(const void* x, long x_batch, long x_row, const float* w, const float* bias, const void* state, const long long* lengths, void* y,
                        void* state_out, int B, int L, int C, int K, int silu, int dtype, void* stream);
 size_t m2_causal_conv_bwd_workspace_bytes(int B, int L, int C, int K, int dtype);

@@ -34,7 +34,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activa
 
 def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
                      out_state: Optional[Tensor] = None) -> Tensor:
-    """`causal_conv` of one position more: x (B, C) -> (B, C).  `state` (contiguous) moves on in place, or stays and the next one goes to `out_state`."""
+    """`causal_conv` of one position more: x (B, C) -> (B, C), any number of sequences (of 2^31 values of x).  `state` (contiguous) moves on in place, or stays and the next one goes to `out_state`."""
     return ops.causal_conv_step(x, state, weight, bias, activation, out_state)
 
 

@@ -318,8 +318,9 @@ int vector_of(int C, std::initializer_list<const void*> pointers, std::initializ
   return 1;
 }
 
-int check_sizes(const char* name, int B, int L, int C, int K, int dtype) {
-  if (B < 1 || L < 1 || C < 1 || B > 65535) return set_error(M2_ERR_ARG, "%s: B=%d (1 .. 65535), L=%d, C=%d", name, B, L, C);
+// sequences: the most that the call's grid holds
+int check_sizes(const char* name, int B, int L, int C, int K, int dtype, int sequences = 65535) {
+  if (B < 1 || L < 1 || C < 1 || B > sequences) return set_error(M2_ERR_ARG, "%s: B=%d (1 .. %d), L=%d, C=%d", name, B, sequences, L, C);
   if (K < 1 || K > kMaxTaps) return set_error(M2_ERR_UNSUPPORTED, "%s: K=%d taps, 1 .. %d are supported", name, K, kMaxTaps);
   if (dtype != M2_DTYPE_F32 && dtype != M2_DTYPE_BF16) return set_error(M2_ERR_ARG, "%s: dtype %d", name, dtype);
   if (C > 1 << 20 || L > 1 << 30 || (long)B * L > (1L << 36) / C) return set_error(M2_ERR_ARG, "%s: at most 2^20 channels, 2^30 positions and 2^36 values", name);
@@ -442,7 +443,7 @@ extern "C" int m2_causal_conv_bwd(const void* x, long x_batch, long x_row, const
 extern "C" int m2_causal_conv_step(const void* x, long x_batch, const void* state, const float* w, const float* bias, void* y, void* state_out, int B, int C, int K, int silu, int dtype,
                                    void* stream) {
   if (!x || !w || !y || (K > 1 && (!state || !state_out))) return set_error(M2_ERR_ARG, "causal_conv_step: null pointer");
-  if (int rc = check_sizes("causal_conv_step", B, 1, C, K, dtype)) return rc;
+  if (int rc = check_sizes("causal_conv_step", B, 1, C, K, dtype, 1 << 30)) return rc;
   if ((long)B * C > 1L << 31) return set_error(M2_ERR_ARG, "causal_conv_step: at most 2^31 values");
   ConvArgs p{};
   p.x = x, p.x_batch = x_batch, p.w = w, p.bias = bias, p.state = state, p.y = y, p.state_out = state_out;
