@@ -78,6 +78,13 @@ __device__ __forceinline__ T value_to(float v) {
 // The value is made here: one made of a loaded register only later would hold that register over the next load into it, which a loop then waits for.
 __device__ __forceinline__ void made_here(float& v) { asm volatile("" : "+v"(v)); }
 
+// A in powers of two, kept within fp32's range: the positions behind an end have a step of 0, and 0 times an infinity would leave them a state that is no number.
+__device__ __forceinline__ float decay_rate(float A) {
+  constexpr float kMost = 3.402823466e38f;
+  const float r = A * kLog2E;
+  return r < -kMost ? -kMost : r > kMost ? kMost : r;      // (NaN stays)
+}
+
 // A value at a byte offset from what is the same for all lanes: a scalar address and a 32-bit offset.
 template <typename V, typename T>
 __device__ __forceinline__ V& at_offset(T* base, uint32_t bytes) {

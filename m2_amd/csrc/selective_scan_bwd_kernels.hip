@@ -216,7 +216,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
       const float total = lane_sum<NS>(own_total, lane);
       float a[TT][NL], h[TT][NL], last[NL], left[NL], A2[NL];
 #pragma unroll
-      for (int j = 0; j < NL; ++j) last[j] = left[j] = 0.f, A2[j] = A[j] * kLog2E;
+      for (int j = 0; j < NL; ++j) last[j] = left[j] = 0.f, A2[j] = decay_rate(A[j]);
 #pragma unroll
       for (int t4 = 0; t4 < TT; t4 += 4) {
         keep_order();
@@ -356,14 +356,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int t = t0 + i * NS;
-        const float gxv = fmaf(d[i], into[i], skip * u[i]), gd = fmaf(xv[i], into[i], kept[i]) * d_slope[i];
+        const bool inside = t + q0 < n;
+        // (behind the end `kept` is what A makes of a state that stays, which may pass fp32's range)
+        const float gxv = fmaf(d[i], into[i], skip * u[i]), gd = inside ? fmaf(xv[i], into[i], kept[i]) * d_slope[i] : 0.f;
         gD = fmaf(u[i], xv[i], gD);
         gbias += gd;
-        const bool inside = t + q0 < n;
         if (on && moves && t + q0 < p.L) {
           const uint32_t at = off + (uint32_t)(i * NS * sizeof(T)) * (uint32_t)p.channels;
           if (p.gx) at_offset<T>(gx, at) = value_to<T>(inside ? gxv : 0.f);
-          if (p.gdt) at_offset<T>(gdt, at) = value_to<T>(inside ? gd : 0.f);
+          if (p.gdt) at_offset<T>(gdt, at) = value_to<T>(gd);
           if (p.gz) at_offset<T>(gzs, at) = value_to<T>(inside ? gz[i] * fmaf(skip, xv[i], out[i]) : 0.f);
         }
       }

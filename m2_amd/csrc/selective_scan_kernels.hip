@@ -50,7 +50,7 @@ __global__ __launch_bounds__(three_waves(NS, NL) ? 768 : 512) __attribute__((amd
   for (int j = 0; j < NL; ++j) {
     const int at = q * NL + j;
     const bool real = on && at < p.N;
-    A2[j] = real ? p.A[(long)ch * p.N + at] * kLog2E : 0.f;
+    A2[j] = real ? decay_rate(p.A[(long)ch * p.N + at]) : 0.f;
     H[j] = real && p.state ? p.state[((long)b * p.channels + ch) * p.N + at] : 0.f;
   }
   const float bias = p.dt_bias ? p.dt_bias[ch] : 0.f, skip = p.D ? p.D[ch] : 0.f;
@@ -271,10 +271,11 @@ __global__ __launch_bounds__(256) void selective_scan_step_kernel(ScanArgs p, in
     }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      const float step = p.softplus ? softplus(d[i]) : d[i], dx = step * xv[i];
+      // (the step in powers of two and not A, whose product with log2 e may pass fp32's range)
+      const float step = p.softplus ? softplus(d[i]) : d[i], dx = step * xv[i], twos = step * kLog2E;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        hv[i][j] = fmaf(__builtin_amdgcn_exp2f(step * (av[i][j] * kLog2E)), hv[i][j], dx * bv[i][j]);
+        hv[i][j] = fmaf(__builtin_amdgcn_exp2f(twos * av[i][j]), hv[i][j], dx * bv[i][j]);
         sum[i] = fmaf(cv[i][j], hv[i][j], sum[i]);
       }
       if (item[i] <= last) store_values<float, V>(p.state_out + (long)item[i] * p.N + n, hv[i]);
