@@ -17,8 +17,7 @@ struct ScanArgs {
   float* saved;                              // (B, parts, D, N): the state ahead of each part of a sequence, for the gradient, or null
   int batch, L, channels, G, N, softplus;
   int per_group, blocks, parts;              // channels of a group, workgroups for them, parts of a sequence
-  int apart;                                 // positions between the states that are kept
-  int kept_parts;                            // the gradient: how many of those a workgroup's step has
+  int apart;                                 // positions between the states that are kept: a step of the gradient's workgroups
   int sets;                                  // the gradient: sets of 64 / NS channels that a workgroup takes one after the other
   // gradients
   const float* gstate_out;                   // or null
@@ -218,7 +217,6 @@ struct GradientShapes {
 // How a call is spread: lanes a channel, states a lane, waves of a workgroup.
 struct ScanPlan {
   int NS, NL, W, blocks, sets;
-  int positions() const { return W * 16; }      // of a workgroup's step
 };
 
 size_t scan_bwd_lds(const ScanPlan& plan);

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(NL == 2 && 
     rows(rdt, p.dt, p.dt_batch, p.dt_row);
     rows(rg, p.gy, p.gy_batch, p.gy_row);
     rows(rz, p.z ? p.z : p.x, p.z ? p.z_batch : p.x_batch, p.z ? p.z_row : p.x_row);      // (no gate: loads that nothing comes of, rather than waits around a branch)
-    const float* kept = p.saved + ((long)b * p.parts + s * p.kept_parts) * p.channels * p.N;
+    const float* kept = p.saved + ((long)b * p.parts + s) * p.channels * p.N;
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const uint32_t at = (__umul24((uint32_t)ch, (uint32_t)p.N) + (uint32_t)min(q * NL + j, p.N - 1)) * 4u;

@@ -369,7 +369,7 @@ ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
 ScanPlan bwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<GradientShapes>(r, B, D, G, N);
-  r.W = m2_selective_scan_span(N) / 16;
+  r.W = m2_selective_scan_span(N) / 16;      // a step from each state that is kept
   const int sets = r.blocks, cus = num_cus();
   long least = 0;
   for (int each = 1; each <= 8; ++each) {
@@ -507,7 +507,7 @@ extern "C" int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gra
   const ScanPlan plan = bwd_plan(p.batch, p.L, p.channels, p.G, p.N);
   if (int rc = check_grid("selective_scan_bwd", p, plan)) return rc;
   const hipStream_t s = (hipStream_t)stream;
-  p.blocks = plan.blocks, p.sets = plan.sets, p.apart = m2_selective_scan_span(p.N), p.parts = (p.L + p.apart - 1) / p.apart, p.kept_parts = plan.positions() / p.apart;
+  p.blocks = plan.blocks, p.sets = plan.sets, p.apart = m2_selective_scan_span(p.N), p.parts = (p.L + p.apart - 1) / p.apart;
   p.gy = out->gy, p.gy_batch = out->gy_batch, p.gy_row = out->gy_row, p.gstate_out = out->gstate_out;
   p.gx = out->gx, p.gdt = out->gdt, p.gz = out->gz, p.gstate = out->gstate;
   p.saved = const_cast<float*>(saved);
