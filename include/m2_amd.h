@@ -453,6 +453,9 @@ typedef struct m2_scan_gradients {
   float *gA, *gD, *gdt_bias, *gstate;
 } m2_scan_gradients;
 int m2_selective_scan_span(int states);
+/* How a call of these sizes is spread (backward: its gradient), for tests and profiles: plan[0 .. 4] = lanes a channel, states a lane, waves of a workgroup (16 positions each), workgroups, and
+ * sets of 64 / lanes channels that a workgroup takes one after the other. */
+int m2_selective_scan_plan(int batch, int length, int channels, int groups, int states, int backward, int* plan);
 int m2_selective_scan_fwd(const m2_scan_inputs* in, void* y, float* state_out, float* saved, int dtype, void* stream);
 size_t m2_selective_scan_bwd_workspace_bytes(int batch, int length, int channels, int groups, int states);
 int m2_selective_scan_bwd(const m2_scan_inputs* in, const m2_scan_gradients* out, const float* saved, void* workspace, int dtype, void* stream);

@@ -191,6 +191,8 @@ def _load() -> ctypes.CDLL:
     lib.m2_causal_conv_step.argtypes = [c_void_p, c_long] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p]
     lib.m2_selective_scan_span.restype = c_int
     lib.m2_selective_scan_span.argtypes = [c_int]
+    lib.m2_selective_scan_plan.restype = c_int
+    lib.m2_selective_scan_plan.argtypes = [c_int] * 6 + [POINTER(c_int)]
     lib.m2_selective_scan_fwd.restype = c_int
     lib.m2_selective_scan_fwd.argtypes = [POINTER(ScanInputs)] + [c_void_p] * 3 + [c_int, c_void_p]
     lib.m2_selective_scan_bwd_workspace_bytes.restype = c_size_t
@@ -216,7 +218,7 @@ EXPORTS = ["m2_version", "m2_last_error", "m2_hyena_filter_workspace_bytes", "m2
            "m2_embed_layernorm_fwd", "m2_blockdiag_linear_layernorm_supported", "m2_blockdiag_linear_layernorm_fwd", "m2_encoder_layers_workspace_bytes", "m2_encoder_layers_fwd", "m2_encoder_layers_taps_fwd",
            "m2_split_bytes", "m2_split_rows_fwd", "m2_split_jobs_fwd", "m2_split_channels_fwd", "m2_split_to_channels_fwd", "m2_split_linear_fwd", "m2_split_glu_fwd",
            "m2_int4_weight_bytes", "m2_int4_workspace_bytes", "m2_int4_linear_fwd", "m2_token_scores_workspace_bytes", "m2_token_scores_fwd", "m2_token_scores_bwd",
-           "m2_causal_conv_fwd", "m2_causal_conv_bwd_workspace_bytes", "m2_causal_conv_bwd", "m2_causal_conv_step", "m2_selective_scan_span", "m2_selective_scan_fwd",
+           "m2_causal_conv_fwd", "m2_causal_conv_bwd_workspace_bytes", "m2_causal_conv_bwd", "m2_causal_conv_step", "m2_selective_scan_span", "m2_selective_scan_plan", "m2_selective_scan_fwd",
            "m2_selective_scan_bwd_workspace_bytes", "m2_selective_scan_bwd", "m2_selective_scan_step", "m2_group_norm_workspace_bytes", "m2_group_norm_fwd", "m2_group_norm_bwd"]
 
 

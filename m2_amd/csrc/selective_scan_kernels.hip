@@ -464,6 +464,17 @@ bool given(const ScanArgs& p) { return p.x && p.dt && p.Bm && p.Cm && p.A; }
 
 }  // namespace
 
+extern "C" int m2_selective_scan_plan(int batch, int length, int channels, int groups, int states, int backward, int* plan) {
+  if (!plan) return set_error(M2_ERR_ARG, "selective_scan_plan: null pointer");
+  ScanArgs p{};
+  p.batch = batch, p.L = length, p.channels = channels, p.G = groups, p.N = states;
+  if (int rc = check_scan("selective_scan_plan", p, M2_DTYPE_F32)) return rc;
+  const ScanPlan r = (backward ? bwd_plan : fwd_plan)(batch, length, channels, groups, states);
+  if (int rc = check_grid("selective_scan_plan", p, r)) return rc;
+  plan[0] = r.NS, plan[1] = r.NL, plan[2] = r.W, plan[3] = r.blocks * groups * batch, plan[4] = backward ? r.sets : 1;
+  return M2_OK;
+}
+
 extern "C" int m2_selective_scan_fwd(const m2_scan_inputs* in, void* y, float* state_out, float* saved, int dtype, void* stream) {
   ScanArgs p{};
   if (in) fill(p, in);

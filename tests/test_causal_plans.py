@@ -18,3 +18,35 @@ def test_scan_gradient_keeps_a_workgroup_for_each_compute_unit(batch, length, ch
     lanes = max(4, 1 << (-(-states // 2) - 1).bit_length())
     most = groups * batch * -(-(channels // groups) // max(1, 64 // min(lanes, 64)))
     assert _workgroups(batch, length, channels, groups, states) >= min(256, most)
+
+
+def _plan(batch, length, channels, groups, states, backward):
+    import ctypes
+    from m2_amd._lib import lib
+    found = (ctypes.c_int * 5)()
+    assert lib.m2_selective_scan_plan(batch, length, channels, groups, states, backward, found) == 0
+    return list(found)
+
+
+def test_scan_plans():
+    """A workgroup's waves lie within a launch's limits, its lanes hold all states, and all channels have a workgroup; the gradient's workspace holds what its workgroups write."""
+    for batch in (1, 3, 40, 700):
+        for length in (1, 17, 100, 8192):
+            for channels, groups in ((1, 1), (24, 8), (768, 1), (1536, 2), (1919, 1), (4096, 4)):
+                for states in (1, 2, 3, 5, 16, 24, 61, 64, 100, 128, 200, 256):
+                    if batch * length * groups * states >= 2 ** 32:      # (refused)
+                        continue
+                    for backward in (0, 1):
+                        lanes, each, waves, workgroups, sets = _plan(batch, length, channels, groups, states, backward)
+                        assert lanes & (lanes - 1) == 0 and 1 <= lanes <= 64 and each in (1, 2, 4) and lanes * each >= states and 1 <= waves <= 12 and sets >= 1
+                        assert workgroups == batch * groups * -(-(channels // groups) // (64 // lanes * sets))
+                    assert _workgroups(batch, length, channels, groups, states) == workgroups
+
+
+def test_scan_plan_refusals():
+    import ctypes
+    from m2_amd._lib import lib
+    found = (ctypes.c_int * 5)()
+    assert lib.m2_selective_scan_plan(1, 8, 16, 1, 4, 0, None) == -1 and lib.m2_selective_scan_plan(1, 8, 16, 3, 4, 0, found) == -1
+    assert lib.m2_selective_scan_plan(0, 8, 16, 1, 4, 1, found) == -1 and lib.m2_selective_scan_plan(1, 8, 16, 1, 257, 1, found) == -2
+    assert lib.m2_selective_scan_plan(1 << 20, 8, 64, 1, 256, 0, found) == -1
