@@ -221,7 +221,7 @@ struct Place {
 __device__ __forceinline__ void join(float& mean, float& m2, float total, float other_mean, float other_m2, float count) {
   const float d = other_mean - mean, share = count / (total + count);
   mean = fmaf(d, share, mean);
-  m2 += fmaf(d * d, total * share, other_m2);
+  m2 += fmaf(d, d * (total * share), other_m2);      // (a first block's d is its mean, whose square may pass fp32's range; total is 0 there)
 }
 
 template <typename T, int V>
