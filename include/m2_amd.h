@@ -418,7 +418,7 @@ int m2_token_scores_bwd(const void* logits, int inner, long outer_stride, long r
  * tensors given as void*.  Tensors are dense unless a batch and row distance (in values) is given; a row's values always lie one behind the other.  `lengths`
  * (B) on the GPU, or NULL: sequence b ends at lengths[b] (taken as 0 .. L); positions behind it are not read, outputs and gradients there are 0.
  *
- * m2_causal_conv_*: x, y (B, L, C), B at most 65535; w (C, K) fp32, the last tap meets the position itself, K 1 .. 8; bias (C) fp32 or NULL; silu 0 or 1; state (B, K - 1, C), the
+ * m2_causal_conv_*: x, y (B, L, C), B at most 65535, C up to 2^20, 2^36 values; w (C, K) fp32, the last tap meets the position itself, K 1 .. 8; bias (C) fp32 or NULL; silu 0 or 1; state (B, K - 1, C), the
  * inputs ahead of the first, oldest first, or NULL (zeros); state_out (B, K - 1, C) or NULL: the last K - 1 inputs.  The gradient takes gy and gstate_out (or
  * NULL) and writes gx, gw (C, K) fp32, gb (C) fp32 and gstate, each unless NULL; `workspace`: m2_causal_conv_bwd_workspace_bytes.  The step: x (B, C), y (B, C),
  * B up to 2^30 and B C up to 2^31; state_out may be state. */
@@ -433,7 +433,8 @@ int m2_causal_conv_step(const void* x, long x_batch, const void* state, const fl
 
 /* The scan:  d = dt + dt_bias, softplus of it if asked for;  h[t] = exp(d A) h[t - 1] + d B[t] x[t];  y[t] = (sum_n C[t, n] h[t, n] + D x[t]) silu(z[t]).
  * x, dt, z (or NULL), y (batch, length, channels); B, C (batch, length, groups, states), a group serving channels / groups neighbouring channels; A
- * (channels, states), D, dt_bias (channels) or NULL and state (batch, channels, states) or NULL (zeros) fp32; states 1 .. 256; rows below 2^24 values apart.
+ * (channels, states), D, dt_bias (channels) or NULL and state (batch, channels, states) or NULL (zeros) fp32; states 1 .. 256; rows below 2^24 values apart;
+ * channels up to 2^20, of all sequences 2^26, length up to 2^30, values of B below 2^32.
  * state_out (batch, channels, states) or NULL: the states behind the last position.  `saved`, for the gradient, or NULL: fp32
  * (batch, ceil(length / m2_selective_scan_span), channels, states).  The gradient takes gy and gstate_out (or NULL) and writes all of m2_scan_gradients that
  * are not NULL, B and C's dense (batch, length, groups, states), of dtype, the others of their inputs' types; `workspace`: m2_selective_scan_bwd_workspace_bytes.
@@ -464,7 +465,8 @@ int m2_selective_scan_step(const m2_scan_inputs* in, void* y, float* state_out, 
 /* Group norm: x (N, S, C), mean and biased variance over the S positions and each of G groups of neighbouring channels, y = act((x - mean) rstd w + b); w, b
  * (C) fp32 or NULL; act 0 none, 1 SiLU, 2 erf-GELU.  stats (N, G, 2) fp32 (mean, rstd) is written and the gradient's input.  x and gy: rows of C one behind
  * the other, a sample N and a position S apart as given.  The gradient writes gx (dense), gw and gb (C) fp32, each unless NULL.  Workspaces:
- * m2_group_norm_workspace_bytes (0: NULL does). */
+ * m2_group_norm_workspace_bytes (0: NULL does).  C up to 2^20, S up to 2^30, 2^36 values; with several positions, or one and groups of more than 256 vectors (16
+ * bytes where C / G and all addresses are multiples of them, else two values or one), N G and N times the chunks of a sample (16 positions or more each) below 2^24. */
 size_t m2_group_norm_workspace_bytes(long N, int S, int C, int G, int backward, int dtype);
 int m2_group_norm_fwd(const void* x, long x_sample, long x_row, const float* w, const float* b, float eps, void* y, float* stats, void* workspace, long N, int S,
                       int C, int G, int act, int dtype, void* stream);

@@ -49,7 +49,8 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Op
     (channels).  `state` (B, channels, N): the states ahead of the first position (None: zeros).  `lengths` as in `causal_conv`.  With `return_state`:
     (y, state), the states behind each sequence's last position.
 
-    Positions are worked on side by side, so results differ in rounding from one step after another, and so do states beyond fp32's range."""
+    Positions are worked on side by side, so results differ in rounding from one step after another, and so do states beyond fp32's range.  At most 2^20 channels, 2^26 of all
+    sequences, and below 2^32 values of B."""
     y, last = ops.selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, return_state)
     return (y, last) if return_state else y
 
@@ -65,5 +66,6 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     """act((x - mean) / sqrt(var + eps) * weight + bias) of x (N, ..., C), mean and (biased) variance of each sample over all positions between the first and the last
     dimension and over each of `groups` groups of neighbouring channels; weight, bias (C); `activation` None, "silu" or "gelu" (erf).
 
-    (tokens, C) normalises each token by itself, heads of channels say; (B, L, C) whole sequences, padding included."""
+    (tokens, C) normalises each token by itself, heads of channels say; (B, L, C) whole sequences, padding included.  At most 2^20 channels and 2^36 values, and below 2^24
+    groups of all sequences, or of all tokens where a group passes 1024 fp32 or 2048 bf16 channels (256 where sizes or addresses are odd)."""
     return ops.group_norm(x, groups, weight, bias, eps, activation)

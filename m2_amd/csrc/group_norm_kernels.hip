@@ -3,7 +3,9 @@
 //   a sample's group: S positions times Cg channels     m = mean x     r = 1 / sqrt(mean (x - m)^2 + eps)     xh = (x - m) r     pre = xh w + b     y = act(pre)
 //   g = gy act'(pre)     t = g w     gx = r (t - mean t - xh mean(t xh))     gw = sum g xh     gb = sum g
 //
-// One position (groups of a token): P neighbouring lanes hold a group in registers, read once.  More: the values are read twice, first for means and squared distances
+// One position (groups of a token): P neighbouring lanes hold a group in registers, read once, up to 256 of the vectors that a lane moves (16 bytes where a group's channels and all addresses are
+// multiples of it, else two values or one).  Wider groups of one position go with those of several, whose threads then mostly have nothing to do: 8192 x 1024 fp32 in one group with SiLU 22 us (74 with
+// the gradient), 8192 x 1536 fp32 147 (447), 8192 x 3584 bf16 470 (1490), 8192 x 1002 bf16 in ones 182 (431).  Several: the values are read twice, first for means and squared distances
 // of small blocks, joined with what their means differ by, so that nothing cancels; second for the result.
 //
 // Bound by memory: 32768 x 1536 bf16 in 24 groups with SiLU 51 us (3.9 TB/s).  8 x 2048 x 1536 with its gradient 107 us: x twice, gy and x twice more, 0.4 GB of reads and writes at 3.8 TB/s, part of

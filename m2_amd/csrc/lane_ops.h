@@ -117,7 +117,8 @@ __device__ __forceinline__ float lane_sum(float v, int lane) {
 
 constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// exp(x), x <= 88, to about 2^-23 of itself: the product with log2 e in two parts, of which the second is a factor near 1.  Below -100: as at -100 (NaN too).
+// exp(x), x <= 88, to about 2^-23 of itself: the product with log2 e in two parts, of which the second is a factor near 1 (1.925963033500e-8 is log2 e less its fp32 rounding, kLog2E).  Below -100: as
+// at -100 (NaN too).
 __device__ __forceinline__ float exp_of(float x) {
   x = fmaxf(x, -100.f);
   const float hi = x * kLog2E;
@@ -125,15 +126,16 @@ __device__ __forceinline__ float exp_of(float x) {
   const float e = __builtin_amdgcn_exp2f(hi);
   return fmaf(e, lo * kLn2, e);
 }
-// x / (1 + exp(-x)), for a result of type T: the exponential of a bf16 result has its argument as it is rounded (off by |x| 2^-23 of itself at most, against bf16's 2^-8), which saves six
-// of eleven instructions.
+// x / (1 + exp(-x)) among values of type T: with bf16 the exponential has its argument as it is rounded (off by |x| 2^-23 of itself at most, against the 2^-8 of a bf16 value), which saves six of
+// eleven instructions.  The same goes for the slopes below, which also are factors of fp32 results (with bf16 hidden states: the gradients of the convolution's and group norm's weights and biases, and of
+// a gated scan's A, D, dt_bias and state): each of their terms is off by |x| 2^-23 of itself more, a fraction of what the bf16 value in it was rounded by.
 template <typename T>
 __device__ __forceinline__ float silu(float x) {
   const float e = sizeof(T) == 2 ? __builtin_amdgcn_exp2f(x * -kLog2E) : exp_of(fminf(-x, 88.f));
   return x * __builtin_amdgcn_rcpf(1.f + e);
 }
 // u = exp(-|x|) and r = 1 / (1 + u): what sigmoid(x), sigmoid(-x), softplus(x) and their products are made of, without cancellation.
-// EXACT: the exponential to 2^-23 of itself; else, for what ends in bf16, as in silu.
+// EXACT: the exponential to 2^-23 of itself; else, for bf16 hidden states, as in silu.
 template <bool EXACT>
 struct Logistic {
   float u, r;

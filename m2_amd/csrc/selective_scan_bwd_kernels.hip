@@ -11,7 +11,7 @@
 // memory; the sums of a workgroup go to memory for scan_join_kernel.  All in a fixed order.
 //
 // Bound by vector instructions (82 % of the cycles): 17 for each state and position, 9 in the trees' sums across lanes, 5 for each lane's own positions.  8 x 2048 x 1536, bf16, 16 states: 462 us of the
-// 668 that forward and gradient take, 404 MB in 79.  Partial gradients of B and C are 2 x 100 MB (two sets a workgroup; 52 us to join them).  Registers: loads of four positions' shared values at a time, and
+// 668 that forward and gradient take, 404 MB in 79.  Partial gradients of B and C are 2 x 100 MB (two sets a workgroup; 34 us to join them).  Registers: loads of four positions' shared values at a time, and
 // arguments read anew where they are used (236 -> 162, three waves a SIMD; 436 moves of spilled scalars gone).
 #include <hip/hip_runtime.h>
 #include <stdint.h>

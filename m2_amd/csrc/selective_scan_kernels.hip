@@ -9,10 +9,11 @@
 // state it starts with and runs over its kept decays once more, now with the right state, for the outputs.  Positions are thus worked on side by side, at one more
 // operation a state than one position after another takes, and the decays' exponentials, four times as costly as the others, are formed once.
 //
-// Bound by vector instructions: nine issue slots of a state and position (product, exponential, product, three sums) and six more for all else, of which the step size's softplus and the gate are
-// half, shared memory being busy 60 % of that time.  bf16, 16 states: 4 x 8192 x 1536 365 us, where bytes would take 79; 1 x 8192 x 1536 134 (192 workgroups for 256 compute units); fp32, 61 states,
-// 5 x 1013 x 1002 142.  A loop must not wait for its prefetch: a choice between two loads, or a value that is made of a loaded register only later, made the compiler move registers at once
-// (4 x 8192 x 1536 464 -> 374 us without).  Addresses are a scalar and 32 bits of a lane: in 64 bits they were a tenth of all instructions.
+// Bound by vector instructions (82 % of the cycles at 4 x 8192 x 1536, shared memory 38 %): nine issue slots of a state and position (product, exponential, product, three sums) and six more for
+// all else, of which the step size's softplus and the gate are half.  bf16, 16 states: 4 x 8192 x 1536 350 - 365 us over several machines, where bytes would take 79; 1 x 8192 x 1536 128 - 134 (192
+// workgroups for 256 compute units); fp32, 61 states, 5 x 1013 x 1002 140, with a sequence's lengths as without: neighbouring workgroups are one sequence's and lie on one XCD, so a padded batch takes as
+// long as an XCD with the longest sequences does (38 % busy then).  A loop must not wait for its prefetch: a choice between two loads, or a value that is made of a loaded register only later, made the
+// compiler move registers at once (4 x 8192 x 1536 464 -> 374 us without).  Addresses are a scalar and 32 bits of a lane: in 64 bits they were a tenth of all instructions.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -152,8 +153,8 @@ __global__ __launch_bounds__(three_waves(NS, NL) ? 768 : 512) __attribute__((amd
       store_values<float, NL>(turn + (w * 2 * 64 + lane) * NL, P);
       store_values<float, NL>(turn + ((w * 2 + 1) * 64 + lane) * NL, h);
       __syncthreads();      // (two turns: what is written next is read behind the next barrier)
-      // four at a time, since one after another would wait for shared memory each (1 x 8192 x 1536 150 -> 132 us); with four states a lane that takes too many registers (61 states, 5 x 1013 x
-      // 1002 142 -> 171)
+      // four at a time, since one after another would wait for shared memory each (1 x 8192 x 1536 139 -> 128 us with twelve waves, 4 x 8192 x 1536 362 -> 350 with four); with four states a lane that
+      // takes too many registers (61 states, 5 x 1013 x 1002 142 -> 171)
       if constexpr (NL < 4) {
         for (int first = 0; first < W; first += 4) {
           float po[4][NL], ho[4][NL];
@@ -331,8 +332,8 @@ size_t fwd_lds(const ScanPlan& s) {
 
 // Lanes a channel and states a lane.  A wave's sixteen positions cost some 150 instructions for each state of a lane (a product, an exponential at four times the cost of others, a product,
 // three sums), 45 for each position whose x, dt, z and y it moves, a sum across lanes, and 60 for what all waves do; four states a lane leave room for two waves a SIMD instead of
-// three (8 % more).  What counts is the share of the compute unit with most workgroups.  16 states, us, with four / two / one a lane: 1 x 8192 x 1536 225 / 154 / 162 (96, 192,
-// 384 workgroups of eight waves), 4 x 8192 x 1536 424 / 374 / 532 (384, 768, 1536); 61 states, 5 x 1013 x 1002 143 / 171 / 240.
+// three (8 % more).  What counts is the share of the compute unit with most workgroups.  us with four / two / one a lane, each with its best number of waves: 16 states, 1 x 8192 x 1536 218 / 128 / 161
+// (96, 192, 384 workgroups), 4 x 8192 x 1536 418 / 350 / 505 (384, 768, 1536), 8 x 2048 x 1536 174 / 164 / - (the rule takes four); 61 states, 5 x 1013 x 1002 140 / 198 / 231.
 template <typename SHAPES>
 void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
   const int per_group = D / G, cus = num_cus();
@@ -346,9 +347,9 @@ void choose_shape(ScanPlan& r, int B, int D, int G, int N) {
     if (least == 0 || cost < least) least = cost, r.NS = NS, r.NL = NL, r.blocks = blocks;
   }
 }
-// Waves of a workgroup: eight, or twelve with two states a lane, where a compute unit has one workgroup (1 x 8192 x 1536 148 us with eight, 132 with twelve); fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there are positions for.
-// us with two / four / eight waves: 1 x 8192 x 1536 (one workgroup a compute unit, two states a lane) 415 / 222 / 154, 4 x 8192 x 1536 (three) 499 / 376 / 473, 8 x 2048 x 1536 (six) with its
-// gradient 717 / 732 / 799; four states a lane, 4 x 8192 x 1536 (two workgroups) 424 with four waves and 457 with eight, 8 x 2048 x 1536 (three) 192 and 171.
+// Waves of a workgroup: eight, or twelve with two states a lane, where a compute unit has one workgroup; fewer, down to two, where more share its registers (two or three waves a SIMD); as many as there
+// are positions for.  us with two / four / eight / twelve waves and two states a lane: 1 x 8192 x 1536 (one workgroup a compute unit) 395 / 213 / 143 / 128, 4 x 8192 x 1536 (three) 499 / 350 / 438,
+// 8 x 2048 x 1536 (six) 164 / 166 / 226; four states a lane with four / eight: 4 x 8192 x 1536 (two workgroups) 418 / 446, 8 x 2048 x 1536 (three) 184 / 174.
 ScanPlan fwd_plan(int B, int L, int D, int G, int N) {
   ScanPlan r{};
   choose_shape<ForwardShapes>(r, B, D, G, N);
